@@ -2,8 +2,8 @@
 //
 // Host-side bookkeeping only: argument validation with the reference's
 // contract, device buffers, row metadata upload, launch planning.  All
-// arithmetic on the attention path runs in the HIP kernels of attn_fwd.hip
-// and kv_cache.hip; there is no CPU fallback.  If no GPU is visible every
+// arithmetic on the attention path runs in the HIP kernels of the kernel
+// sources beside it; there is no CPU fallback.  If no GPU is visible every
 // compute entry point fails with DR_ERR_NO_DEVICE.
 #include "dr_attn.h"
 
@@ -186,6 +186,8 @@ struct dr_step_cache {
     std::vector<int> hkv, hd, hd_tile;
     std::vector<uint16_t*> k, vt;  // [layer * n_batch + batch]
     std::vector<uint16_t*> klo, vlo;  // lo halves of K and V^T (DR_PRECISION_HILO layers), else nullptr
+    // DR_PRECISION_FP8 layers: code planes and scale bytes (then k, vt, klo and vlo are nullptr), else nullptr
+    std::vector<uint8_t*> k8, v8, sc;
     std::vector<Slot> slot;
     int32_t* h_meta = nullptr;     // [6] split results, pinned host memory the kernel writes
     int32_t* h_meta_dev = nullptr; // its device address
@@ -444,8 +446,8 @@ int dr_ctx_set_wave_rows(dr_ctx* ctx, int rows) {
 
 int dr_ctx_set_kernel(dr_ctx* ctx, int kernel) {
     if (!ctx) return fail(DR_ERR_INVALID, "dr_ctx_set_kernel: ctx is NULL");
-    if (kernel < DR_KERNEL_AUTO || kernel > DR_KERNEL_HILO)
-        return fail(DR_ERR_INVALID, "kernel %d not DR_KERNEL_AUTO, _STAGED, _STREAMS or _HILO", kernel);
+    if (kernel < DR_KERNEL_AUTO || kernel > DR_KERNEL_FP8)
+        return fail(DR_ERR_INVALID, "kernel %d not DR_KERNEL_AUTO, _STAGED, _STREAMS, _HILO or _FP8", kernel);
     ctx->force_kernel = kernel;
     return DR_OK;
 }
@@ -535,8 +537,70 @@ void dr_pass_destroy(dr_pass* pass) {
 
 // ---------------------------------------------------------------- cache
 
-int dr_cache_create(dr_ctx* ctx, size_t n_total, size_t n_layer, const size_t* n_head_kv,
-                    const size_t* head_dim, size_t n_batch, dr_step_cache** out) {
+extern "C++" {
+namespace {
+
+bool precision_ok(int precision) {
+    return precision == DR_PRECISION_BF16 || precision == DR_PRECISION_HILO || precision == DR_PRECISION_FP8;
+}
+
+// The planes that a layer of some precision keeps per batch slot, and where
+// each is held; bytes of one of them.
+struct Plane {
+    std::vector<uint16_t*>* p16;
+    std::vector<uint8_t*>* p8;
+    size_t bytes;
+    void* get(size_t i) const { return p16 ? static_cast<void*>((*p16)[i]) : (*p8)[i]; }
+    void set(size_t i, void* p) const {
+        if (p16)
+            (*p16)[i] = static_cast<uint16_t*>(p);
+        else
+            (*p8)[i] = static_cast<uint8_t*>(p);
+    }
+};
+
+std::vector<Plane> planes_of(dr_step_cache* c, size_t layer, int precision) {
+    const size_t values = (size_t)c->hkv[layer] * c->cap * c->hd_tile[layer];
+    if (precision == DR_PRECISION_FP8)
+        return {{nullptr, &c->k8, values},
+                {nullptr, &c->v8, values},
+                {nullptr, &c->sc, (size_t)c->hkv[layer] * c->cap * 2}};
+    std::vector<Plane> v = {{&c->k, nullptr, 2 * values}, {&c->vt, nullptr, 2 * values}};
+    if (precision == DR_PRECISION_HILO) {
+        v.push_back({&c->klo, nullptr, 2 * values});
+        v.push_back({&c->vlo, nullptr, 2 * values});
+    }
+    return v;
+}
+
+// Allocates (zeroed) what of a layer's planes for `precision` is not there
+// yet.  On failure what this call allocated is freed again.
+int add_planes(dr_step_cache* c, size_t layer, int precision, const char* what) {
+    std::vector<std::pair<Plane, size_t>> made;
+    hipError_t e = hipSuccess;
+    for (const Plane& pl : planes_of(c, layer, precision))
+        for (size_t i = layer * c->n_batch; e == hipSuccess && i < (layer + 1) * c->n_batch; ++i) {
+            if (pl.get(i)) continue;
+            void* p = nullptr;
+            e = dev_malloc(&p, pl.bytes);
+            if (e != hipSuccess) break;
+            pl.set(i, p);
+            made.push_back({pl, i});
+            // (on the context's own stream and waited for: its calls run on
+            // streams that the null stream does not order)
+            e = hipMemsetAsync(p, 0, pl.bytes, c->ctx->own);
+        }
+    if (e == hipSuccess) e = hipStreamSynchronize(c->ctx->own);
+    if (e == hipSuccess) return DR_OK;
+    for (auto& m : made) {
+        (void)hipFree(m.first.get(m.second));
+        m.first.set(m.second, nullptr);
+    }
+    return hip_fail(e, what);
+}
+
+int create_cache(dr_ctx* ctx, size_t n_total, size_t n_layer, const size_t* n_head_kv, const size_t* head_dim,
+                 const int* precision, size_t n_batch, dr_step_cache** out) {
     if (!ctx || !out) return fail(DR_ERR_INVALID, "dr_cache_create: NULL argument");
     *out = nullptr;
     if (n_layer > 0 && (!n_head_kv || !head_dim))
@@ -560,10 +624,8 @@ int dr_cache_create(dr_ctx* ctx, size_t n_total, size_t n_layer, const size_t* n
     c->cap = round_up(std::max(n_total, (size_t)1), dr::KEY_ALIGN);
     c->n_layer = n_layer;
     c->n_batch = n_batch;
-    c->k.assign(n_layer * n_batch, nullptr);
-    c->vt.assign(n_layer * n_batch, nullptr);
-    c->klo.assign(n_layer * n_batch, nullptr);
-    c->vlo.assign(n_layer * n_batch, nullptr);
+    for (auto* v : {&c->k, &c->vt, &c->klo, &c->vlo}) v->assign(n_layer * n_batch, nullptr);
+    for (auto* v : {&c->k8, &c->v8, &c->sc}) v->assign(n_layer * n_batch, nullptr);
     c->slot.resize(n_batch);
     for (auto& s : c->slot) {
         s.prev_seq.assign(n_total, -1);
@@ -573,20 +635,25 @@ int dr_cache_create(dr_ctx* ctx, size_t n_total, size_t n_layer, const size_t* n
         c->hkv.push_back((int)n_head_kv[l]);
         c->hd.push_back((int)head_dim[l]);
         c->hd_tile.push_back(hd_tile_for(head_dim[l]));
-        const size_t bytes = (size_t)n_head_kv[l] * c->cap * c->hd_tile[l] * sizeof(uint16_t);
-        for (size_t b = 0; b < n_batch; ++b) {
-            for (uint16_t** dst : {&c->k[l * n_batch + b], &c->vt[l * n_batch + b]}) {
-                hipError_t e = dev_malloc(reinterpret_cast<void**>(dst), bytes);
-                if (e == hipSuccess) e = hipMemset(*dst, 0, bytes);
-                if (e != hipSuccess) {
-                    dr_cache_destroy(c);
-                    return hip_fail(e, "KV cache allocation");
-                }
-            }
+    }
+    for (size_t l = 0; l < n_layer; ++l) {
+        const int rc = add_planes(c, l, precision ? precision[l] : DR_PRECISION_BF16, "KV cache allocation");
+        if (rc != DR_OK) {
+            const std::string msg = g_err;
+            dr_cache_destroy(c);
+            return fail(rc, "%s", msg.c_str());
         }
     }
     *out = c;
     return DR_OK;
+}
+
+}  // namespace
+}  // extern "C++"
+
+int dr_cache_create(dr_ctx* ctx, size_t n_total, size_t n_layer, const size_t* n_head_kv,
+                    const size_t* head_dim, size_t n_batch, dr_step_cache** out) {
+    return create_cache(ctx, n_total, n_layer, n_head_kv, head_dim, nullptr, n_batch, out);
 }
 
 int dr_cache_create_layers(dr_ctx* ctx, size_t n_total, size_t n_layer, const size_t* n_head_kv,
@@ -594,36 +661,22 @@ int dr_cache_create_layers(dr_ctx* ctx, size_t n_total, size_t n_layer, const si
                            dr_step_cache** out) {
     if (precision)
         for (size_t l = 0; l < n_layer; ++l)
-            if (precision[l] != DR_PRECISION_BF16 && precision[l] != DR_PRECISION_HILO)
-                return fail(DR_ERR_INVALID, "layer %zu: precision %d not DR_PRECISION_BF16 or _HILO", l,
+            if (!precision_ok(precision[l]))
+                return fail(DR_ERR_INVALID, "layer %zu: precision %d not DR_PRECISION_BF16, _HILO or _FP8", l,
                             precision[l]);
-    DR_CHECK(dr_cache_create(ctx, n_total, n_layer, n_head_kv, head_dim, n_batch, out));
-    if (precision)
-        for (size_t l = 0; l < n_layer; ++l) {
-            if (precision[l] == DR_PRECISION_BF16) continue;
-            const int rc = dr_cache_set_precision(*out, l, precision[l]);
-            if (rc != DR_OK) {
-                const std::string msg = g_err;
-                dr_cache_destroy(*out);
-                *out = nullptr;
-                return fail(rc, "%s", msg.c_str());
-            }
-        }
-    return DR_OK;
+    return create_cache(ctx, n_total, n_layer, n_head_kv, head_dim, precision, n_batch, out);
 }
 
 void dr_cache_destroy(dr_step_cache* cache) {
     if (!cache) return;
     (void)hipSetDevice(cache->ctx->device);
     (void)hipStreamSynchronize(cache->ctx->stream);
-    for (uint16_t* p : cache->k)
-        if (p) (void)hipFree(p);
-    for (uint16_t* p : cache->vt)
-        if (p) (void)hipFree(p);
-    for (uint16_t* p : cache->klo)
-        if (p) (void)hipFree(p);
-    for (uint16_t* p : cache->vlo)
-        if (p) (void)hipFree(p);
+    for (auto* v : {&cache->k, &cache->vt, &cache->klo, &cache->vlo})
+        for (uint16_t* p : *v)
+            if (p) (void)hipFree(p);
+    for (auto* v : {&cache->k8, &cache->v8, &cache->sc})
+        for (uint8_t* p : *v)
+            if (p) (void)hipFree(p);
     for (auto& s : cache->slot) {
         if (s.d_prev) (void)hipFree(s.d_prev);
         if (s.d_lc) (void)hipFree(s.d_lc);
@@ -638,30 +691,28 @@ int dr_cache_set_precision(dr_step_cache* cache, size_t layer, int precision) {
     if (!cache) return fail(DR_ERR_INVALID, "dr_cache_set_precision: cache is NULL");
     if (layer >= cache->n_layer)
         return fail(DR_ERR_INVALID, "dr_cache_set_precision: layer %zu >= %zu", layer, cache->n_layer);
-    if (precision != DR_PRECISION_BF16 && precision != DR_PRECISION_HILO)
-        return fail(DR_ERR_INVALID, "dr_cache_set_precision: precision %d is not DR_PRECISION_BF16 (0) or "
-                    "DR_PRECISION_HILO (1)", precision);
+    if (!precision_ok(precision))
+        return fail(DR_ERR_INVALID, "dr_cache_set_precision: precision %d is not DR_PRECISION_BF16 (0), "
+                    "DR_PRECISION_HILO (1) or DR_PRECISION_FP8 (2)", precision);
     DR_CHECK(use_device(cache->ctx));
-    const size_t bytes = (size_t)cache->hkv[layer] * cache->cap * cache->hd_tile[layer] * sizeof(uint16_t);
-    for (size_t b = 0; b < cache->n_batch; ++b) {
-        for (uint16_t** plo : {&cache->klo[layer * cache->n_batch + b], &cache->vlo[layer * cache->n_batch + b]}) {
-            uint16_t*& lo = *plo;
-            if (precision == DR_PRECISION_HILO && !lo) {
-                // (zero: rows stored before this call carry no lo half)
-                hipError_t e = dev_malloc(reinterpret_cast<void**>(&lo), bytes);
-                if (e == hipSuccess) e = hipMemset(lo, 0, bytes);
-                if (e != hipSuccess) {
-                    if (lo) (void)hipFree(lo);
-                    lo = nullptr;
-                    return hip_fail(e, "lo plane allocation");
-                }
-            } else if (precision == DR_PRECISION_BF16 && lo) {
-                (void)hipStreamSynchronize(cache->ctx->stream);
-                (void)hipFree(lo);
-                lo = nullptr;
+    // (zero: rows stored before this call carry no lo half, and none of them
+    // passes between the 8 bit planes and the others)
+    DR_CHECK(add_planes(cache, layer, precision, "cache plane allocation"));
+    const std::vector<Plane> keep = planes_of(cache, layer, precision);
+    bool waited = false;
+    for (int other : {DR_PRECISION_HILO, DR_PRECISION_FP8})
+        for (const Plane& pl : planes_of(cache, layer, other)) {
+            bool kept = false;
+            for (const Plane& k : keep) kept = kept || (k.p16 == pl.p16 && k.p8 == pl.p8);
+            if (kept) continue;
+            for (size_t i = layer * cache->n_batch; i < (layer + 1) * cache->n_batch; ++i) {
+                if (!pl.get(i)) continue;
+                if (!waited) (void)hipStreamSynchronize(cache->ctx->stream);
+                waited = true;
+                (void)hipFree(pl.get(i));
+                pl.set(i, nullptr);
             }
         }
-    }
     return DR_OK;
 }
 
@@ -822,9 +873,60 @@ static int store_rows(dr_step_cache* cache, size_t layer, size_t batch, const dr
     a.v_norm = v_norm ? 1 : 0;
     a.rope = rope ? rope->d_table : nullptr;
     a.rot = rope ? (int)rope->rope_dim : 0;
-    hipError_t e = dr::launch_store(cache->hd_tile[layer], a, cache->ctx->stream);
+    const size_t at = layer * cache->n_batch + batch;
+    if (cache->sc[at]) {
+        a.kc = reinterpret_cast<uint16_t*>(cache->k8[at]);
+        a.vtc = reinterpret_cast<uint16_t*>(cache->v8[at]);
+        a.sc = cache->sc[at];
+    }
+    hipError_t e = a.sc ? dr::launch_store_fp8(cache->hd_tile[layer], a, cache->ctx->stream)
+                        : dr::launch_store(cache->hd_tile[layer], a, cache->ctx->stream);
     if (e != hipSuccess) return hip_fail(e, "kv_store launch");
     return DR_OK;
+}
+
+// StepCache::gather of n positions on the device (pos0 >= 0: pos0, pos0 + 1, ...).
+static int gather_rows(dr_step_cache* cache, size_t layer, size_t batch, const int* pos, size_t n, int pos0,
+                       float* out_k, float* out_v) {
+    const size_t at = layer * cache->n_batch + batch;
+    dr::GatherArgs a{};
+    a.kc = cache->k[at];
+    a.vtc = cache->vt[at];
+    a.klo = cache->klo[at];
+    a.vlo = cache->vlo[at];
+    a.pos = pos;
+    a.n = (int)n;
+    a.n_head_kv = cache->hkv[layer];
+    a.hd = cache->hd[layer];
+    a.cap = (int)cache->cap;
+    a.out_k = out_k;
+    a.out_v = out_v;
+    a.pos0 = pos0;
+    if (cache->sc[at]) {
+        a.kc = reinterpret_cast<const uint16_t*>(cache->k8[at]);
+        a.vtc = reinterpret_cast<const uint16_t*>(cache->v8[at]);
+        a.sc = cache->sc[at];
+    }
+    hipError_t e = a.sc ? dr::launch_gather_fp8(cache->hd_tile[layer], a, cache->ctx->stream)
+                        : dr::launch_gather(cache->hd_tile[layer], a, cache->ctx->stream);
+    if (e != hipSuccess) return hip_fail(e, "kv_gather launch");
+    return DR_OK;
+}
+
+int dr_cache_gather_pass(dr_step_cache* cache, size_t layer, size_t batch, const dr_pass* pass, float* out_k,
+                         float* out_v) {
+    DR_CHECK(check_slot(cache, layer, batch, "dr_cache_gather_pass"));
+    if (!pass) return fail(DR_ERR_INVALID, "dr_cache_gather_pass: pass is NULL");
+    if (pass->ctx != cache->ctx)
+        return fail(DR_ERR_INVALID, "dr_cache_gather_pass: pass and cache use different contexts");
+    if (pass->n == 0) return DR_OK;
+    if (pass->max_pos >= cache->n_total)
+        return fail(DR_ERR_INVALID, "dr_cache_gather_pass: position %zu >= n_total %zu", pass->max_pos,
+                    cache->n_total);
+    if (!out_k || !out_v) return fail(DR_ERR_INVALID, "dr_cache_gather_pass: out_k/out_v is NULL");
+    DR_CHECK(use_device(cache->ctx));
+    return gather_rows(cache, layer, batch, pass->d_pos, pass->n,
+                       pass->max_pos - pass->min_pos + 1 == pass->n ? (int)pass->min_pos : -1, out_k, out_v);
 }
 
 int dr_cache_gather(dr_step_cache* cache, size_t layer, size_t batch, const size_t* positions,
@@ -844,20 +946,7 @@ int dr_cache_gather(dr_step_cache* cache, size_t layer, size_t batch, const size
     DR_CHECK(ensure(ctx->meta, n * sizeof(int32_t)));
     DR_HIP(hipMemcpyAsync(ctx->meta.p, h.data(), n * sizeof(int32_t), hipMemcpyHostToDevice,
                           ctx->stream));
-    dr::GatherArgs a{};
-    a.kc = cache->k[layer * cache->n_batch + batch];
-    a.vtc = cache->vt[layer * cache->n_batch + batch];
-    a.klo = cache->klo[layer * cache->n_batch + batch];
-    a.vlo = cache->vlo[layer * cache->n_batch + batch];
-    a.pos = static_cast<const int*>(ctx->meta.p);
-    a.n = (int)n;
-    a.n_head_kv = cache->hkv[layer];
-    a.hd = cache->hd[layer];
-    a.cap = (int)cache->cap;
-    a.out_k = out_k;
-    a.out_v = out_v;
-    hipError_t e = dr::launch_gather(cache->hd_tile[layer], a, ctx->stream);
-    if (e != hipSuccess) return hip_fail(e, "kv_gather launch");
+    DR_CHECK(gather_rows(cache, layer, batch, static_cast<const int*>(ctx->meta.p), n, -1, out_k, out_v));
     // the staging vector h dies here; the copy above was from pageable memory
     // and is complete when hipMemcpyAsync returns.
     return DR_OK;
@@ -1260,12 +1349,15 @@ static dr::LaunchPlan plan_for(dr_ctx* ctx, const dr::AttnArgs& a, int hd, int m
                                int max_nk, int mask, int qepi) {
     // a layer that keeps K's lo half gets f32-accurate scores, unless another
     // kernel family is forced (then the lo half is not read)
+    if (a.fp8)
+        return dr::plan_fp8(hd_tile_for((size_t)hd), a.n_batch, a.n_head_kv, a.group, max_nq, a.key_band, mask,
+                            ctx->n_cu, ctx->force_split);
     const bool hilo_asked = ctx->force_kernel == dr::KERNEL_AUTO || ctx->force_kernel == dr::KERNEL_HILO;
     const bool bf16_rows = a.q_bf16 || a.o_bf16;
     if (a.slot[0].klo && hilo_asked && !bf16_rows) return plan_hilo(ctx, a, hd, max_nq, max_nk, mask);
     // bf16 Q or output rows: only the per-wave-stream kernel reads / writes them
     const int kernel = bf16_rows ? dr::KERNEL_STREAMS
-                                : (ctx->force_kernel == dr::KERNEL_HILO ? dr::KERNEL_AUTO : ctx->force_kernel);
+                                : (ctx->force_kernel >= dr::KERNEL_HILO ? dr::KERNEL_AUTO : ctx->force_kernel);
     return dr::plan_attention(hd, a.n_batch, a.n_head_kv, a.group, max_nq, max_nk, mask, qepi,
                               mask == dr::MASK_POS ? a.window : -1, a.rope ? a.rot : 0, ctx->n_cu,
                               ctx->force_rb, ctx->force_kq, ctx->force_split, ctx->force_rows, kernel,
@@ -1331,7 +1423,7 @@ static int hilo_prepare_q(dr_ctx* ctx, dr::AttnArgs& a, float* base) {
 // plan that needs more than it holds is an error).
 // bf16 Q rows are read by the per-wave-stream kernel only.
 static int check_q_dtype(const dr::AttnArgs& a, const dr::LaunchPlan& p, const char* who) {
-    if ((!a.q_bf16 && !a.o_bf16) || p.kernel == dr::KERNEL_STREAMS) return DR_OK;
+    if ((!a.q_bf16 && !a.o_bf16) || p.kernel == dr::KERNEL_STREAMS || p.kernel == dr::KERNEL_FP8) return DR_OK;
     return fail(DR_ERR_UNSUPPORTED,
                 "%s: bf16 Q / output rows (dr_ctx_set_q_dtype, dr_ctx_set_o_dtype) are read and written by the "
                 "per-wave-stream kernel only: head dim 128 or 256, no per-key masks, a Q epilogue of at most "
@@ -1437,15 +1529,22 @@ static int cached_args(dr_step_cache* cache, size_t layer, const dr_batch_item* 
     // 11-23 times it and moves outputs by ~0.24 on a bf16 layer.  Such a call
     // needs a DR_PRECISION_HILO layer, unless the caller forced a kernel
     // family and so asked for bf16 scores.
+    // An 8 bit layer's K is coarser still; only its own kernel reads it.
     const bool hilo_layer = cache->klo[layer * cache->n_batch] != nullptr;
-    if (!hilo_layer && ctx->force_kernel == dr::KERNEL_AUTO &&
+    const bool fp8_layer = cache->sc[layer * cache->n_batch] != nullptr;
+    a.fp8 = fp8_layer ? 1 : 0;
+    if (fp8_layer && ctx->force_kernel != dr::KERNEL_AUTO && ctx->force_kernel != dr::KERNEL_FP8)
+        return fail(DR_ERR_UNSUPPORTED, "%s: layer %zu is held at DR_PRECISION_FP8, which the forced kernel family "
+                    "(dr_ctx_set_kernel) does not read", who, layer);
+    const bool forced = ctx->force_kernel != dr::KERNEL_AUTO && (fp8_layer || ctx->force_kernel != dr::KERNEL_FP8);
+    if (!hilo_layer && !forced &&
         std::fabs(scale) * std::sqrt((double)hd) > MAX_BF16_SCALE)
         return fail(DR_ERR_UNSUPPORTED,
-                    "%s: scale %g is %.1f times 1/sqrt(head_dim %zu), more than bf16 scores hold to the 1e-2 bar; "
+                    "%s: scale %g is %.1f times 1/sqrt(head_dim %zu), more than bf16 or 8 bit scores hold to the 1e-2 bar; "
                     "keep layer %zu at DR_PRECISION_HILO (dr_cache_create_layers, dr_cache_set_precision), or force "
-                    "a kernel family (dr_ctx_set_kernel) to accept bf16 scores",
+                    "a kernel family (dr_ctx_set_kernel) to accept them",
                     who, scale, std::fabs(scale) * std::sqrt((double)hd), hd, layer);
-    if ((a.q_bf16 || a.o_bf16) && ((hd != 128 && hd != 256) || cache->klo[layer * cache->n_batch]))
+    if ((a.q_bf16 || a.o_bf16) && !fp8_layer && ((hd != 128 && hd != 256) || cache->klo[layer * cache->n_batch]))
         return fail(DR_ERR_UNSUPPORTED,
                     "%s: bf16 Q / output rows (dr_ctx_set_q_dtype, dr_ctx_set_o_dtype) need head dim 128 or "
                     "256 and a bf16 layer (head dim %zu%s)",
@@ -1470,6 +1569,11 @@ static int cached_args(dr_step_cache* cache, size_t layer, const dr_batch_item* 
         s.vt = cache->vt[layer * cache->n_batch + b];
         s.klo = cache->klo[layer * cache->n_batch + b];
         s.vlo = cache->vlo[layer * cache->n_batch + b];
+        if (fp8_layer) {
+            s.k = reinterpret_cast<const uint16_t*>(cache->k8[layer * cache->n_batch + b]);
+            s.vt = reinterpret_cast<const uint16_t*>(cache->v8[layer * cache->n_batch + b]);
+            s.klo = reinterpret_cast<const uint16_t*>(cache->sc[layer * cache->n_batch + b]);
+        }
         s.nq = (int)it.pass->n;
         s.nk = (int)cache->n_total;
         s.qpos_sorted = 1;  // dr_pass positions are strictly ascending

@@ -81,6 +81,9 @@ struct AttnArgs {
     // (the union of the query rows' sliding-window bands), 0: not known
     int key_band;
     int ring_rot;  // the per-wave-stream kernel rotates each row group's tile walk
+    // (host planning only) a DR_PRECISION_FP8 layer: slot[].k and .vt are its
+    // code planes and .klo its scale bytes (fp8_common.hpp)
+    int fp8;
 };
 static_assert(offsetof(AttnArgs, slot) == 64, "scalar block of AttnArgs is one 64-byte line");
 
@@ -111,6 +114,7 @@ struct StoreArgs {
     const float* rope;   // [max_len][rot/2][2] (sin, cos) table, or nullptr
     int rot;             // rotated dims per head
     int pos0;            // >= 0: pos[r] == pos0 + r (contiguous rows), read without a load
+    uint8_t* sc;         // launch_store_fp8: scale bytes, kc and vtc being code planes (fp8_common.hpp)
 };
 
 struct GatherArgs {
@@ -125,6 +129,8 @@ struct GatherArgs {
     int cap;
     float* out_k;        // [n][n_head_kv][hd] f32
     float* out_v;
+    const uint8_t* sc;   // launch_gather_fp8: scale bytes, kc and vtc being code planes (fp8_common.hpp)
+    int pos0;            // the same: >= 0: pos[r] == pos0 + r, read without a load
 };
 
 // The Q/K/V epilogue of attention_block (forward.rs:291-310), in place on
@@ -331,12 +337,14 @@ struct LaunchPlan {
 // streams its own key tiles (no mask or MASK_POS, Q norm only).  HILO:
 // attn_hilo_kernel, f32-accurate scores and values from bf16 hi/lo halves of
 // Q, K and V (layers whose cache holds the lo halves, and the drop-in; every
-// mask mode, plain Q).
+// mask mode, plain Q).  FP8: attn_fp8_kernel, layers held as 8 bit codes (no
+// mask or MASK_POS, the whole Q epilogue, f32 and bf16 rows).
 enum KernelKind : int {
     KERNEL_AUTO = 0,
     KERNEL_STAGED = 1,
     KERNEL_STREAMS = 2,
     KERNEL_HILO = 3,
+    KERNEL_FP8 = 4,
 };
 
 // What of the Q/K/V epilogue the attention prologue applies to Q: nothing,
@@ -382,6 +390,13 @@ int hilo_rows();  // query rows per workgroup of attn_hilo_kernel
 hipError_t launch_rows(const LaunchPlan& p, const AttnArgs& a, hipStream_t st);
 hipError_t launch_hilo32(const LaunchPlan& p, const AttnArgs& a, hipStream_t st);
 int hilo32_rows(int hd_tile);  // the same of attn_hilo32_kernel (0: head dim not built)
+// DR_PRECISION_FP8 layers: the attention's plan and kernels (attn_fp8.hip), the
+// store and the gather (kv_fp8.hip).
+LaunchPlan plan_fp8(int hd_tile, int n_batch, int n_head_kv, int group, int max_nq, int max_nk, int mask, int n_cu,
+                    int force_split);
+hipError_t launch_fp8(const LaunchPlan& p, const AttnArgs& a, hipStream_t st);
+hipError_t launch_store_fp8(int hd_tile, const StoreArgs& a, hipStream_t st);
+hipError_t launch_gather_fp8(int hd_tile, const GatherArgs& a, hipStream_t st);
 hipError_t launch_store(int hd_tile, const StoreArgs& a, hipStream_t st);
 hipError_t launch_gather(int hd_tile, const GatherArgs& a, hipStream_t st);
 hipError_t launch_epilogue(const EpiArgs& a, hipStream_t st);

@@ -27,9 +27,9 @@ LIB_PATH = HERE / "lib" / "libdr_attn.so"
 HEADER_PATH = HERE.parent / "include" / "dr_attn.h"
 
 DR_OK, DR_ERR_INVALID, DR_ERR_NO_DEVICE, DR_ERR_OOM, DR_ERR_HIP, DR_ERR_UNSUPPORTED, DR_ERR_BUSY = range(7)
-KERNEL_AUTO, KERNEL_STAGED, KERNEL_STREAMS, KERNEL_HILO = range(4)
+KERNEL_AUTO, KERNEL_STAGED, KERNEL_STREAMS, KERNEL_HILO, KERNEL_FP8 = range(5)
 DTYPE_F32, DTYPE_BF16 = 0, 1
-PRECISION_BF16, PRECISION_HILO = 0, 1  # dr_cache_set_precision
+PRECISION_BF16, PRECISION_HILO, PRECISION_FP8 = 0, 1, 2  # dr_cache_set_precision
 STATUS_NAMES = {
     DR_OK: "DR_OK",
     DR_ERR_INVALID: "DR_ERR_INVALID",
@@ -164,6 +164,7 @@ _SIGS = {
     "dr_cache_set_precision": (_I, [_VP, _SZ, _I]),
     "dr_cache_store": (_I, [_VP, _SZ, _SZ, _VP, _VP, _VP, _VP, _F]),
     "dr_cache_gather": (_I, [_VP, _SZ, _SZ, c_size_p, _SZ, _VP, _VP]),
+    "dr_cache_gather_pass": (_I, [_VP, _SZ, _SZ, _VP, _VP, _VP]),
     "dr_cache_update_seq": (_I, [_VP, _SZ, _VP, _SZ]),
     "dr_cache_split_active": (_I, [_VP, _SZ, _VP, _VP, _SZ, _SZ, c_size_p, c_size_p, c_size_p, c_size_p]),
     "dr_split_active": (_I, [_VP, _VP, _VP, _VP, _SZ, _SZ, _SZ, c_size_p, c_size_p, c_size_p, c_size_p]),
@@ -347,7 +348,7 @@ class Context:
         _check(self.lib.dr_ctx_set_wave_rows(self.h, rows))
 
     def set_kernel(self, kernel: int) -> None:
-        """KERNEL_AUTO, KERNEL_STAGED, KERNEL_STREAMS or KERNEL_HILO (dr_ctx_set_kernel)."""
+        """KERNEL_AUTO, KERNEL_STAGED, KERNEL_STREAMS, KERNEL_HILO or KERNEL_FP8 (dr_ctx_set_kernel)."""
         _check(self.lib.dr_ctx_set_kernel(self.h, kernel))
 
     def set_q_dtype(self, dtype: int) -> None:
@@ -467,11 +468,12 @@ def _ptr(t) -> int:
 
 
 class StepCache:
-    """dr_step_cache: per-layer bf16 K/V for every position, in HBM."""
+    """dr_step_cache: per-layer K/V for every position, in HBM: bf16, bf16 hi/lo
+    halves or 8 bit codes with a scale per position and KV head."""
 
     def __init__(self, ctx: Context, n_total: int, n_head_kv: Sequence[int],
                  head_dim: Sequence[int], n_batch: int = 1, precision: Optional[Sequence[int]] = None):
-        """precision: per-layer PRECISION_BF16 / PRECISION_HILO
+        """precision: per-layer PRECISION_BF16 / _HILO / _FP8
         (dr_cache_create_layers); None: every layer bf16 (dr_cache_create)."""
         self.ctx = ctx
         hkv, hkv_p, n_layer = _usize_array(n_head_kv)
@@ -491,8 +493,9 @@ class StepCache:
         self.n_batch = n_batch
 
     def set_precision(self, layer: int, precision: int) -> None:
-        """PRECISION_BF16 or PRECISION_HILO for one layer (dr_cache_set_precision):
-        HILO keeps K's lo half and gives the layer f32-accurate scores."""
+        """PRECISION_BF16, _HILO or _FP8 for one layer (dr_cache_set_precision):
+        HILO keeps K's lo half and gives the layer f32-accurate scores; FP8
+        holds K and V in 8 bits (to or from it the layer's rows are dropped)."""
         _check(self.ctx.lib.dr_cache_set_precision(self.h, layer, precision))
 
     def store(self, layer: int, p: Pass, k, v, k_norm_w=None, eps: float = 1e-6, batch: int = 0):
@@ -503,6 +506,11 @@ class StepCache:
         arr, ptr, n = _usize_array(positions)
         _check(self.ctx.lib.dr_cache_gather(self.h, layer, batch, ptr, n, _ptr(out_k),
                                             _ptr(out_v)))
+
+    def gather_pass(self, layer: int, p: Pass, out_k, out_v, batch: int = 0) -> None:
+        """gather() at a pass's positions, which are on the device
+        (dr_cache_gather_pass): nothing is uploaded or waited for."""
+        _check(self.ctx.lib.dr_cache_gather_pass(self.h, layer, batch, p.h, _ptr(out_k), _ptr(out_v)))
 
     def update_seq(self, seq, batch: int = 0) -> None:
         a = np.ascontiguousarray(seq, dtype=np.int32)

@@ -178,17 +178,36 @@ void dr_cache_destroy(dr_step_cache* cache);
  * query sequence ids). */
 #define DR_PRECISION_BF16 0
 #define DR_PRECISION_HILO 1
+/* DR_PRECISION_FP8: the layer holds K and V in 8 bits, half the memory of a
+ * bf16 layer.  The head_dim values of one position of one KV head are a block:
+ * they share a power of two 2^e, the smallest that keeps the largest magnitude
+ * within 448 (e >= -126), and each is held as the e4m3 code of x / 2^e (to
+ * nearest, ties to even); e is one byte per block.  Each store quantises its
+ * own rows and no others, so what a layer holds does not depend on the order of
+ * stores.  A value is kept to 2^-4 of itself (to 2^(e-10) where it is smaller
+ * than 2^(e-6)).  A row with a NaN or an infinity has no 8 bit form: all of it
+ * stands for NaN.  A position that was never stored reads as zeros.
+ * dr_cache_store and the step calls (with their whole epilogue) write such a
+ * layer, dr_cache_gather and dr_cache_gather_pass give back the f32 values that
+ * it stands for, and every cached attention call reads it: f32 rows with
+ * f32-accurate arithmetic on those values, so the cache's own rounding is the
+ * only one that counts; bf16 Q and output rows (both: dr_ctx_set_q_dtype,
+ * dr_ctx_set_o_dtype) with 11 bit weights, at any head dim.  The scale limit of
+ * bf16 layers applies (dr_cache_create_layers).  Changing a layer to or from
+ * DR_PRECISION_FP8 drops the rows it holds (they read as zeros) and frees its
+ * planes: a captured hipGraph that uses the layer must not be replayed after. */
+#define DR_PRECISION_FP8 2
 int dr_cache_set_precision(dr_step_cache* cache, size_t layer, int precision);
 /* dr_cache_create with each layer's score precision given up front
- * (precision: n_layer entries, DR_PRECISION_BF16 or DR_PRECISION_HILO; NULL =
+ * (precision: n_layer entries, DR_PRECISION_BF16, _HILO or _FP8; NULL =
  * all bf16), so a binding sets it from the layer's attention scale when it
  * builds the cache: DiffusionGemma, whose layers all use kq_scale 1.0
  * (forward.rs:338-341), takes DR_PRECISION_HILO for every layer.  A cached
  * attention call (dr_attention_cached, _noalloc, _step, _step_epi) on a
- * DR_PRECISION_BF16 layer with |scale| * sqrt(head_dim) > 2 fails with
+ * DR_PRECISION_BF16 or _FP8 layer with |scale| * sqrt(head_dim) > 2 fails with
  * DR_ERR_UNSUPPORTED, since bf16 scores miss the 1e-2 bar there (outputs move
  * by ~0.24 at Gemma's 1.0), unless a kernel family was forced with
- * dr_ctx_set_kernel (then the caller accepts bf16 scores). */
+ * dr_ctx_set_kernel (then the caller accepts bf16 or 8 bit scores). */
 int dr_cache_create_layers(dr_ctx* ctx, size_t n_total, size_t n_layer, const size_t* n_head_kv,
                            const size_t* head_dim, const int* precision, size_t n_batch,
                            dr_step_cache** out);
@@ -206,6 +225,13 @@ int dr_cache_store(dr_step_cache* cache, size_t layer, size_t batch, const dr_pa
  * cache contents widened to f32. */
 int dr_cache_gather(dr_step_cache* cache, size_t layer, size_t batch, const size_t* positions,
                     size_t n, float* out_k, float* out_v);
+/* The same at a pass's positions, which are on the device already: nothing is
+ * uploaded, and the call only enqueues (no counterpart in the reference, whose
+ * lists are host slices; the cached list of dr_cache_split_active_dev is a
+ * pass).  Any layer precision; on DR_PRECISION_FP8 layers the f32 values that
+ * the codes stand for. */
+int dr_cache_gather_pass(dr_step_cache* cache, size_t layer, size_t batch, const dr_pass* pass, float* out_k,
+                         float* out_v);
 
 /* StepCache::update_seq (cache.rs:56-59) for one batch slot (host data). */
 int dr_cache_update_seq(dr_step_cache* cache, size_t batch, const int32_t* seq, size_t n);
@@ -462,7 +488,7 @@ typedef struct {
     int key_groups;
     int rows_per_wave; /* query rows per compute wave: 32, or 16 (STAGED: two waves per row
                         * block; STREAMS at head dim 256: one 16-row block per workgroup) */
-    int kernel; /* DR_KERNEL_STAGED, DR_KERNEL_STREAMS or DR_KERNEL_HILO: which attention kernel ran */
+    int kernel; /* DR_KERNEL_STAGED, _STREAMS, _HILO or _FP8: which attention kernel ran */
     int split_merge; /* key splits merged: 0 no split, 1 by a second kernel, 2 in-kernel */
 } dr_launch_info;
 int dr_ctx_last_launch(const dr_ctx* ctx, dr_launch_info* info);
@@ -485,11 +511,15 @@ int dr_ctx_set_wave_rows(dr_ctx* ctx, int rows);
  * (f32-accurate scores and values from bf16 hi/lo halves of Q, K and V; see
  * dr_cache_set_precision). */
 #define DR_KERNEL_HILO 3
+/* FP8: layers kept at DR_PRECISION_FP8. */
+#define DR_KERNEL_FP8 4
 /* Pick the kernel family for later calls on ctx: DR_KERNEL_AUTO (the
- * planner: HILO on hi/lo layers, else STREAMS wherever it applies), or force
- * STAGED / STREAMS (STREAMS falls back to STAGED where it does not apply; on
- * a hi/lo layer both ignore the lo half).  A tuning knob, for measurement
- * and tests. */
+ * planner: HILO on hi/lo layers, FP8 on 8 bit layers, else STREAMS wherever it
+ * applies), or force STAGED / STREAMS (STREAMS falls back to STAGED where it
+ * does not apply; on a hi/lo layer both ignore the lo half).  An 8 bit layer is
+ * read by its own family only: with another one forced its calls fail with
+ * DR_ERR_UNSUPPORTED; HILO and FP8 mean AUTO on layers that are not theirs.  A
+ * tuning knob, for measurement and tests. */
 int dr_ctx_set_kernel(dr_ctx* ctx, int kernel);
 /* The element type of the Q rows that later dr_attention_cached /
  * _cached_noalloc / _step / _step_epi calls on ctx read (no counterpart in
@@ -497,8 +527,8 @@ int dr_ctx_set_kernel(dr_ctx* ctx, int kernel);
  * produce bf16).  DR_DTYPE_F32 (the default): q points at float rows.
  * DR_DTYPE_BF16: q points at bf16 rows of the same shape (uint16 bit
  * patterns), read by the per-wave-stream kernel, which applies the Q
- * epilogue and the scale to them as to f32 rows.  Calls that that kernel
- * cannot run (head dims other than 128 / 256, hi/lo layers, RoPE below full
+ * epilogue and the scale to them as to f32 rows, and on DR_PRECISION_FP8
+ * layers by theirs.  Calls on other layers that that kernel cannot run (head dims other than 128 / 256, hi/lo layers, RoPE below full
  * rotary, forced tile shapes) fail with DR_ERR_UNSUPPORTED before any
  * store. */
 #define DR_DTYPE_F32 0
@@ -510,8 +540,8 @@ int dr_ctx_set_q_dtype(dr_ctx* ctx, int dtype);
  * projection reads bf16).  DR_DTYPE_F32 (the default): out points at float
  * rows.  DR_DTYPE_BF16: out points at bf16 rows of the same shape (uint16
  * bit patterns), each the f32 result rounded to nearest even; written by the
- * per-wave-stream kernel, with the same restrictions and errors as
- * dr_ctx_set_q_dtype's bf16 rows. */
+ * per-wave-stream kernel and the 8 bit layers' kernel, with the same
+ * restrictions and errors as dr_ctx_set_q_dtype's bf16 rows. */
 int dr_ctx_set_o_dtype(dr_ctx* ctx, int dtype);
 /* How key splits of the STREAMS kernel are merged on later calls on ctx (a
  * tuning knob with no counterpart in the reference, for measurement and
