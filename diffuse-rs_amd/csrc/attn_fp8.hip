@@ -35,8 +35,8 @@
 // waves take tiles t, t + NW, ..., each with its own state, and merge through
 // LDS.  Tiles come straight from memory into registers, one ahead: the planes
 // hold a tile in operand order, so every load is one contiguous run.  Few
-// workgroups split the keys further; the partial states go to a workspace and
-// fp8_merge_kernel joins them.
+// workgroups split the keys further: each leaves its state in a workspace, and
+// the last one of a row block to finish (an atomic ticket) joins them.
 //
 // A key that a row may not see never reaches its output: its p is set to 0 and
 // its codes are finite always (a row that held a NaN has codes 0 and the NaN in
@@ -47,6 +47,8 @@
 
 #include <algorithm>
 #include <type_traits>
+
+#include <float.h>
 
 #include <math.h>
 
@@ -59,9 +61,7 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 constexpr float P0 = 8.0f, MOVE = 7.0f;
-constexpr int NW = 4;  // waves per workgroup
-
-template <int HD, int QR, int PL>
+template <int HD, int QR, int PL, int NW>
 struct Fp8Geo {
     static constexpr int KB = QR == 32 ? 1 : 2;       // A blocks (32 or 16 keys) of a tile
     static constexpr int SK = QR == 32 ? 16 : 32;     // contraction of one MFMA
@@ -72,16 +72,15 @@ struct Fp8Geo {
     static constexpr int KCH = HD * 32 / 16 / 64;     // 16-byte K pieces per lane and tile
     static constexpr int VW = HD * 32 / 4 / 64;       // dwords of V per lane and tile
     // Head dim 512: the query planes (128 registers) are read from LDS as they
-    // are multiplied, and no tile is fetched ahead, for the registers' sake.
+    // are multiplied, for the registers' sake.
     static constexpr bool BIG = HD > 256;
     static constexpr int QP = HD + 8;                 // f16 pitch of a staged query row
     static constexpr int OP = HD + 4;                 // f32 pitch of a merged row
     static constexpr size_t Q_BYTES = (size_t)PL * QR * QP * 2;
-    static constexpr size_t EPI_BYTES = (size_t)NW * HD * 4;
     static constexpr size_t O_BYTES = (size_t)NW * QR * OP * 4;
-    static constexpr size_t BODY = O_BYTES > Q_BYTES + EPI_BYTES ? O_BYTES : Q_BYTES + EPI_BYTES;
-    // then: per-row scales, wave states, V scales of each wave's tile
-    static constexpr size_t LDS = BODY + QR * 4 + 2 * NW * QR * 4 + NW * 32 * 4;
+    static constexpr size_t BODY = O_BYTES > Q_BYTES ? O_BYTES : Q_BYTES;
+    // then: per-row scales, wave states, V scales (f16) of each wave's tile, the ticket
+    static constexpr size_t LDS = BODY + QR * 4 + 2 * NW * QR * 4 + NW * 32 * 2 + 16;
 };
 
 __device__ __forceinline__ f32x16 mfma(const f16x8& a, const f16x8& b, const f32x16& c) {
@@ -105,64 +104,136 @@ __device__ __forceinline__ float pow2_biased(int e) { return __uint_as_float((ui
 // dword w of p, as loaded bytes
 __device__ __forceinline__ int byte_of(const u32x4& w, int i) { return (int)(w[i / 4] >> (8 * (i % 4))) & 255; }
 
-// The query row of packed row r: its values with the Q epilogue applied
-// (forward.rs:291-310: bias, RMSNorm with f32 squares summed in f64, RoPE), EPL
-// consecutive ones per lane.  `scratch`: HD floats of this wave.
+__device__ __forceinline__ int row_pos(const AttnSlot& S, int qi) { return S.qpos0 >= 0 ? S.qpos0 + qi : S.qpos[qi]; }
+
+// Values d..d + 3 of a query row (0 past head_dim), f32.
 template <int HD>
-__device__ __forceinline__ void load_query(const AttnArgs& a, const AttnSlot& S, int qi, int head, int pos,
-                                           float* scratch, float (&y)[HD / 64]) {
-#pragma clang fp contract(off)
-    constexpr int EPL = HD / 64;
-    const int lane = threadIdx.x & 63, d0 = lane * EPL, hd = a.hd;
-    const size_t off = (size_t)qi * a.q_rstride + (size_t)head * hd + d0;
+__device__ __forceinline__ f32x4 query4(const AttnArgs& a, const AttnSlot& S, size_t row, int d) {
+    f32x4 y;
     if (a.q_bf16) {
-        const uint16_t* q = static_cast<const uint16_t*>(S.q) + off;
+        const uint16_t* q = static_cast<const uint16_t*>(S.q) + row + d;
+        if (a.hd == HD) {  // (rows and heads start 8-byte aligned)
+            const u32x2 w = gload<u32x2>(q);
+            y = f32x4{__uint_as_float(w[0] << 16), __uint_as_float(w[0] & 0xffff0000u), __uint_as_float(w[1] << 16),
+                      __uint_as_float(w[1] & 0xffff0000u)};
+        } else {
 #pragma unroll
-        for (int e = 0; e < EPL; ++e)
-            y[e] = d0 + e < hd ? __uint_as_float((uint32_t)gload<uint16_t>(q + e) << 16) : 0.0f;
+            for (int e = 0; e < 4; ++e)
+                y[e] = d + e < a.hd ? __uint_as_float((uint32_t)gload<uint16_t>(q + e) << 16) : 0.0f;
+        }
     } else {
-        const float* q = static_cast<const float*>(S.q) + off;
+        const float* q = static_cast<const float*>(S.q) + row + d;
+        if (a.hd == HD) {
+            y = gload<f32x4>(q);
+        } else {
 #pragma unroll
-        for (int e = 0; e < EPL; ++e) y[e] = d0 + e < hd ? gload<float>(q + e) : 0.0f;
+            for (int e = 0; e < 4; ++e) y[e] = d + e < a.hd ? gload<float>(q + e) : 0.0f;
+        }
     }
-    if (a.qb)
+    return y;
+}
+
+// Four values of a vector of head_dim parameters (0 past it).
+__device__ __forceinline__ f32x4 param4(const float* w, int d, int hd) {
+    f32x4 y;
 #pragma unroll
-        for (int e = 0; e < EPL; ++e) y[e] += d0 + e < hd ? a.qb[(size_t)head * hd + d0 + e] : 0.0f;
+    for (int e = 0; e < 4; ++e) y[e] = d + e < hd ? w[d + e] : 0.0f;
+    return y;
+}
+
+// The Q epilogue (forward.rs:291-310) on values d0..d0 + 15 of a query row that
+// HD / 16 consecutive lanes hold: bias, RMSNorm (f32 squares summed in f64),
+// RoPE, whose partners d +- rot/2 (rot/2 a multiple of 4) are loaded again.
+template <int HD>
+__device__ __forceinline__ void query_epilogue(const AttnArgs& a, const AttnSlot& S, size_t row, int head, int pos,
+                                               int d0, f32x4 (&y)[4]) {
+#pragma clang fp contract(off)
+    const float* bias = a.qb ? a.qb + (size_t)head * a.hd : nullptr;
+    if (bias)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] += param4(bias, d0 + 4 * i, a.hd);
+    float sc = 1.0f;
     if (a.qn_w) {
         double ss = 0.0;
 #pragma unroll
-        for (int e = 0; e < EPL; ++e) {
-            const float sq = y[e] * y[e];
-            ss += (double)sq;
-        }
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int o = 32; o > 0; o >>= 1) ss += __shfl_xor(ss, o);
-        const float sc = 1.0f / (float)sqrt(ss / (double)hd + (double)a.qn_eps);
+            for (int e = 0; e < 4; ++e) {
+                const float sq = y[i][e] * y[i][e];
+                ss += (double)sq;
+            }
 #pragma unroll
-        for (int e = 0; e < EPL; ++e) y[e] = y[e] * sc * (d0 + e < hd ? a.qn_w[d0 + e] : 0.0f);
+        for (int o = HD / 32; o > 0; o >>= 1) ss += __shfl_xor(ss, o);
+        sc = 1.0f / (float)sqrt(ss / (double)a.hd + (double)a.qn_eps);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] = y[i] * sc * param4(a.qn_w, d0 + 4 * i, a.hd);
     }
     if (a.rope) {
         const int half = a.rot / 2;
 #pragma unroll
-        for (int e = 0; e < EPL; ++e) scratch[d0 + e] = y[e];
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        for (int i = 0; i < 4; ++i) {
+            const int d = d0 + 4 * i;
+            if (d >= a.rot) continue;  // (rot is a multiple of 8)
+            const int pd = d < half ? d + half : d - half, j = d < half ? d : pd;
+            f32x4 x = query4<HD>(a, S, row, pd);
+            if (bias) x += param4(bias, pd, a.hd);
+            if (a.qn_w) x = x * sc * param4(a.qn_w, pd, a.hd);
+            const float* t = a.rope + ((size_t)pos * half + j) * 2;
 #pragma unroll
-        for (int e = 0; e < EPL; ++e) {
-            const int d = d0 + e;
-            if (d >= a.rot) continue;
-            const int j = d < half ? d : d - half;
-            const float2 t = *reinterpret_cast<const float2*>(a.rope + ((size_t)pos * half + j) * 2);
-            y[e] = d < half ? rope_lo(y[e], scratch[d + half], t.x, t.y) : rope_hi(scratch[j], y[e], t.x, t.y);
+            for (int e = 0; e < 4; ++e)
+                y[i][e] = d < half ? rope_lo(y[i][e], x[e], t[2 * e], t[2 * e + 1])
+                                   : rope_hi(x[e], y[i][e], t[2 * e], t[2 * e + 1]);
         }
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     }
 }
 
-__device__ __forceinline__ int row_pos(const AttnSlot& S, int qi) { return S.qpos0 >= 0 ? S.qpos0 + qi : S.qpos[qi]; }
+// The query rows r0 .. r0 + ROWS - 1: with the epilogue applied, scaled by a
+// power of two each (inverse to srow), split into PL planes of f16 in sq
+// [PL][ROWS][QP].  A thread takes 16 values of a row, all rows of a pass in
+// flight at once.
+template <int HD, int ROWS, int PL, int NT, int QP>
+__device__ __forceinline__ void stage_queries(const AttnArgs& a, const AttnSlot& S, int g, int r0, int rows,
+                                              _Float16* sq, float* srow) {
+    constexpr int LPR = HD / 16, PER = NT / LPR;  // lanes per row, rows per pass
+    const int tid = threadIdx.x, d0 = tid % LPR * 16;
+#pragma unroll
+    for (int p = 0; p < (ROWS + PER - 1) / PER; ++p) {
+        const int i = p * PER + tid / LPR;
+        // (a row past the last is the last again; lanes of a row agree)
+        const int r = min(r0 + min(i, ROWS - 1), rows - 1), qi = r / a.group, head = g * a.group + r - qi * a.group;
+        const size_t row = (size_t)qi * a.q_rstride + (size_t)head * a.hd;
+        f32x4 y[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = query4<HD>(a, S, row, d0 + 4 * e);
+        if (a.qb || a.qn_w || a.rope) query_epilogue<HD>(a, S, row, head, a.rope ? row_pos(S, qi) : 0, d0, y);
+        uint32_t top = 0;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) top = max(top, __float_as_uint(y[e / 4][e % 4]) & 0x7fffffffu);
+#pragma unroll
+        for (int o = LPR / 2; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o));
+        // 2^14 <= |largest| * up < 2^15; a row with a NaN or an infinity gives NaN
+        const bool bad = top >= 0x7f800000u;
+        const int ex = min(268 - (int)(top >> 23), 254);
+        float up = bad ? __uint_as_float(0x7fc00000u) : pow2_biased(ex);
+        if (a.c < 0.0f) up = -up;
+        if (i < ROWS) {
+            if (tid % LPR == 0) srow[i] = pow2_biased(bad ? 127 : 254 - ex);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                f16x8 hi, lo;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float z = y[2 * h + e / 4][e % 4] * up;
+                    hi[e] = (_Float16)z;
+                    lo[e] = (_Float16)(z - (float)hi[e]);
+                }
+                *reinterpret_cast<f16x8*>(sq + i * QP + d0 + 8 * h) = hi;
+                if constexpr (PL == 2) *reinterpret_cast<f16x8*>(sq + (ROWS + i) * QP + d0 + 8 * h) = lo;
+            }
+        }
+    }
+}
+
 
 // out[row] of packed row r, four values from d on
 template <int HD>
@@ -188,18 +259,18 @@ __device__ __forceinline__ void write_out(const AttnArgs& a, const AttnSlot& S, 
     }
 }
 
-template <int HD, int QR, int PL>
+template <int HD, int QR, int PL, int NW>
 __global__ __launch_bounds__(NW * 64) void attn_fp8_kernel(const AttnArgs a) {
-    using G = Fp8Geo<HD, QR, PL>;
+    using G = Fp8Geo<HD, QR, PL, NW>;
     using Acc = std::conditional_t<QR == 32, f32x16, f32x4>;
     extern __shared__ __align__(16) char lds[];
     _Float16* const sq = reinterpret_cast<_Float16*>(lds);                 // [PL][QR][QP]
-    float* const sepi = reinterpret_cast<float*>(lds + G::Q_BYTES);        // [NW][HD]
     float* const so = reinterpret_cast<float*>(lds);                       // [NW][QR][OP], after the key loop
     float* const srow = reinterpret_cast<float*>(lds + G::BODY);           // [QR]
     float* const sm = srow + QR;                                           // [NW][QR]
     float* const sl = sm + NW * QR;                                        // [NW][QR]
-    float* const svs = sl + NW * QR;                                       // [NW][32]
+    _Float16* const svs = reinterpret_cast<_Float16*>(sl + NW * QR);       // [NW][32]
+    int* const stick = reinterpret_cast<int*>(svs + NW * 32);
 
     // Workgroup -> (batch slot, KV head, key split, row block): each XCD (the
     // hardware deals workgroups round robin over the 8) takes a contiguous run,
@@ -215,46 +286,8 @@ __global__ __launch_bounds__(NW * 64) void attn_fp8_kernel(const AttnArgs a) {
     const AttnSlot& S = a.slot[b];
     const int rows = S.nq * a.group, r0 = rb * QR;
     if (r0 >= rows) return;  // (a shorter pass of the batch)
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int col = lane % QR, half = lane / QR;  // query column; 0..1 (0..3 with 16 rows)
-
-    // ---- the query rows: scaled, split into planes, staged in LDS
-    for (int i = wave; i < QR; i += NW) {
-        float y[HD / 64];
-        const int r = r0 + i;
-        const bool ok = r < rows;
-        const int rr = ok ? r : rows - 1, qi = rr / a.group;
-        load_query<HD>(a, S, qi, g * a.group + rr - qi * a.group, a.rope ? row_pos(S, qi) : 0, sepi + wave * HD, y);
-        uint32_t top = 0;
-#pragma unroll
-        for (int e = 0; e < HD / 64; ++e) top = max(top, __float_as_uint(y[e]) & 0x7fffffffu);
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o));
-        // 2^14 <= |largest| * up < 2^15; a row with a NaN or an infinity gives NaN
-        const int e = min(268 - (int)(top >> 23), 254);
-        const float up = top >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : pow2_biased(e);
-        if (lane == 0) srow[i] = pow2_biased(top >= 0x7f800000u ? 127 : 254 - e);
-#pragma unroll
-        for (int k = 0; k < HD / 64; ++k) {
-            const float z = (a.c < 0.0f ? -y[k] : y[k]) * up;
-            const _Float16 hi = (_Float16)z;
-            sq[i * G::QP + lane * (HD / 64) + k] = hi;
-            if constexpr (PL == 2) sq[(QR + i) * G::QP + lane * (HD / 64) + k] = (_Float16)(z - (float)hi);
-        }
-    }
-    __syncthreads();
-    auto query = [&](int p, int s) __attribute__((always_inline)) {
-        // K piece j of a lane holds 16 values, steps 2j and 2j + 1
-        const int d = ((64 / QR) * (s / 2) + half) * 16 + s % 2 * 8;
-        return *reinterpret_cast<const f16x8*>(sq + (p * QR + col) * G::QP + d);
-    };
-    f16x8 q[PL][G::BIG ? 1 : G::NS];
-    if constexpr (!G::BIG)
-#pragma unroll
-        for (int p = 0; p < PL; ++p)
-#pragma unroll
-            for (int s = 0; s < G::NS; ++s) q[p][s] = query(p, s);
-    const float cq = fabsf(a.c) * srow[col];
 
     // ---- the key tiles this workgroup's rows can see
     const int q_lo = row_pos(S, r0 / a.group), q_hi = row_pos(S, (min(r0 + QR, rows) - 1) / a.group);
@@ -276,23 +309,23 @@ __global__ __launch_bounds__(NW * 64) void attn_fp8_kernel(const AttnArgs a) {
         uint32_t v[G::VW];
         int kb, vb;  // scale bytes: K's of this lane's A row (16 rows: of both blocks, 8 bits each), V's of key lane % 32
     };
-    auto fetch = [&](int t, Tile& x) __attribute__((always_inline)) {
+    // K and scales, then V: a step refills K's registers once its scores are
+    // formed and V's once its product is, so the loads run under the rest of the
+    // step and a tile ahead costs no registers.  (A tile past the plane's end,
+    // which nobody multiplies, is its last one.)
+    auto fetch_k = [&](int t, Tile& x) __attribute__((always_inline)) {
         t = min(t, last_tile);
         const uint8_t* kt = kbase + (size_t)t * 32 * HD;
-        const uint8_t* vt = vbase + (size_t)t * 32 * HD;
         const uint8_t* st = sbase + (size_t)t * 64;
         if constexpr (QR == 32) {
             const int key = sigma(col);
+            x.kb = gload<uint8_t>(st + key);
+            x.vb = gload<uint8_t>(st + 32 + (lane & 31));
 #pragma unroll
             for (int j = 0; j < G::KCH; ++j) x.k[j] = gload<u32x4>(kt + (2 * j + half) * 512 + key * 16);
-#pragma unroll
-            for (int db = 0; db < G::DB; ++db) {
-                const u32x4 w = gload<u32x4>(vt + (32 * db + col) * 32 + half * 16);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) x.v[4 * db + e] = w[e];
-            }
-            x.kb = gload<uint8_t>(st + key);
         } else {
+            x.kb = (int)gload<uint8_t>(st + kappa(col)) | (int)gload<uint8_t>(st + kappa(16 + col)) << 8;
+            x.vb = gload<uint8_t>(st + 32 + (lane & 31));
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb) {
                 const int key = kappa(16 * kb + col);
@@ -300,16 +333,49 @@ __global__ __launch_bounds__(NW * 64) void attn_fp8_kernel(const AttnArgs a) {
                 for (int j = 0; j < G::KCH / 2; ++j)
                     x.k[kb * (G::KCH / 2) + j] = gload<u32x4>(kt + (4 * j + half) * 512 + key * 16);
             }
+        }
+    };
+    auto fetch_v = [&](int t, Tile& x) __attribute__((always_inline)) {
+        const uint8_t* vt = vbase + (size_t)min(t, last_tile) * 32 * HD;
+        if constexpr (QR == 32) {
+#pragma unroll
+            for (int db = 0; db < G::DB; ++db) {
+                const u32x4 w = gload<u32x4>(vt + (32 * db + col) * 32 + half * 16);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x.v[4 * db + e] = w[e];
+            }
+        } else {
 #pragma unroll
             for (int db = 0; db < G::DB; ++db) {
                 const u32x2 w = gload<u32x2>(vt + (16 * db + col) * 32 + half * 8);
                 x.v[2 * db] = w[0];
                 x.v[2 * db + 1] = w[1];
             }
-            x.kb = (int)gload<uint8_t>(st + kappa(col)) | (int)gload<uint8_t>(st + kappa(16 + col)) << 8;
         }
-        x.vb = gload<uint8_t>(st + 32 + (lane & 31));
     };
+
+    Tile x;
+    const int t_first = t0 + wave;
+    if (t_first < t1) {  // (in flight while the query rows are staged)
+        fetch_k(t_first, x);
+        fetch_v(t_first, x);
+    }
+
+    // ---- the query rows
+    stage_queries<HD, QR, PL, NW * 64, G::QP>(a, S, g, r0, rows, sq, srow);
+    __syncthreads();
+    auto query = [&](int p, int s) __attribute__((always_inline)) {
+        // K piece j of a lane holds 16 values, steps 2j and 2j + 1
+        const int d = ((64 / QR) * (s / 2) + half) * 16 + s % 2 * 8;
+        return *reinterpret_cast<const f16x8*>(sq + (p * QR + col) * G::QP + d);
+    };
+    f16x8 q[PL][G::BIG ? 1 : G::NS];
+    if constexpr (!G::BIG)
+#pragma unroll
+        for (int p = 0; p < PL; ++p)
+#pragma unroll
+            for (int s = 0; s < G::NS; ++s) q[p][s] = query(p, s);
+    const float cq = fabsf(a.c) * srow[col];
 
     Acc o[G::DB];
 #pragma unroll
@@ -318,9 +384,9 @@ __global__ __launch_bounds__(NW * 64) void attn_fp8_kernel(const AttnArgs a) {
         for (int i = 0; i < G::SPL; ++i) o[db][i] = 0.0f;
     float m = -INFINITY, l = 0.0f, kc = 0.0f;
     int kref = 0, vref = 0;
-    float* const my_vs = svs + wave * 32;
+    _Float16* const my_vs = svs + wave * 32;
 
-    auto step = [&](int t, const Tile& x) __attribute__((always_inline)) {
+    auto step = [&](int t, Tile& x) __attribute__((always_inline)) {
         // ---- scales: relative to the largest so far
         bool slow = !(32 * t + 32 <= S.nk && (a.window < 0 || (q_hi - 32 * t < a.window && 32 * t + 31 - q_lo < a.window)) &&
                       (a.prefix < 0 || q_lo >= a.prefix || 32 * t + 31 <= q_lo));
@@ -336,7 +402,9 @@ __global__ __launch_bounds__(NW * 64) void attn_fp8_kernel(const AttnArgs a) {
                 vt = max(vt, __shfl_xor(vt, off));
             }
             kref = max(kref, kt);
+            // (never 0: a hidden score of -infinity has to stay one)
             kc = ldexpf(cq, kref - 127 - 7);
+            kc = kc < FLT_MIN ? FLT_MIN : kc;
             if (vt > vref) {
                 const float f = pow2_biased(vref - vt + 127);
 #pragma unroll
@@ -344,7 +412,8 @@ __global__ __launch_bounds__(NW * 64) void attn_fp8_kernel(const AttnArgs a) {
                 vref = vt;
             }
         }
-        if (lane < 32) my_vs[lane] = x.vb == FP8_NAN ? INFINITY : pow2_biased(x.vb - vref + 127);
+        // V's scales, f16 (the smallest powers of two are f16's subnormals)
+        if (lane < 32) my_vs[lane] = (_Float16)(x.vb == FP8_NAN ? INFINITY : pow2_biased(x.vb - vref + 127));
         const float ks0 = pow2_biased(min(kb0 - kref, 0) + 127 + 7), ks1 = pow2_biased(min(kb1 - kref, 0) + 127 + 7);
 
         // ---- scores of this lane's column: key 16 half + i (32 rows) or 8 half + i
@@ -374,6 +443,8 @@ __global__ __launch_bounds__(NW * 64) void attn_fp8_kernel(const AttnArgs a) {
                 for (int i = 0; i < 4; ++i) s[4 * kb + i] = acc[i];
             }
         }
+
+        fetch_k(t + NW, x);
 
         // ---- masks: scores the row may not use
         uint32_t hidden = 0;
@@ -411,28 +482,40 @@ __global__ __launch_bounds__(NW * 64) void attn_fp8_kernel(const AttnArgs a) {
 #pragma unroll
             for (int db = 0; db < G::DB; ++db) o[db] *= f;
         }
-        const float off = P0 - m;
-        float vs[G::NP];
+        const float off = P0 - (m == -INFINITY ? 0.0f : m);
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        f16x8 vs[G::NP / 8];
 #pragma unroll
-        for (int i = 0; i < G::NP; i += 4) {
-            const f32x4 w = *reinterpret_cast<const f32x4*>(my_vs + G::NP * half + i);
+        for (int i = 0; i < G::NP / 8; ++i) vs[i] = *reinterpret_cast<const f16x8*>(my_vs + G::NP * half + 8 * i);
+        if (slow)  // (a hidden key's p is 0; a scale of infinity would still make it NaN)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) vs[i + e] = w[e];
-        }
+            for (int i = 0; i < G::NP; ++i) vs[i / 8][i % 8] = hidden >> i & 1 ? (_Float16)0.0f : vs[i / 8][i % 8];
         f16x8 ph[G::NP / 8], pl[G::NP / 8];
 #pragma unroll
-        for (int i = 0; i < G::NP; ++i) {
-            float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], kc, off));
-            if (slow && (hidden >> i & 1)) p = 0.0f;
-            l += p;
-            float pv = p * vs[i];
-            if (slow && (hidden >> i & 1)) pv = 0.0f;
-            const _Float16 hi = (_Float16)pv;
-            ph[i / 8][i % 8] = hi;
-            if constexpr (PL == 2) pl[i / 8][i % 8] = (_Float16)(pv - (float)hi);
+        for (int i = 0; i < G::NP; i += 2) {
+            const f32x2 p = {__builtin_amdgcn_exp2f(__builtin_fmaf(s[i], kc, off)),
+                             __builtin_amdgcn_exp2f(__builtin_fmaf(s[i + 1], kc, off))};
+            const f16x2 hi = __builtin_convertvector(p, f16x2);
+            if constexpr (PL == 1) {
+                // the sum is of the weights that the product takes
+                l = __builtin_amdgcn_fdot2(hi, f16x2{(_Float16)1.0f, (_Float16)1.0f}, l, false);
+            } else {
+                l += p[0];
+                l += p[1];
+                const f32x2 r = {p[0] - (float)hi[0], p[1] - (float)hi[1]};
+                const f16x2 lo = __builtin_convertvector(r, f16x2);
+                pl[i / 8][i % 8] = lo[0];
+                pl[i / 8][i % 8 + 1] = lo[1];
+            }
+            ph[i / 8][i % 8] = hi[0];
+            ph[i / 8][i % 8 + 1] = hi[1];
+        }
+#pragma unroll
+        for (int i = 0; i < G::NP / 8; ++i) {
+            ph[i] *= vs[i];
+            if constexpr (PL == 2) pl[i] *= vs[i];
         }
         // ---- O^T += V^T P^T
 #pragma unroll
@@ -443,31 +526,14 @@ __global__ __launch_bounds__(NW * 64) void attn_fp8_kernel(const AttnArgs a) {
                 o[db] = mfma(v8, ph[st], o[db]);
                 if constexpr (PL == 2) o[db] = mfma(v8, pl[st], o[db]);
             }
+        fetch_v(t + NW, x);
         // (the next tile's V scales are written after this tile's reads)
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     };
 
-    const int t_first = t0 + wave;
-    if (t_first < t1) {
-        Tile x, y;
-        if constexpr (G::BIG) {
-            for (int t = t_first; t < t1; t += NW) {
-                fetch(t, x);
-                step(t, x);
-            }
-        } else {
-        fetch(t_first, x);
-        for (int t = t_first; t < t1; t += 2 * NW) {
-            fetch(t + NW, y);
-            step(t, x);
-            if (t + NW >= t1) break;
-            fetch(t + 2 * NW, x);
-            step(t + NW, y);
-        }
-        }
-    }
+    for (int t = t_first; t < t1; t += NW) step(t, x);
     if constexpr (G::BIG) __syncthreads();  // (the merge area lies over the query rows)
 
     // ---- merge the waves
@@ -494,99 +560,148 @@ __global__ __launch_bounds__(NW * 64) void attn_fp8_kernel(const AttnArgs a) {
                 f32x4{o[db][i] * f, o[db][i + 1] * f, o[db][i + 2] * f, o[db][i + 3] * f};
         }
     __syncthreads();
-    const size_t prow0 = ((size_t)b * a.n_head_kv + g) * a.part_rows;
-    const size_t plane = (size_t)a.n_batch * a.n_head_kv * a.part_rows;
-    for (int p = tid; p < QR * (HD / 4); p += NW * 64) {
-        const int i = p / (HD / 4), d = p % (HD / 4) * 4, r = r0 + i;
-        if (r >= rows) continue;
-        float Mr = sm[i];
+    // ---- this workgroup's rows: the sum relative to the row maximum M, and L
+    constexpr int NT = NW * 64;
+    const int nr = min(QR, rows - r0), items = nr * (HD / 4);
+    auto state = [&](int i, int d, float& M, float& L) __attribute__((always_inline)) {
+        M = sm[i];
 #pragma unroll
-        for (int w = 1; w < NW; ++w) Mr = __builtin_fmaxf(Mr, sm[w * QR + i]);
+        for (int w = 1; w < NW; ++w) M = __builtin_fmaxf(M, sm[w * QR + i]);
         f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-        float L = 0.0f;
+        L = 0.0f;
 #pragma unroll
         for (int w = 0; w < NW; ++w) {
             const float mw = sm[w * QR + i], lw = sl[w * QR + i];
-            L += mw == -INFINITY ? (lw != lw ? lw : 0.0f) : lw * __builtin_amdgcn_exp2f(mw - Mr);
+            L += mw == -INFINITY ? (lw != lw ? lw : 0.0f) : lw * __builtin_amdgcn_exp2f(mw - M);
             acc += *reinterpret_cast<const f32x4*>(so + (w * QR + i) * G::OP + d);
         }
-        if (a.n_split > 1) {
-            const size_t at = (size_t)split * plane + prow0 + r;
-            *reinterpret_cast<f32x4*>(a.part_o + at * HD + d) = acc;
-            if (d == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(Mr, L);
+        return acc;
+    };
+    if (a.n_split == 1) {
+        for (int p = tid; p < items; p += NT) {
+            const int i = p / (HD / 4), d = p % (HD / 4) * 4;
+            float M, L;
+            const f32x4 acc = state(i, d, M, L);
+            write_out<HD>(a, S, g, r0 + i, d, acc * (1.0f / L));
+        }
+        return;
+    }
+
+    // ---- key splits.  Each workgroup stores its states with agent-scope
+    // accesses and waits until they are complete; one thread then takes the row
+    // block's ticket.  The one that draws n_split - 1 is the last: the others'
+    // stores are complete and its agent-scope loads see them.  It joins the
+    // splits in an order of its own (the same bits whichever comes last) and
+    // resets the ticket for the next call.  No workgroup waits for another.
+    // (Byte offsets of the workspace fit 32 bits: the host checks.)
+    const size_t prow0 = ((size_t)b * a.n_head_kv + g) * a.part_rows + r0;
+    const size_t plane = (size_t)a.n_batch * a.n_head_kv * a.part_rows;
+    const __amdgpu_buffer_rsrc_t ro = make_rsrc(a.part_o, 0xffffffffu);
+    const __amdgpu_buffer_rsrc_t rm = make_rsrc(a.part_ml, 0xffffffffu);
+    for (int p = tid; p < items; p += NT) {
+        const int i = p / (HD / 4), d = p % (HD / 4) * 4;
+        float M, L;
+        const f32x4 acc = state(i, d, M, L);
+        const size_t at = (size_t)split * plane + prow0 + i;
+        store_sc1(ro, (int)((at * HD + d) * 4), acc);
+        // (a NaN without any finite score must not pass for a row without keys)
+        if (d == 0) store2_sc1(rm, (int)(at * 8), L != L && M == -INFINITY ? 0.0f : M, L);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    int* const tk = a.ticket + (b * a.n_head_kv + g) * a.rowgroups + rb;
+    if (tid == 0) *stick = __hip_atomic_fetch_add(tk, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    if (*stick != a.n_split - 1) return;
+    if (tid == 0) __hip_atomic_store(tk, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    // Few rows leave threads over: `share` threads take an item's splits (thread
+    // k of them takes splits k, k + share, ...), so that all loads of a wide split
+    // are in flight together; their states join through LDS.
+    int share = 1;
+    while (2 * share * items <= NT) share *= 2;
+    float* const sj = so;  // [share][items][6]
+    for (int p = tid; p < share * items; p += NT) {
+        const int k = p / items, it = p - k * items, i = it / (HD / 4), d = it % (HD / 4) * 4;
+        float M = -INFINITY, L = 0.0f;
+        f32x4 acc[1] = {{0.0f, 0.0f, 0.0f, 0.0f}};
+        for (int s0 = k; s0 < a.n_split; s0 += 8 * share) {
+            float m[8], l[8];
+            f32x4 o8[8][1];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int sp = s0 + j * share;
+                const size_t at = (size_t)min(sp, a.n_split - 1) * plane + prow0 + i;
+                const float2 ml = load2_sc1(rm, (int)(at * 8));
+                o8[j][0] = load_sc1(ro, (int)((at * HD + d) * 4));
+                m[j] = sp < a.n_split ? ml.x : -INFINITY;
+                l[j] = ml.y;
+            }
+            __builtin_amdgcn_sched_barrier(0);  // (every load above before any wait)
+            merge_split_states<8, 1>(M, L, acc, m, l, o8);
+        }
+        if (share == 1) {
+            write_out<HD>(a, S, g, r0 + i, d, acc[0] * (1.0f / L));
         } else {
-            write_out<HD>(a, S, g, r, d, acc * (1.0f / L));
+            float* t = sj + p * 6;
+            t[0] = M;
+            t[1] = L;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) t[2 + e] = acc[0][e];
         }
     }
-}
-
-// Joins the key splits: one thread per (packed row, four values).
-template <int HD>
-__global__ __launch_bounds__(256) void fp8_merge_kernel(const AttnArgs a) {
-    const size_t plane = (size_t)a.n_batch * a.n_head_kv * a.part_rows;
-    const size_t item = (size_t)blockIdx.x * 256 + threadIdx.x;
-    if (item >= plane * (HD / 4)) return;
-    const size_t prow = item / (HD / 4);
-    const int d = (int)(item % (HD / 4)) * 4;
-    const int bg = (int)(prow / a.part_rows), r = (int)(prow % a.part_rows);
-    const int b = bg / a.n_head_kv, g = bg % a.n_head_kv;
-    const AttnSlot& S = a.slot[b];
-    if (r >= a.group * S.nq) return;
-    float M = -INFINITY;
-    for (int s = 0; s < a.n_split; ++s) M = __builtin_fmaxf(M, a.part_ml[((size_t)s * plane + prow) * 2]);
-    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-    float L = 0.0f;
-    for (int s = 0; s < a.n_split; ++s) {
-        const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + ((size_t)s * plane + prow) * 2);
-        const f32x4 w = *reinterpret_cast<const f32x4*>(a.part_o + ((size_t)s * plane + prow) * HD + d);
-        const float f = ml.x == -INFINITY ? (ml.y != ml.y ? ml.y : 0.0f) : __builtin_amdgcn_exp2f(ml.x - M);
-        L += f * ml.y;
-        acc += w * f;
+    if (share == 1) return;
+    __syncthreads();
+    if (tid < items) {
+        float M = -INFINITY, L = 0.0f;
+        f32x4 acc[1] = {{0.0f, 0.0f, 0.0f, 0.0f}};
+        for (int k = 0; k < share; ++k) {
+            const float* t = sj + (k * items + tid) * 6;
+            const float m[1] = {t[0]}, l[1] = {t[1]};
+            const f32x4 w[1][1] = {{{t[2], t[3], t[4], t[5]}}};
+            merge_split_states<1, 1>(M, L, acc, m, l, w);
+        }
+        write_out<HD>(a, S, g, r0 + tid / (HD / 4), tid % (HD / 4) * 4, acc[0] * (1.0f / L));
     }
-    write_out<HD>(a, S, g, r, d, acc * (1.0f / L));
 }
 
-template <int HD, int QR, int PL>
+template <int HD, int QR, int PL, int NW>
 hipError_t launch(const AttnArgs& a, hipStream_t st) {
-    using G = Fp8Geo<HD, QR, PL>;
+    using G = Fp8Geo<HD, QR, PL, NW>;
     static_assert(G::LDS <= 160 * 1024, "LDS");
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(attn_fp8_kernel<HD, QR, PL>),
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(attn_fp8_kernel<HD, QR, PL, NW>),
                                              hipFuncAttributeMaxDynamicSharedMemorySize, (int)G::LDS);
     if (e != hipSuccess) return e;
     const dim3 grid((unsigned)((a.n_wg + 7) / 8 * 8));
-    hipLaunchKernelGGL((attn_fp8_kernel<HD, QR, PL>), grid, dim3(NW * 64), G::LDS, st, a);
+    hipLaunchKernelGGL((attn_fp8_kernel<HD, QR, PL, NW>), grid, dim3(NW * 64), G::LDS, st, a);
     return hipGetLastError();
 }
 
 template <int HD>
 hipError_t launch_hd(const LaunchPlan& p, const AttnArgs& a, hipStream_t st) {
     const bool one = a.q_bf16 && a.o_bf16;
-    hipError_t e;
+    hipError_t e = hipErrorInvalidValue;
     if constexpr (HD <= 128) {
-        if (!p.w16)
-            e = one ? launch<HD, 32, 1>(a, st) : launch<HD, 32, 2>(a, st);
+        if (p.w16)
+            e = p.waves == 8 ? (one ? launch<HD, 16, 1, 8>(a, st) : launch<HD, 16, 2, 8>(a, st))
+                             : (one ? launch<HD, 16, 1, 4>(a, st) : launch<HD, 16, 2, 4>(a, st));
         else
-            e = one ? launch<HD, 16, 1>(a, st) : launch<HD, 16, 2>(a, st);
-    } else {
-        if (!p.w16) return hipErrorInvalidValue;
-        e = one ? launch<HD, 16, 1>(a, st) : launch<HD, 16, 2>(a, st);
+            e = p.waves == 8 ? (one ? launch<HD, 32, 1, 8>(a, st) : launch<HD, 32, 2, 8>(a, st))
+                             : (one ? launch<HD, 32, 1, 4>(a, st) : launch<HD, 32, 2, 4>(a, st));
+    } else if (p.w16 && p.waves == 4) {
+        e = one ? launch<HD, 16, 1, 4>(a, st) : launch<HD, 16, 2, 4>(a, st);
     }
-    if (e != hipSuccess || p.n_split <= 1) return e;
-    const size_t items = (size_t)a.n_batch * a.n_head_kv * a.part_rows * (HD / 4);
-    hipLaunchKernelGGL(fp8_merge_kernel<HD>, dim3((unsigned)((items + 255) / 256)), dim3(256), 0, st, a);
-    return hipGetLastError();
+    return e;
 }
 
 }  // namespace
 
 LaunchPlan plan_fp8(int hd_tile, int n_batch, int n_head_kv, int group, int max_nq, int max_nk, int mask, int n_cu,
-                    int force_split) {
+                    int force_split, int max_tickets) {
     LaunchPlan p{};
     p.hd_tile = hd_tile;
     p.block_n = 32;
     p.rb = 1;
     p.kq = 1;
-    p.waves = NW;
     p.stages = 1;
     p.mask = mask;
     p.kernel = KERNEL_FP8;
@@ -595,12 +710,18 @@ LaunchPlan plan_fp8(int hd_tile, int n_batch, int n_head_kv, int group, int max_
     p.rowgroups = (group * max_nq + qr - 1) / qr;
     const int base = n_batch * n_head_kv * p.rowgroups;
     const int tiles = std::max(1, (max_nk + 31) / 32);
+    // 8 waves where a workgroup per CU is all there is, else 4 (two workgroups per CU)
+    p.waves = hd_tile <= 128 && base <= n_cu ? 8 : 4;
+    const int slots = p.waves == 8 ? n_cu : 2 * n_cu;
     int split = 1;
     if (force_split > 0)
         split = force_split;
-    else if (2 * base <= 2 * n_cu)
-        split = std::min(2 * n_cu / base, (tiles + NW - 1) / NW);
+    else if (2 * base <= slots)
+        split = std::min(slots / base, (tiles + p.waves - 1) / p.waves);
     p.n_split = std::max(1, split);
+    // (the splits' tickets, and 32-bit offsets into their workspace: only a
+    // forced split can outgrow them)
+    if (base > max_tickets || split_workspace_bytes(p, n_batch, n_head_kv) >= ((size_t)1 << 31)) p.n_split = 1;
     p.n_workgroups = base * p.n_split;
     return p;
 }

@@ -1730,8 +1730,8 @@ hipError_t launch_attention(const LaunchPlan& p, AttnArgs& a, hipStream_t st) {
     a.mg_hkv = div_magic(a.n_head_kv, p.n_workgroups);
     a.part_rows = p.rowgroups * p.rb * 32;
     a.ring_rot = p.rotate ? 1 : 0;
+    if (p.kernel == KERNEL_FP8) return p.n_split > 1 && !a.ticket ? hipErrorInvalidValue : launch_fp8(p, a, st);
     if (p.kernel != KERNEL_STREAMS) a.ticket = nullptr;  // (the others always merge in a second kernel)
-    if (p.kernel == KERNEL_FP8) return launch_fp8(p, a, st);  // (it joins its own splits)
     hipError_t e = p.kernel == KERNEL_STREAMS ? launch_ring(p, a, st)
                    : p.kernel == KERNEL_HILO  ? launch_hilo(p, a, st)
                    : p.rows                   ? launch_rows(p, a, st)

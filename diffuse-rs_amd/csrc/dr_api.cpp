@@ -1351,7 +1351,7 @@ static dr::LaunchPlan plan_for(dr_ctx* ctx, const dr::AttnArgs& a, int hd, int m
     // kernel family is forced (then the lo half is not read)
     if (a.fp8)
         return dr::plan_fp8(hd_tile_for((size_t)hd), a.n_batch, a.n_head_kv, a.group, max_nq, a.key_band, mask,
-                            ctx->n_cu, ctx->force_split);
+                            ctx->n_cu, ctx->force_split, (int)TICKETS);
     const bool hilo_asked = ctx->force_kernel == dr::KERNEL_AUTO || ctx->force_kernel == dr::KERNEL_HILO;
     const bool bf16_rows = a.q_bf16 || a.o_bf16;
     if (a.slot[0].klo && hilo_asked && !bf16_rows) return plan_hilo(ctx, a, hd, max_nq, max_nk, mask);
@@ -1471,6 +1471,8 @@ static int launch_plan(dr_ctx* ctx, dr::AttnArgs& a, const dr::LaunchPlan& p, bo
         const size_t blocks = (size_t)a.n_batch * a.n_head_kv * p.rowgroups;
         if (blocks <= TICKETS && ws < ((size_t)1 << 31)) a.ticket = static_cast<int*>(ctx->tick.p);
     }
+    // (an 8 bit layer's kernel always merges its own, and its plan keeps to both limits)
+    if (p.kernel == dr::KERNEL_FP8 && p.n_split > 1) a.ticket = static_cast<int*>(ctx->tick.p);
     hipError_t e = dr::launch_attention(p, a, ctx->stream);
     if (e != hipSuccess) return hip_fail(e, "attention launch");
     ctx->last = p;

@@ -68,7 +68,8 @@ struct AttnArgs {
     // Per-row-block arrival counters [batch*kv head][rowgroups], zero between
     // calls, or nullptr.  Set: the last split of each row block to finish
     // merges the partials in-kernel (agent-scope accesses) and resets its
-    // counter; no split_merge_kernel follows.  The per-wave-stream kernel only.
+    // counter; no split_merge_kernel follows.  The per-wave-stream kernel, and
+    // always that of DR_PRECISION_FP8 layers.
     int* ticket;
     int q_bf16;                    // Q rows are bf16 (the per-wave-stream kernel reads them)
     int o_bf16;                    // output rows are bf16 (the per-wave-stream kernel writes them)
@@ -393,7 +394,7 @@ int hilo32_rows(int hd_tile);  // the same of attn_hilo32_kernel (0: head dim no
 // DR_PRECISION_FP8 layers: the attention's plan and kernels (attn_fp8.hip), the
 // store and the gather (kv_fp8.hip).
 LaunchPlan plan_fp8(int hd_tile, int n_batch, int n_head_kv, int group, int max_nq, int max_nk, int mask, int n_cu,
-                    int force_split);
+                    int force_split, int max_tickets);
 hipError_t launch_fp8(const LaunchPlan& p, const AttnArgs& a, hipStream_t st);
 hipError_t launch_store_fp8(int hd_tile, const StoreArgs& a, hipStream_t st);
 hipError_t launch_gather_fp8(int hd_tile, const GatherArgs& a, hipStream_t st);
