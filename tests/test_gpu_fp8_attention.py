@@ -124,6 +124,9 @@ CASES = {
     "window_wide": (2, 2, 128, 90, range(40, 90), 100000, None, 0),
     "scattered": (4, 4, 128, 400, [0, 1, 5, 31, 32, 100, 163, 255, 256, 398, 399], 120, 200, 0),
     "group_spans_blocks": (20, 2, 128, 130, range(100, 130), 40, 110, 0),
+    "rows_one_past_a_block": (2, 2, 128, 400, range(303, 400), None, None, 0),
+    "many_blocks_causal": (8, 8, 128, 1500, range(1500), None, 1400, 0),
+    "many_blocks_64_window": (16, 8, 64, 900, range(0, 900, 2), 33, None, 0),
 }
 
 
