@@ -28,39 +28,48 @@ struct Fp8Geo {
     static constexpr size_t Q_BYTES = (size_t)PL * QR * QP * 2;
     static constexpr size_t O_BYTES = (size_t)NW * QR * (HD + 4) * 4;
     static constexpr size_t BODY = O_BYTES > Q_BYTES ? O_BYTES : Q_BYTES;
-    // then: per-row scales, wave states, V scales (f16) of each wave's tile, the ticket
-    static constexpr size_t LDS = BODY + QR * 4 + 2 * NW * QR * 4 + NW * 32 * 2 + 16;
+    // then: per-row scales, wave states, row states, V scales (f16) of each wave's tile, the ticket
+    static constexpr size_t LDS = BODY + QR * 4 + 2 * NW * QR * 4 + 2 * QR * 4 + NW * 32 * 2 + 16;
 };
 
-// The query rows r0 .. r0 + ROWS - 1: scaled by a power of two each (inverse to
-// srow), split into PL planes of f16 in sq [PL][ROWS][QP].  A thread takes 16
-// values of a row, all rows of a pass in flight at once.
-template <int HD, int ROWS, int PL, int NT, int QP>
-__device__ __forceinline__ void stage_queries(const AttnArgs& a, const AttnSlot& S, int g, int r0, int rows,
-                                              _Float16* sq, float* srow) {
-    constexpr int LPR = HD / 16, PER = NT / LPR;  // lanes per row, rows per pass
-    const int tid = threadIdx.x, d0 = tid % LPR * 16;
+// The query rows r0 .. r0 + QR - 1 on their way to LDS: a thread takes 16 values
+// of a row, all rows of a pass in flight at once.
+template <int HD, int QR, int PL, int NT, int QP>
+struct Fp8Queries {
+    static constexpr int LPR = HD / 16, PER = NT / LPR, PASSES = (QR + PER - 1) / PER;  // lanes per row, rows per pass
+    f32x4 y[PASSES][4];
+
+    __device__ __forceinline__ void load(const AttnArgs& a, const AttnSlot& S, int g, int r0, int rows) {
 #pragma unroll
-    for (int p = 0; p < (ROWS + PER - 1) / PER; ++p) {
-        const int i = p * PER + tid / LPR;
-        // (a row past the last is the last again; lanes of a row agree)
-        const int r = min(r0 + min(i, ROWS - 1), rows - 1), qi = r / a.group;
-        f32x4 y[4];
-        load_query<HD>(a, S, qi, g * a.group + r - qi * a.group, d0, y);
-        float up, down;
-        query_scale<LPR>(a, y, up, down);
-        if (i < ROWS) {
-            if (tid % LPR == 0) srow[i] = down;
+        for (int p = 0; p < PASSES; ++p) {
+            // (a row past the last is the last again; lanes of a row agree)
+            const int i = p * PER + (int)threadIdx.x / LPR, r = min(r0 + min(i, QR - 1), rows - 1);
+            const int qi = udiv(r, a.group, a.mg_group);
+            load_query<HD>(a, S, qi, g * a.group + r - qi * a.group, (int)threadIdx.x % LPR * 16, y[p]);
+        }
+    }
+    // scaled by a power of two each (inverse to srow), split into PL planes of f16
+    // in sq [PL][QR][QP]
+    __device__ __forceinline__ void stage(const AttnArgs& a, _Float16* sq, float* srow) const {
+        const int tid = threadIdx.x, d0 = tid % LPR * 16;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                f16x8 hi, lo;
-                split8(y, h, up, hi, lo);
-                *reinterpret_cast<f16x8*>(sq + i * QP + d0 + 8 * h) = hi;
-                if constexpr (PL == 2) *reinterpret_cast<f16x8*>(sq + (ROWS + i) * QP + d0 + 8 * h) = lo;
+        for (int p = 0; p < PASSES; ++p) {
+            const int i = p * PER + tid / LPR;
+            float up, down;
+            query_scale<LPR>(a, y[p], up, down);
+            if (i < QR) {
+                if (tid % LPR == 0) srow[i] = down;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    f16x8 hi, lo;
+                    split8(y[p], h, up, hi, lo);
+                    *reinterpret_cast<f16x8*>(sq + i * QP + d0 + 8 * h) = hi;
+                    if constexpr (PL == 2) *reinterpret_cast<f16x8*>(sq + (QR + i) * QP + d0 + 8 * h) = lo;
+                }
             }
         }
     }
-}
+};
 
 template <int HD, int QR, int PL, int NW>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(HD > 256 ? 1 : 2)))
@@ -72,7 +81,8 @@ void attn_fp8_kernel(const AttnArgs a) {
     float* const srow = reinterpret_cast<float*>(lds + G::BODY);
     float* const sm = srow + QR;
     float* const sl = sm + NW * QR;
-    _Float16* const svs = reinterpret_cast<_Float16*>(sl + NW * QR);  // [NW][32]
+    float* const sr = sl + NW * QR;
+    _Float16* const svs = reinterpret_cast<_Float16*>(sr + 2 * QR);  // [NW][32]
     int* const stick = reinterpret_cast<int*>(svs + NW * 32);
 
     const Fp8Place at(a);
@@ -83,9 +93,12 @@ void attn_fp8_kernel(const AttnArgs a) {
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int col = lane % QR, half = lane / QR;  // query column; 0..1 (0..3 with 16 rows)
 
+    Fp8Queries<HD, QR, PL, NW * 64, G::QP> queries;
+    queries.load(a, S, at.g, r0, rows);
+
     // ---- the key tiles that this workgroup's rows can see
-    const int q_lo = uniform_pos(S, r0 / a.group), q_hi = uniform_pos(S, (min(r0 + QR, rows) - 1) / a.group);
-    const int my_pos = row_pos(S, min(r0 + col, rows - 1) / a.group);
+    const int q_lo = uniform_pos(S, udiv(r0, a.group, a.mg_group)), q_hi = uniform_pos(S, udiv(min(r0 + QR, rows) - 1, a.group, a.mg_group));
+    const int my_pos = row_pos(S, udiv(min(r0 + col, rows - 1), a.group, a.mg_group));
     int kt_lo, kt_hi, t0, t1;
     row_tiles(a, S.nk, q_lo, q_hi, kt_lo, kt_hi);
     split_tile_range(kt_lo, kt_hi, a.n_split, at.split, t0, t1);
@@ -144,11 +157,11 @@ void attn_fp8_kernel(const AttnArgs a) {
 
     Tile x;
     const int t_first = t0 + wave;
-    if (t_first < t1) {  // (in flight while the query rows are staged)
+    if (t_first < t1) {  // (in flight behind the query rows while those are staged)
         fetch_k(t_first, x);
         fetch_v(t_first, x);
     }
-    stage_queries<HD, QR, PL, NW * 64, G::QP>(a, S, at.g, r0, rows, sq, srow);
+    queries.stage(a, sq, srow);
     __syncthreads();
     auto staged = [&](int p, int s) __attribute__((always_inline)) {
         // K piece j of a lane holds 16 values, steps 2j and 2j + 1
@@ -185,7 +198,7 @@ void attn_fp8_kernel(const AttnArgs a) {
         fetch_v(t + NW, x);
     }
     if constexpr (G::BIG) __syncthreads();  // (the merge area lies over the query rows)
-    fp8_finish<HD, QR, PL, NW>(a, at, st, r0, reinterpret_cast<float*>(lds), sm, sl, stick);
+    fp8_finish<HD, QR, PL, NW>(a, at, st, r0, reinterpret_cast<float*>(lds), sm, sl, sr, stick);
 }
 
 template <int HD, int QR, int PL, int NW>

@@ -1728,6 +1728,7 @@ hipError_t launch_attention(const LaunchPlan& p, AttnArgs& a, hipStream_t st) {
     a.mg_split = div_magic(a.n_split, p.n_workgroups);
     a.mg_rowgroups = div_magic(a.rowgroups, p.n_workgroups);
     a.mg_hkv = div_magic(a.n_head_kv, p.n_workgroups);
+    a.mg_group = div_magic(a.group, p.rowgroups * p.rb * 32);
     a.part_rows = p.rowgroups * p.rb * 32;
     a.ring_rot = p.rotate ? 1 : 0;
     if (p.kernel == KERNEL_FP8) return p.n_split > 1 && !a.ticket ? hipErrorInvalidValue : launch_fp8(p, a, st);

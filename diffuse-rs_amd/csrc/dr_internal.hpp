@@ -85,6 +85,7 @@ struct AttnArgs {
     // (host planning only) a DR_PRECISION_FP8 layer: slot[].k and .vt are its
     // code planes and .klo its scale bytes (fp8_common.hpp)
     int fp8;
+    uint32_t mg_group;  // division magic of packed rows by group (udiv)
 };
 static_assert(offsetof(AttnArgs, slot) == 64, "scalar block of AttnArgs is one 64-byte line");
 

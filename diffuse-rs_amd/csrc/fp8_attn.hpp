@@ -199,7 +199,7 @@ __device__ __forceinline__ void split8(const f32x4 (&y)[4], int h, float up, f16
 // out[row] of packed row r, four values from d on
 template <int HD>
 __device__ __forceinline__ void write_out(const AttnArgs& a, const AttnSlot& S, int g, int r, int d, const f32x4& y) {
-    const int qi = r / a.group, head = g * a.group + (r - qi * a.group);
+    const int qi = udiv(r, a.group, a.mg_group), head = g * a.group + (r - qi * a.group);
     const size_t o = (size_t)qi * a.o_rstride + (size_t)head * a.hd + d;
     if (a.o_bf16) {
         uint16_t* to = reinterpret_cast<uint16_t*>(S.out) + o;
@@ -442,22 +442,22 @@ struct Fp8Place {
         const int per = (a.n_wg + 7) / 8;
         int id = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
         ok = (int)(blockIdx.x >> 3) < per && id < a.n_wg;
-        rg = id % a.rowgroups;
-        id /= a.rowgroups;
-        split = id % a.n_split;
-        id /= a.n_split;
-        g = id % a.n_head_kv;
-        b = id / a.n_head_kv;
+        const int t = udiv(id, a.rowgroups, a.mg_rowgroups);
+        rg = id - t * a.rowgroups;
+        const int u = a.n_split > 1 ? udiv(t, a.n_split, a.mg_split) : t;
+        split = t - u * a.n_split;
+        b = udiv(u, a.n_head_kv, a.mg_hkv);
+        g = u - b * a.n_head_kv;
     }
 };
 inline unsigned fp8_grid(const AttnArgs& a) { return (unsigned)((a.n_wg + 7) / 8 * 8); }
 
 // The end of a workgroup of NW waves on one block of QR rows: their states meet
-// in LDS, the rows leave, or, with key splits, join the other splits'.  LDS: so [NW][QR][HD + 4] floats, sm and sl [NW][QR], stick
-// one int; so may lie over what the waves read before (a barrier precedes).
+// in LDS, the rows leave, or, with key splits, join the other splits'.  LDS: so [NW][QR][HD + 4] floats, sm and sl [NW][QR], sr
+// [2][QR], stick one int; so may lie over what the waves read before (a barrier precedes).
 template <int HD, int QR, int PL, int NW>
 __device__ __forceinline__ void fp8_finish(const AttnArgs& a, const Fp8Place& at, const Fp8State<HD, QR, PL>& st, int r0,
-                                           float* so, float* sm, float* sl, int* stick) {
+                                           float* so, float* sm, float* sl, float* sr, int* stick) {
     using T = Fp8State<HD, QR, PL>;
     constexpr int OP = HD + 4, NT = NW * 64;
     const AttnSlot& S = a.slot[at.b];
@@ -471,6 +471,16 @@ __device__ __forceinline__ void fp8_finish(const AttnArgs& a, const Fp8Place& at
     float M = sm[col];
 #pragma unroll
     for (int k = 1; k < NW; ++k) M = __builtin_fmaxf(M, sm[k * QR + col]);
+    if (tid < QR) {  // the row's maximum and sum over the waves
+        float L = 0.0f;
+#pragma unroll
+        for (int k = 0; k < NW; ++k) {
+            const float mw = sm[k * QR + col], lw = sl[k * QR + col];
+            L += mw == -INFINITY ? (lw != lw ? lw : 0.0f) : lw * __builtin_amdgcn_exp2f(mw - M);
+        }
+        sr[col] = M;
+        sr[QR + col] = L;
+    }
     const float f = st.weight(M);
 #pragma unroll
     for (int db = 0; db < T::DB; ++db)
@@ -479,28 +489,18 @@ __device__ __forceinline__ void fp8_finish(const AttnArgs& a, const Fp8Place& at
             *reinterpret_cast<f32x4*>(so + (wave * QR + col) * OP + T::dim(db, i, half)) =
                 f32x4{st.o[db][i] * f, st.o[db][i + 1] * f, st.o[db][i + 2] * f, st.o[db][i + 3] * f};
     __syncthreads();
-    // row i of the workgroup: the sum relative to the row maximum M, and L
     const int nr = min(QR, S.nq * a.group - r0), items = nr * (HD / 4);
-    auto state = [&](int i, int d, float& Mi, float& L) __attribute__((always_inline)) {
-        Mi = sm[i];
+    // four values of row i, relative to its maximum
+    auto joined = [&](int i, int d) __attribute__((always_inline)) {
+        f32x4 acc = *reinterpret_cast<const f32x4*>(so + i * OP + d);
 #pragma unroll
-        for (int k = 1; k < NW; ++k) Mi = __builtin_fmaxf(Mi, sm[k * QR + i]);
-        f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-        L = 0.0f;
-#pragma unroll
-        for (int k = 0; k < NW; ++k) {
-            const float mw = sm[k * QR + i], lw = sl[k * QR + i];
-            L += mw == -INFINITY ? (lw != lw ? lw : 0.0f) : lw * __builtin_amdgcn_exp2f(mw - Mi);
-            acc += *reinterpret_cast<const f32x4*>(so + (k * QR + i) * OP + d);
-        }
+        for (int k = 1; k < NW; ++k) acc += *reinterpret_cast<const f32x4*>(so + (k * QR + i) * OP + d);
         return acc;
     };
     if (a.n_split == 1) {
         for (int p = tid; p < items; p += NT) {
             const int i = p / (HD / 4), d = p % (HD / 4) * 4;
-            float Mi, L;
-            const f32x4 acc = state(i, d, Mi, L);
-            write_out<HD>(a, S, at.g, r0 + i, d, acc * (1.0f / L));
+            write_out<HD>(a, S, at.g, r0 + i, d, joined(i, d) * (1.0f / sr[QR + i]));
         }
         return;
     }
@@ -518,11 +518,11 @@ __device__ __forceinline__ void fp8_finish(const AttnArgs& a, const Fp8Place& at
     const __amdgpu_buffer_rsrc_t rm = make_rsrc(a.part_ml, 0xffffffffu);
     for (int p = tid; p < items; p += NT) {
         const int i = p / (HD / 4), d = p % (HD / 4) * 4;
-        float Mi, L;
-        const f32x4 acc = state(i, d, Mi, L);
+        const f32x4 acc = joined(i, d);
         const size_t row = (size_t)at.split * plane + prow0 + i;
         store_sc1(ro, (int)((row * HD + d) * 4), acc);
         // (a NaN without any finite score must not pass for a row without keys)
+        const float Mi = sr[i], L = sr[QR + i];
         if (d == 0) store2_sc1(rm, (int)(row * 8), L != L && Mi == -INFINITY ? 0.0f : Mi, L);
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
