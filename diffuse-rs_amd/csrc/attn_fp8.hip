@@ -13,6 +13,7 @@
 #include "fp8_attn.hpp"
 
 #include <algorithm>
+#include <cmath>
 
 namespace dr {
 namespace {
@@ -30,45 +31,6 @@ struct Fp8Geo {
     static constexpr size_t BODY = O_BYTES > Q_BYTES ? O_BYTES : Q_BYTES;
     // then: per-row scales, wave states, row states, V scales (f16) of each wave's tile, the ticket
     static constexpr size_t LDS = BODY + QR * 4 + 2 * NW * QR * 4 + 2 * QR * 4 + NW * 32 * 2 + 16;
-};
-
-// The query rows r0 .. r0 + QR - 1 on their way to LDS: a thread takes 16 values
-// of a row, all rows of a pass in flight at once.
-template <int HD, int QR, int PL, int NT, int QP>
-struct Fp8Queries {
-    static constexpr int LPR = HD / 16, PER = NT / LPR, PASSES = (QR + PER - 1) / PER;  // lanes per row, rows per pass
-    f32x4 y[PASSES][4];
-
-    __device__ __forceinline__ void load(const AttnArgs& a, const AttnSlot& S, int g, int r0, int rows) {
-#pragma unroll
-        for (int p = 0; p < PASSES; ++p) {
-            // (a row past the last is the last again; lanes of a row agree)
-            const int i = p * PER + (int)threadIdx.x / LPR, r = min(r0 + min(i, QR - 1), rows - 1);
-            const int qi = udiv(r, a.group, a.mg_group);
-            load_query<HD>(a, S, qi, g * a.group + r - qi * a.group, (int)threadIdx.x % LPR * 16, y[p]);
-        }
-    }
-    // scaled by a power of two each (inverse to srow), split into PL planes of f16
-    // in sq [PL][QR][QP]
-    __device__ __forceinline__ void stage(const AttnArgs& a, _Float16* sq, float* srow) const {
-        const int tid = threadIdx.x, d0 = tid % LPR * 16;
-#pragma unroll
-        for (int p = 0; p < PASSES; ++p) {
-            const int i = p * PER + tid / LPR;
-            float up, down;
-            query_scale<LPR>(a, y[p], up, down);
-            if (i < QR) {
-                if (tid % LPR == 0) srow[i] = down;
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    f16x8 hi, lo;
-                    split8(y[p], h, up, hi, lo);
-                    *reinterpret_cast<f16x8*>(sq + i * QP + d0 + 8 * h) = hi;
-                    if constexpr (PL == 2) *reinterpret_cast<f16x8*>(sq + (QR + i) * QP + d0 + 8 * h) = lo;
-                }
-            }
-        }
-    }
 };
 
 template <int HD, int QR, int PL, int NW>
@@ -223,7 +185,9 @@ hipError_t launch_hd(const LaunchPlan& p, const AttnArgs& a, hipStream_t st) {
         else
             e = p.waves == 8 ? (one ? launch<HD, 32, 1, 8>(a, st) : launch<HD, 32, 2, 8>(a, st))
                              : (one ? launch<HD, 32, 1, 4>(a, st) : launch<HD, 32, 2, 4>(a, st));
-    } else if (p.w16 && p.waves == 4) {
+    } else if (!p.w16) {
+        return HD > 256 ? launch_fp8_wide(a, st) : hipErrorInvalidValue;
+    } else if (p.waves == 4) {
         e = one ? launch<HD, 16, 1, 4>(a, st) : launch<HD, 16, 2, 4>(a, st);
     }
     return e;
@@ -231,29 +195,56 @@ hipError_t launch_hd(const LaunchPlan& p, const AttnArgs& a, hipStream_t st) {
 
 }  // namespace
 
+// The launch shape of an 8 bit call.
+//
+// Row blocks: 16 rows where O^T of 32 would not fit the registers (head dims above
+// 128) or where 16 hold all, else 32.  Head dims 257-512 with many rows take 64 in
+// the wide kernel: it starts slower (24 us against 8 of fixed time) but a 32-key
+// tile costs it 1.6 us for 64 rows, where four waves take 2.6 us for four tiles of
+// 16 rows.  Measured, 16-row / wide, f32 rows over 2 KV heads of 512 dims, group 8:
+// 256 rows over 600 keys 27 / 36 us, over 4352 101 / 91, over 32768 680 / 531;
+// 600 rows over 600 keys 69 / 48, over 4352 277 / 243.  (Few row blocks would be
+// split often, and 64 rows are dear to join: 32 rows over 32768 keys 117 / 147.)
+//
+// Waves: 8 where a workgroup per CU is all there is, else 4, two workgroups per CU.
+//
+// Key splits.  A step of a workgroup (one tile of each wave, or of the wide kernel)
+// takes `step` us, a split's join reads its rows of floats at 13000 a us, and a join
+// at all about 2 us: so steps / n * step + n * floats / 13000 is smallest at n =
+// sqrt(steps * step * 13000 / floats).  More workgroups than CUs only wait for each
+// other (16 rows x 8 heads of 256 dims over 32768 keys: 16 splits 38 us, 32 61).
+// A split for every tile and CU, as cheap single rows take it, costs more rows up to
+// twice the time (5 rows x 4 heads of 512 dims, 4352 keys: 34 splits 44 us, 9 33).
 LaunchPlan plan_fp8(int hd_tile, int n_batch, int n_head_kv, int group, int max_nq, int max_nk, int mask, int n_cu,
                     int force_split, int max_tickets) {
     LaunchPlan p{};
     p.hd_tile = hd_tile;
     p.block_n = 32;
-    p.rb = 1;
-    p.kq = 1;
     p.stages = 1;
     p.mask = mask;
     p.kernel = KERNEL_FP8;
-    p.w16 = hd_tile > 128 || group * max_nq <= 16;
-    const int qr = p.w16 ? 16 : 32;
-    p.rowgroups = (group * max_nq + qr - 1) / qr;
+    const int tiles = std::max(1, (max_nk + 31) / 32), packed = group * max_nq;
+    const int64_t base16 = (int64_t)n_batch * n_head_kv * ((packed + 15) / 16);
+    const bool wide = hd_tile > 256 && packed > 32 && (base16 > n_cu || (4 * base16 >= n_cu && base16 * tiles >= (int64_t)120 * n_cu));
+    p.w16 = !wide && (hd_tile > 128 || packed <= 16);
+    p.rb = wide ? 2 : 1;
+    const int qr = p.w16 ? 16 : 32 * p.rb;
+    p.rowgroups = (packed + qr - 1) / qr;
     const int base = n_batch * n_head_kv * p.rowgroups;
-    const int tiles = std::max(1, (max_nk + 31) / 32);
-    // 8 waves where a workgroup per CU is all there is, else 4 (two workgroups per CU)
-    p.waves = hd_tile <= 128 && base <= n_cu ? 8 : 4;
-    p.kq = p.waves;
+    p.waves = wide || (hd_tile <= 128 && base <= n_cu) ? 8 : 4;
+    p.kq = wide ? 1 : p.waves;
     int split = 1;
-    if (force_split > 0)
+    if (force_split > 0) {
         split = force_split;
-    else if (2 * base <= n_cu)
-        split = std::min((p.waves == 8 ? 1 : 2) * n_cu / base, (tiles + p.waves - 1) / p.waves);
+    } else if (2 * base <= n_cu) {
+        const float step = wide ? 1.6f : hd_tile > 256 ? 2.6f : p.w16 ? 1.0f : 1.3f;
+        const int steps = (tiles + p.kq - 1) / p.kq;
+        const float join = (float)(std::min(qr, packed) * hd_tile) / 13000.0f;
+        split = std::clamp((int)std::sqrt((float)steps * step / join), 1, std::min(n_cu / base, steps));
+        const int most = (steps + split - 1) / split;  // steps of a workgroup
+        split = (steps + most - 1) / most;             // (no more splits than that takes)
+        if ((float)(steps - most) * step < 2.0f + (float)split * join) split = 1;
+    }
     p.n_split = std::max(1, split);
     // (the splits' tickets, and 32-bit offsets into their workspace: only a
     // forced split can outgrow them)

@@ -220,6 +220,45 @@ __device__ __forceinline__ void write_out(const AttnArgs& a, const AttnSlot& S, 
     }
 }
 
+// The query rows r0 .. r0 + QR - 1 on their way to LDS: a thread takes 16 values
+// of a row, all rows of a pass in flight at once.
+template <int HD, int QR, int PL, int NT, int QP>
+struct Fp8Queries {
+    static constexpr int LPR = HD / 16, PER = NT / LPR, PASSES = (QR + PER - 1) / PER;  // lanes per row, rows per pass
+    f32x4 y[PASSES][4];
+
+    __device__ __forceinline__ void load(const AttnArgs& a, const AttnSlot& S, int g, int r0, int rows) {
+#pragma unroll
+        for (int p = 0; p < PASSES; ++p) {
+            // (a row past the last is the last again; lanes of a row agree)
+            const int i = p * PER + (int)threadIdx.x / LPR, r = min(r0 + min(i, QR - 1), rows - 1);
+            const int qi = udiv(r, a.group, a.mg_group);
+            load_query<HD>(a, S, qi, g * a.group + r - qi * a.group, (int)threadIdx.x % LPR * 16, y[p]);
+        }
+    }
+    // scaled by a power of two each (inverse to srow), split into PL planes of f16
+    // in sq [PL][QR][QP]
+    __device__ __forceinline__ void stage(const AttnArgs& a, _Float16* sq, float* srow) const {
+        const int tid = threadIdx.x, d0 = tid % LPR * 16;
+#pragma unroll
+        for (int p = 0; p < PASSES; ++p) {
+            const int i = p * PER + tid / LPR;
+            float up, down;
+            query_scale<LPR>(a, y[p], up, down);
+            if (i < QR) {
+                if (tid % LPR == 0) srow[i] = down;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    f16x8 hi, lo;
+                    split8(y[p], h, up, hi, lo);
+                    *reinterpret_cast<f16x8*>(sq + i * QP + d0 + 8 * h) = hi;
+                    if constexpr (PL == 2) *reinterpret_cast<f16x8*>(sq + (QR + i) * QP + d0 + 8 * h) = lo;
+                }
+            }
+        }
+    }
+};
+
 // One row block's running state and the work of one key tile on it.  QR query
 // rows (columns of the transposed products): 32, or 16.
 template <int HD, int QR, int PL>
@@ -433,8 +472,10 @@ __device__ __forceinline__ void row_tiles(const AttnArgs& a, int nk, int q_lo, i
 
 // A workgroup of an 8 bit attention launch: its place in the grid.  Each XCD
 // (the hardware deals workgroups round robin over the 8) takes a contiguous run
-// of (batch slot, KV head, key split, row group), row groups fastest, so those
-// that read the same keys share an L2.
+// of (batch slot, KV head, row group, key split), splits fastest: the splits of a
+// row group share its query rows in an L2, and the joins are spread over the XCDs
+// (with row groups fastest they ended on the XCD of the last split: 64 joins of 64
+// rows of 512 dims, 4 splits, took 20 us instead of 13).
 struct Fp8Place {
     int rg, split, g, b;
     bool ok;
@@ -442,15 +483,133 @@ struct Fp8Place {
         const int per = (a.n_wg + 7) / 8;
         int id = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
         ok = (int)(blockIdx.x >> 3) < per && id < a.n_wg;
-        const int t = udiv(id, a.rowgroups, a.mg_rowgroups);
-        rg = id - t * a.rowgroups;
-        const int u = a.n_split > 1 ? udiv(t, a.n_split, a.mg_split) : t;
-        split = t - u * a.n_split;
+        const int t = a.n_split > 1 ? udiv(id, a.n_split, a.mg_split) : id;
+        split = id - t * a.n_split;
+        const int u = udiv(t, a.rowgroups, a.mg_rowgroups);
+        rg = t - u * a.rowgroups;
         b = udiv(u, a.n_head_kv, a.mg_hkv);
         g = u - b * a.n_head_kv;
     }
 };
 inline unsigned fp8_grid(const AttnArgs& a) { return (unsigned)((a.n_wg + 7) / 8 * 8); }
+
+// Key splits.  Each workgroup has stored the states of its rows r0 .. r0 + nr - 1
+// with agent-scope accesses; it waits until they are complete, and one thread
+// takes the row group's ticket.  The one that draws n_split - 1 is the last: the
+// others' stores are complete and its agent-scope loads see them.  It joins the
+// splits in an order of its own (the same bits whichever comes last), writes the
+// rows and resets the ticket for the next call.  No workgroup waits for another.
+// so: LDS of NT * 6 floats that nobody reads any more; stick: one int in LDS.
+// (Byte offsets of the workspace fit 32 bits: the host checks.)
+template <int HD, int NT>
+__device__ __forceinline__ void fp8_join(const AttnArgs& a, const Fp8Place& at, int r0, int nr, float* so, int* stick) {
+    const AttnSlot& S = a.slot[at.b];
+    const int tid = threadIdx.x, items = nr * (HD / 4);
+    const size_t prow0 = ((size_t)at.b * a.n_head_kv + at.g) * a.part_rows + r0;
+    const size_t plane = (size_t)a.n_batch * a.n_head_kv * a.part_rows;
+    const __amdgpu_buffer_rsrc_t ro = make_rsrc(a.part_o, 0xffffffffu);
+    const __amdgpu_buffer_rsrc_t rm = make_rsrc(a.part_ml, 0xffffffffu);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    int* const tk = a.ticket + (at.b * a.n_head_kv + at.g) * a.rowgroups + at.rg;
+    if (tid == 0) *stick = __hip_atomic_fetch_add(tk, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    if (*stick != a.n_split - 1) return;
+    if (tid == 0) __hip_atomic_store(tk, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    // Few rows leave threads over: `share` threads take an item's splits (thread
+    // k of them takes splits k, k + share, ...), so that all loads of a wide
+    // split are in flight together; their states join through LDS.
+    // Many rows: a thread takes several items at once, 16 loads in flight.
+    auto many = [&](auto ni, auto ns) __attribute__((always_inline)) {
+        constexpr int NI = decltype(ni)::value, NS = decltype(ns)::value;
+        for (int p = tid; p < items; p += NI * NT) {
+            float Mx[NI], L[NI];
+            f32x4 acc[NI][1];
+#pragma unroll
+            for (int q = 0; q < NI; ++q) {
+                Mx[q] = -INFINITY;
+                L[q] = 0.0f;
+                acc[q][0] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            }
+            for (int s0 = 0; s0 < a.n_split; s0 += NS) {
+                float m[NI][NS], l[NI][NS];
+                f32x4 o[NI][NS][1];
+#pragma unroll
+                for (int q = 0; q < NI; ++q) {
+                    const int it = min(p + q * NT, items - 1);
+#pragma unroll
+                    for (int j = 0; j < NS; ++j) {
+                        const size_t row = (size_t)min(s0 + j, a.n_split - 1) * plane + prow0 + it / (HD / 4);
+                        const float2 ml = load2_sc1(rm, (int)(row * 8));
+                        o[q][j][0] = load_sc1(ro, (int)((row * HD + it % (HD / 4) * 4) * 4));
+                        m[q][j] = s0 + j < a.n_split ? ml.x : -INFINITY;
+                        l[q][j] = ml.y;
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);  // (every load above before any wait)
+#pragma unroll
+                for (int q = 0; q < NI; ++q) merge_split_states<NS, 1>(Mx[q], L[q], acc[q], m[q], l[q], o[q]);
+            }
+#pragma unroll
+            for (int q = 0; q < NI; ++q) {
+                const int it = p + q * NT;
+                if (it < items)
+                    write_out<HD>(a, S, at.g, r0 + it / (HD / 4), it % (HD / 4) * 4, acc[q][0] * (1.0f / L[q]));
+            }
+        }
+    };
+    if (items >= 2 * NT) {
+        if (a.n_split <= 4)
+            many(std::integral_constant<int, 4>{}, std::integral_constant<int, 4>{});
+        else
+            many(std::integral_constant<int, 2>{}, std::integral_constant<int, 8>{});
+        return;
+    }
+    int share = 1;
+    while (2 * share * items <= NT) share *= 2;
+    for (int p = tid; p < share * items; p += NT) {
+        const int k = p / items, it = p - k * items, i = it / (HD / 4), d = it % (HD / 4) * 4;
+        float Mx = -INFINITY, L = 0.0f;
+        f32x4 acc[1] = {{0.0f, 0.0f, 0.0f, 0.0f}};
+        for (int s0 = k; s0 < a.n_split; s0 += 8 * share) {
+            float m[8], l[8];
+            f32x4 o8[8][1];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int sp = s0 + j * share;
+                const size_t row = (size_t)min(sp, a.n_split - 1) * plane + prow0 + i;
+                const float2 ml = load2_sc1(rm, (int)(row * 8));
+                o8[j][0] = load_sc1(ro, (int)((row * HD + d) * 4));
+                m[j] = sp < a.n_split ? ml.x : -INFINITY;
+                l[j] = ml.y;
+            }
+            __builtin_amdgcn_sched_barrier(0);  // (every load above before any wait)
+            merge_split_states<8, 1>(Mx, L, acc, m, l, o8);
+        }
+        if (share == 1) {
+            write_out<HD>(a, S, at.g, r0 + i, d, acc[0] * (1.0f / L));
+        } else {
+            float* t = so + p * 6;
+            t[0] = Mx;
+            t[1] = L;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) t[2 + e] = acc[0][e];
+        }
+    }
+    if (share == 1) return;
+    __syncthreads();
+    if (tid < items) {
+        float Mx = -INFINITY, L = 0.0f;
+        f32x4 acc[1] = {{0.0f, 0.0f, 0.0f, 0.0f}};
+        for (int k = 0; k < share; ++k) {
+            const float* t = so + (k * items + tid) * 6;
+            const float m[1] = {t[0]}, l[1] = {t[1]};
+            const f32x4 w[1][1] = {{{t[2], t[3], t[4], t[5]}}};
+            merge_split_states<1, 1>(Mx, L, acc, m, l, w);
+        }
+        write_out<HD>(a, S, at.g, r0 + tid / (HD / 4), tid % (HD / 4) * 4, acc[0] * (1.0f / L));
+    }
+}
 
 // The end of a workgroup of NW waves on one block of QR rows: their states meet
 // in LDS, the rows leave, or, with key splits, join the other splits'.  LDS: so [NW][QR][HD + 4] floats, sm and sl [NW][QR], sr
@@ -505,13 +664,7 @@ __device__ __forceinline__ void fp8_finish(const AttnArgs& a, const Fp8Place& at
         return;
     }
 
-    // ---- key splits.  Each workgroup stores its states with agent-scope
-    // accesses and waits until they are complete; one thread then takes the row
-    // group's ticket.  The one that draws n_split - 1 is the last: the others'
-    // stores are complete and its agent-scope loads see them.  It joins the
-    // splits in an order of its own (the same bits whichever comes last) and
-    // resets the ticket for the next call.  No workgroup waits for another.
-    // (Byte offsets of the workspace fit 32 bits: the host checks.)
+    // ---- key splits: this workgroup's states
     const size_t prow0 = ((size_t)at.b * a.n_head_kv + at.g) * a.part_rows + r0;
     const size_t plane = (size_t)a.n_batch * a.n_head_kv * a.part_rows;
     const __amdgpu_buffer_rsrc_t ro = make_rsrc(a.part_o, 0xffffffffu);
@@ -525,60 +678,7 @@ __device__ __forceinline__ void fp8_finish(const AttnArgs& a, const Fp8Place& at
         const float Mi = sr[i], L = sr[QR + i];
         if (d == 0) store2_sc1(rm, (int)(row * 8), L != L && Mi == -INFINITY ? 0.0f : Mi, L);
     }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    int* const tk = a.ticket + (at.b * a.n_head_kv + at.g) * a.rowgroups + at.rg;
-    if (tid == 0) *stick = __hip_atomic_fetch_add(tk, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    __syncthreads();
-    if (*stick != a.n_split - 1) return;
-    if (tid == 0) __hip_atomic_store(tk, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    // Few rows leave threads over: `share` threads take an item's splits (thread
-    // k of them takes splits k, k + share, ...), so that all loads of a wide
-    // split are in flight together; their states join through LDS.
-    int share = 1;
-    while (2 * share * items <= NT) share *= 2;
-    for (int p = tid; p < share * items; p += NT) {
-        const int k = p / items, it = p - k * items, i = it / (HD / 4), d = it % (HD / 4) * 4;
-        float Mx = -INFINITY, L = 0.0f;
-        f32x4 acc[1] = {{0.0f, 0.0f, 0.0f, 0.0f}};
-        for (int s0 = k; s0 < a.n_split; s0 += 8 * share) {
-            float m[8], l[8];
-            f32x4 o8[8][1];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int sp = s0 + j * share;
-                const size_t row = (size_t)min(sp, a.n_split - 1) * plane + prow0 + i;
-                const float2 ml = load2_sc1(rm, (int)(row * 8));
-                o8[j][0] = load_sc1(ro, (int)((row * HD + d) * 4));
-                m[j] = sp < a.n_split ? ml.x : -INFINITY;
-                l[j] = ml.y;
-            }
-            __builtin_amdgcn_sched_barrier(0);  // (every load above before any wait)
-            merge_split_states<8, 1>(Mx, L, acc, m, l, o8);
-        }
-        if (share == 1) {
-            write_out<HD>(a, S, at.g, r0 + i, d, acc[0] * (1.0f / L));
-        } else {
-            float* t = so + p * 6;
-            t[0] = Mx;
-            t[1] = L;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) t[2 + e] = acc[0][e];
-        }
-    }
-    if (share == 1) return;
-    __syncthreads();
-    if (tid < items) {
-        float Mx = -INFINITY, L = 0.0f;
-        f32x4 acc[1] = {{0.0f, 0.0f, 0.0f, 0.0f}};
-        for (int k = 0; k < share; ++k) {
-            const float* t = so + (k * items + tid) * 6;
-            const float m[1] = {t[0]}, l[1] = {t[1]};
-            const f32x4 w[1][1] = {{{t[2], t[3], t[4], t[5]}}};
-            merge_split_states<1, 1>(Mx, L, acc, m, l, w);
-        }
-        write_out<HD>(a, S, at.g, r0 + tid / (HD / 4), tid % (HD / 4) * 4, acc[0] * (1.0f / L));
-    }
+    fp8_join<HD, NT>(a, at, r0, nr, so, stick);
 }
 
 }  // namespace
