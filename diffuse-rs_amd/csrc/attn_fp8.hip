@@ -216,7 +216,7 @@ hipError_t launch_hd(const LaunchPlan& p, const AttnArgs& a, hipStream_t st) {
 // A split for every tile and CU, as cheap single rows take it, costs more rows up to
 // twice the time (5 rows x 4 heads of 512 dims, 4352 keys: 34 splits 44 us, 9 33).
 LaunchPlan plan_fp8(int hd_tile, int n_batch, int n_head_kv, int group, int max_nq, int max_nk, int mask, int n_cu,
-                    int force_split, int max_tickets) {
+                    int force_split, int force_rows, int max_tickets) {
     LaunchPlan p{};
     p.hd_tile = hd_tile;
     p.block_n = 32;
@@ -225,8 +225,9 @@ LaunchPlan plan_fp8(int hd_tile, int n_batch, int n_head_kv, int group, int max_
     p.kernel = KERNEL_FP8;
     const int tiles = std::max(1, (max_nk + 31) / 32), packed = group * max_nq;
     const int64_t base16 = (int64_t)n_batch * n_head_kv * ((packed + 15) / 16);
-    const bool wide = hd_tile > 256 && packed > 32 && (base16 > n_cu || (4 * base16 >= n_cu && base16 * tiles >= (int64_t)120 * n_cu));
-    p.w16 = !wide && (hd_tile > 128 || packed <= 16);
+    const bool many = packed > 32 && (base16 > n_cu || (4 * base16 >= n_cu && base16 * tiles >= (int64_t)120 * n_cu));
+    const bool wide = hd_tile > 256 && (force_rows ? force_rows == 32 : many);
+    p.w16 = !wide && (hd_tile > 128 || (force_rows ? force_rows == 16 : packed <= 16));
     p.rb = wide ? 2 : 1;
     const int qr = p.w16 ? 16 : 32 * p.rb;
     p.rowgroups = (packed + qr - 1) / qr;

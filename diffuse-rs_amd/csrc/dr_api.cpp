@@ -1351,8 +1351,10 @@ static dr::LaunchPlan plan_for(dr_ctx* ctx, const dr::AttnArgs& a, int hd, int m
     // kernel family is forced (then the lo half is not read)
     if (a.fp8)
         return dr::plan_fp8(hd_tile_for((size_t)hd), a.n_batch, a.n_head_kv, a.group, max_nq, a.key_band, mask,
-                            ctx->n_cu, ctx->force_split, (int)TICKETS);
-    const bool hilo_asked = ctx->force_kernel == dr::KERNEL_AUTO || ctx->force_kernel == dr::KERNEL_HILO;
+                            ctx->n_cu, ctx->force_split, ctx->force_rows, (int)TICKETS);
+    // (the 8 bit family forced is no choice for a layer that is not 8 bit: automatic)
+    const bool hilo_asked = ctx->force_kernel == dr::KERNEL_AUTO || ctx->force_kernel == dr::KERNEL_HILO ||
+                            ctx->force_kernel == dr::KERNEL_FP8;
     const bool bf16_rows = a.q_bf16 || a.o_bf16;
     if (a.slot[0].klo && hilo_asked && !bf16_rows) return plan_hilo(ctx, a, hd, max_nq, max_nk, mask);
     // bf16 Q or output rows: only the per-wave-stream kernel reads / writes them

@@ -395,7 +395,7 @@ int hilo32_rows(int hd_tile);  // the same of attn_hilo32_kernel (0: head dim no
 // DR_PRECISION_FP8 layers: the attention's plan and kernels (attn_fp8.hip), the
 // store and the gather (kv_fp8.hip).
 LaunchPlan plan_fp8(int hd_tile, int n_batch, int n_head_kv, int group, int max_nq, int max_nk, int mask, int n_cu,
-                    int force_split, int max_tickets);
+                    int force_split, int force_rows, int max_tickets);
 hipError_t launch_fp8(const LaunchPlan& p, const AttnArgs& a, hipStream_t st);
 hipError_t launch_fp8_wide(const AttnArgs& a, hipStream_t st);  // head-dim tile 512, many rows
 hipError_t launch_store_fp8(int hd_tile, const StoreArgs& a, hipStream_t st);

@@ -497,7 +497,9 @@ int dr_ctx_last_launch(const dr_ctx* ctx, dr_launch_info* info);
 int dr_ctx_set_split(dr_ctx* ctx, int n_split);
 /* Query rows per compute wave for later calls on ctx: 16 or 32 where the
  * head-dim tile builds both, 0 = automatic.  With DR_KERNEL_STREAMS at head
- * dim 256, 16 selects the 16-row-wave stream kernel (no key split). */
+ * dim 256, 16 selects the 16-row-wave stream kernel (no key split).  8 bit layers
+ * have both at head dims up to 128 and above 256 (32 there: workgroups of 64 rows
+ * whose waves split the head dim). */
 int dr_ctx_set_wave_rows(dr_ctx* ctx, int rows);
 /* Attention kernel families, for dr_ctx_set_kernel and dr_launch_info.kernel.
  * STAGED: the workgroup's waves share K/V super-tiles staged in LDS (every
@@ -517,9 +519,9 @@ int dr_ctx_set_wave_rows(dr_ctx* ctx, int rows);
  * planner: HILO on hi/lo layers, FP8 on 8 bit layers, else STREAMS wherever it
  * applies), or force STAGED / STREAMS (STREAMS falls back to STAGED where it
  * does not apply; on a hi/lo layer both ignore the lo half).  An 8 bit layer is
- * read by its own family only: with another one forced its calls fail with
- * DR_ERR_UNSUPPORTED; HILO and FP8 mean AUTO on layers that are not theirs.  A
- * tuning knob, for measurement and tests. */
+ * read by its own family only: with STAGED, STREAMS or HILO forced its calls fail
+ * with DR_ERR_UNSUPPORTED.  FP8 means AUTO on every other layer, HILO on bf16
+ * layers.  A tuning knob, for measurement and tests. */
 int dr_ctx_set_kernel(dr_ctx* ctx, int kernel);
 /* The element type of the Q rows that later dr_attention_cached /
  * _cached_noalloc / _step / _step_epi calls on ctx read (no counterpart in
