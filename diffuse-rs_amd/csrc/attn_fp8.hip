@@ -47,9 +47,10 @@ void attn_fp8_kernel(const AttnArgs a) {
     _Float16* const svs = reinterpret_cast<_Float16*>(sr + 2 * QR);  // [NW][32]
     int* const stick = reinterpret_cast<int*>(svs + NW * 32);
 
+    AttnSlot S = request_args(a);
     const Fp8Place at(a);
     if (!at.ok) return;
-    const AttnSlot& S = a.slot[at.b];
+    if (a.n_batch > 1) S = a.slot[at.b];
     const int rows = S.nq * a.group, r0 = at.rg * QR;
     if (r0 >= rows) return;  // (a shorter pass of the batch)
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
@@ -160,7 +161,7 @@ void attn_fp8_kernel(const AttnArgs a) {
         fetch_v(t + NW, x);
     }
     if constexpr (G::BIG) __syncthreads();  // (the merge area lies over the query rows)
-    fp8_finish<HD, QR, PL, NW>(a, at, st, r0, reinterpret_cast<float*>(lds), sm, sl, sr, stick);
+    fp8_finish<HD, QR, PL, NW>(a, S, at, st, r0, reinterpret_cast<float*>(lds), sm, sl, sr, stick);
 }
 
 template <int HD, int QR, int PL, int NW>

@@ -50,9 +50,10 @@ void attn_fp8_wide_kernel(const AttnArgs a) {
     int* const sflag = reinterpret_cast<int*>(ssum + NW * 32);    // [2]
     int* const stick = sflag + 4;
 
+    AttnSlot S = request_args(a);
     const Fp8Place at(a);
     if (!at.ok) return;
-    const AttnSlot& S = a.slot[at.b];
+    if (a.n_batch > 1) S = a.slot[at.b];
     const int rows = S.nq * a.group, r0 = at.rg * G::ROWS;
     if (r0 >= rows) return;  // (a shorter pass of the batch)
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
@@ -342,7 +343,7 @@ void attn_fp8_wide_kernel(const AttnArgs a) {
         else
             store_sc1(ro, (int)((((size_t)at.split * plane + prow0 + i) * HD + d) * 4), y);
     }
-    if (a.n_split > 1) fp8_join<HD, 512>(a, at, r0, nr, so, stick);
+    if (a.n_split > 1) fp8_join<HD, 512>(a, S, at, r0, nr, so, stick);
 }
 
 template <int PL>

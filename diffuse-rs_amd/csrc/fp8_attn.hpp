@@ -83,6 +83,21 @@ __device__ __forceinline__ f32x2 residual(const f32x2& p, const f16x2& hi) {
 
 __device__ __forceinline__ float pow2_biased(int e) { return __uint_as_float((uint32_t)max(e, 0) << 23); }
 
+// What every workgroup takes from the arguments, batch slot 0 included, is
+// requested at its start in a few wide scalar loads with one wait; left to first
+// uses, eight loads wait for each other (1 us of a call's 10).  The empty asm also
+// keeps the compiler from choosing the slot by its address, which is one more.
+__device__ __forceinline__ AttnSlot request_args(const AttnArgs& a) {
+    AttnSlot S = a.slot[0];
+    asm volatile("" : "+s"(S.q), "+s"(S.out), "+s"(S.qpos), "+s"(S.k), "+s"(S.vt), "+s"(S.klo), "+s"(S.nq), "+s"(S.nk),
+                 "+s"(S.qpos0)
+                 : "s"(a.n_batch), "s"(a.n_head_kv), "s"(a.group), "s"(a.hd), "s"(a.cap), "s"(a.q_rstride),
+                   "s"(a.rowgroups), "s"(a.n_split), "s"(a.mg_split), "s"(a.mg_rowgroups), "s"(a.mg_hkv), "s"(a.c),
+                   "s"(a.n_wg), "s"(a.window), "s"(a.prefix), "s"(a.o_rstride), "s"(a.qn_w), "s"(a.qb), "s"(a.rope),
+                   "s"(a.q_bf16), "s"(a.o_bf16), "s"(a.mg_group));
+    return S;
+}
+
 __device__ __forceinline__ int row_pos(const AttnSlot& S, int qi) { return S.qpos0 >= 0 ? S.qpos0 + qi : S.qpos[qi]; }
 
 // Values d..d + 3 of a query row (0 past head_dim), f32.
@@ -502,8 +517,8 @@ inline unsigned fp8_grid(const AttnArgs& a) { return (unsigned)((a.n_wg + 7) / 8
 // so: LDS of NT * 6 floats that nobody reads any more; stick: one int in LDS.
 // (Byte offsets of the workspace fit 32 bits: the host checks.)
 template <int HD, int NT>
-__device__ __forceinline__ void fp8_join(const AttnArgs& a, const Fp8Place& at, int r0, int nr, float* so, int* stick) {
-    const AttnSlot& S = a.slot[at.b];
+__device__ __forceinline__ void fp8_join(const AttnArgs& a, const AttnSlot& S, const Fp8Place& at, int r0, int nr,
+                                         float* so, int* stick) {
     const int tid = threadIdx.x, items = nr * (HD / 4);
     const size_t prow0 = ((size_t)at.b * a.n_head_kv + at.g) * a.part_rows + r0;
     const size_t plane = (size_t)a.n_batch * a.n_head_kv * a.part_rows;
@@ -615,11 +630,11 @@ __device__ __forceinline__ void fp8_join(const AttnArgs& a, const Fp8Place& at, 
 // in LDS, the rows leave, or, with key splits, join the other splits'.  LDS: so [NW][QR][HD + 4] floats, sm and sl [NW][QR], sr
 // [2][QR], stick one int; so may lie over what the waves read before (a barrier precedes).
 template <int HD, int QR, int PL, int NW>
-__device__ __forceinline__ void fp8_finish(const AttnArgs& a, const Fp8Place& at, const Fp8State<HD, QR, PL>& st, int r0,
-                                           float* so, float* sm, float* sl, float* sr, int* stick) {
+__device__ __forceinline__ void fp8_finish(const AttnArgs& a, const AttnSlot& S, const Fp8Place& at,
+                                           const Fp8State<HD, QR, PL>& st, int r0, float* so, float* sm,
+                                           float* sl, float* sr, int* stick) {
     using T = Fp8State<HD, QR, PL>;
     constexpr int OP = HD + 4, NT = NW * 64;
-    const AttnSlot& S = a.slot[at.b];
     const int tid = threadIdx.x, wave = tid >> 6, col = (tid & 63) % QR, half = (tid & 63) / QR;
     const float lt = st.row_sum();
     if (half == 0) {
@@ -678,7 +693,7 @@ __device__ __forceinline__ void fp8_finish(const AttnArgs& a, const Fp8Place& at
         const float Mi = sr[i], L = sr[QR + i];
         if (d == 0) store2_sc1(rm, (int)(row * 8), L != L && Mi == -INFINITY ? 0.0f : Mi, L);
     }
-    fp8_join<HD, NT>(a, at, r0, nr, so, stick);
+    fp8_join<HD, NT>(a, S, at, r0, nr, so, stick);
 }
 
 }  // namespace
