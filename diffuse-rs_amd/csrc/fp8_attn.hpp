@@ -331,9 +331,11 @@ struct Fp8State {
             kc = ldexpf(cq, kref - 127 - 7);
             kc = kc < FLT_MIN ? FLT_MIN : kc;
             if (vt > vref) {
-                const float f = pow2_biased(vref - vt + 127);
+                if (vref > 0) {  // (else o is 0)
+                    const float f = pow2_biased(vref - vt + 127);
 #pragma unroll
-                for (int db = 0; db < DB; ++db) o[db] *= f;
+                    for (int db = 0; db < DB; ++db) o[db] *= f;
+                }
                 vref = vt;
             }
         }
@@ -384,10 +386,11 @@ struct Fp8State {
             for (int off = QR; off < 64; off <<= 1) nm = __builtin_fmaxf(nm, __shfl_xor(nm, off));
             nm = nm > m + MOVE ? nm : m;
             const float f = m == nm ? 1.0f : __builtin_amdgcn_exp2f(m - nm);
-            m = nm;
             l *= f;
+            if (__any(m != -INFINITY))  // (else o is 0)
 #pragma unroll
-            for (int db = 0; db < DB; ++db) o[db] *= f;
+                for (int db = 0; db < DB; ++db) o[db] *= f;
+            m = nm;
         }
         const float off = P0 - (m == -INFINITY ? 0.0f : m);
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -501,7 +504,7 @@ struct Fp8Place {
         const int t = a.n_split > 1 ? udiv(id, a.n_split, a.mg_split) : id;
         split = id - t * a.n_split;
         const int u = udiv(t, a.rowgroups, a.mg_rowgroups);
-        rg = t - u * a.rowgroups;
+        rg = a.rowgroups - 1 - (t - u * a.rowgroups);  // (under a causal prefix the last see the most keys)
         b = udiv(u, a.n_head_kv, a.mg_hkv);
         g = u - b * a.n_head_kv;
     }
