@@ -140,9 +140,10 @@ void attn_fp8_kernel(const AttnArgs a) {
 
     T st;
     st.init(fabsf(a.c) * srow[col]);
-    for (int t = t_first; t < t1; t += NW) {
-        st.tile(
-            x.kb0, x.kb1, x.vb, svs + wave * 32, !tile_visible(a, S.nk, t, q_lo, q_hi),
+    for (int t = t_first, cap = FP8_NAN; t < t1;) {
+        int then = t;
+        const int next = st.tile(
+            cap, x.kb0, x.kb1, x.vb, svs + wave * 32, !tile_visible(a, S.nk, t, q_lo, q_hi),
             [&](int kb, int s) {
                 const u32x4& w = x.k[kb * (G::KCH / 2) + s / 2];
                 return u32x2{w[s % 2 * 2], w[s % 2 * 2 + 1]};
@@ -157,8 +158,13 @@ void attn_fp8_kernel(const AttnArgs a) {
                 return (key < S.nk) & visible(my_pos, key, 0, 0, a.window, a.prefix);
             },
             [&](int i) { return (int)gload<uint8_t>(sbase + (size_t)t * 64 + T::NP * half + i); },
-            [&]() { fetch_k(t + NW, x); });
-        fetch_v(t + NW, x);
+            [&](int again) {
+                then = again ? t : t + NW;
+                fetch_k(then, x);
+            });
+        fetch_v(then, x);
+        t = then;
+        cap = next ? next : FP8_NAN;
     }
     if constexpr (G::BIG) __syncthreads();  // (the merge area lies over the query rows)
     fp8_finish<HD, QR, PL, NW>(a, S, at, st, r0, reinterpret_cast<float*>(lds), sm, sl, sr, stick);

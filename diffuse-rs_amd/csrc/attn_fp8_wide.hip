@@ -120,15 +120,15 @@ void attn_fp8_wide_kernel(const AttnArgs a) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[db][i] = 0.0f;
     float m = -INFINITY, l = 0.0f;  // row col's maximum; this lane's part of its sum
-    int kref = 0, vref = 0;
-    float kc = 0.0f;
+    int kref = 0, vref = 0;  // (vref: a row's own once `apart`)
+    bool apart = false;
+    float kc = FLT_MIN;
     // the tile whose weights wait in LDS: its scores and what turns them into weights
     float s[4], s_kc = 0.0f, l_before = 0.0f;
     f16x2 s_vs[2];
 
-    // weights of the kept scores into buffer b
-    auto weigh = [&](int b) __attribute__((always_inline)) {
-        const float off = P0 - (m == -INFINITY ? 0.0f : m);
+    // weights exp2(kept scores + off) into buffer b
+    auto weigh = [&](int b, float off) __attribute__((always_inline)) {
         l = l_before;
         char* const to = pbuf + b * G::PBUF + rb * PL * 2048 + (quad >> 1) * 1024 + lane * 16 + (quad & 1) * 8;
         f16x2 hi[2], lo[2];
@@ -178,7 +178,7 @@ void attn_fp8_wide_kernel(const AttnArgs a) {
             l_before *= f;
 #pragma unroll
             for (int db = 0; db < DB; ++db) o[db] *= f;
-            weigh(k & 1);
+            weigh(k & 1, P0 - (m == -INFINITY ? 0.0f : m));
             lds_barrier();
             weights(k, w);
         }
@@ -198,41 +198,46 @@ void attn_fp8_wide_kernel(const AttnArgs a) {
 
     Scales x;
     u32x4 kq[DB], vq[DB];
-    const int n = t1 - t0;
-    // tile k of this workgroup: its scores, the values of the tile before, its weights
+    // Walk k of this workgroup: tile t's scores, the values of the walk before, its
+    // weights.  (cap and t as of Fp8State::tile and its loop.)
+    int t = t0, cap = FP8_NAN;
     auto step = [&](int k) __attribute__((always_inline)) {
-        const int t = t0 + k;
-        // ---- K's scales relative to the largest so far, the partial scores
+        // ---- K's and V's scales, the partial scores
         bool nan = false;
         float vdown = 1.0f;
-        if (__any(x.kb > kref || x.vb > vref)) {
-            // (the same decision in every wave: each sees all 64 bytes)
-            const int k0 = x.kb == FP8_NAN ? 0 : x.kb;
-            int kt = k0, vt = x.vb == FP8_NAN ? 0 : x.vb;
+        int next = 0;
+        Band band{};
+        bool banded = cap != FP8_NAN;
+        if (__any((unsigned)(x.kb - kref + TK) > (unsigned)TK || (unsigned)(x.vb - vref + TV<PL>) > (unsigned)TV<PL> ||
+                  apart || banded)) {
+            // (the same decisions in every wave: each sees all 64 bytes)
+            const int k0 = x.kb > min(cap, FP8_NAN - 1) ? 0 : x.kb;
+            const int kt = wave_max(k0), vt = wave_max(x.vb == FP8_NAN ? 0 : x.vb);
             nan = __any(x.kb == FP8_NAN || x.vb == FP8_NAN);
-#pragma unroll
-            for (int off = 32; off > 0; off >>= 1) {
-                kt = max(kt, __shfl_xor(kt, off));
-                vt = max(vt, __shfl_xor(vt, off));
+            if (kt > 1) {
+                kref = kt;
+                kc = __builtin_fmaxf(ldexpf(cq, kref - 127 - 7), FLT_MIN);
             }
-            kref = max(kref, kt);
-            // (never 0: a hidden score of -infinity has to stay one)
-            kc = ldexpf(cq, kref - 127 - 7);
-            kc = kc < FLT_MIN ? FLT_MIN : kc;
-            if (vt > vref) {
-                vdown = pow2_biased(vref - vt + 127);
+            next = wave_max(scale_far(k0, kref, TK) ? k0 : 0);
+            banded = banded || next > 0;
+            band = {kref, cap == FP8_NAN, next == 0};
+            if (!apart && vt > vref && !(vref > 1 && vt > vref + TV_RISE)) {
+                if (vref > 1) vdown = pow2_biased(vref - vt + 127);
                 vref = vt;
             }
+            apart = apart || __any(scale_far(x.vb, vref, TV<PL>));
         }
+        const bool far = __builtin_amdgcn_readfirstlane(apart);
         const bool slow = __builtin_amdgcn_readfirstlane(!tile_visible(a, nk, t, q_lo, q_hi));
-        const float ks = pow2_biased(min(x.kb - kref, 0) + 127 + 7);
+        const uint32_t vbytes = x.vq;
         f16x2 vs[2];  // V's scales of the four keys
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const int vb = (int)(x.vq >> (8 * j)) & 255;
+            const int vb = (int)(vbytes >> (8 * j)) & 255;
             vs[j / 2][j % 2] = (_Float16)(vb == FP8_NAN ? INFINITY : pow2_biased(vb - vref + 127));
         }
         f32x16 acc = {};
+        const float ks = band_scale(x.kb, kref);
 #pragma unroll
         for (int st = 0; st < NS; ++st) {
             const u32x4& w = kq[st / 2];
@@ -240,7 +245,9 @@ void attn_fp8_wide_kernel(const AttnArgs a) {
 #pragma unroll
             for (int p = 0; p < PL; ++p) acc = mfma(k8, q[p][st], acc);
         }
-        fetch_k(t + 1, x, kq);
+        next = __builtin_amdgcn_readfirstlane(next);
+        const int then = next ? t : t + 1;
+        fetch_k(then, x, kq);
         char* const mine = part + (k & 1) * G::PART + wave * 4096 + lane * 16;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -257,7 +264,7 @@ void attn_fp8_wide_kernel(const AttnArgs a) {
         weights(k + 1, w);  // (tile k - 1's buffer)
         __builtin_amdgcn_sched_barrier(0);
         // this wave's scores, and their weights
-        auto scored = [&]() __attribute__((always_inline)) {
+        auto masked = [&]() __attribute__((always_inline)) {
             f32x4 sum = pr[0];
 #pragma unroll
             for (int w = 1; w < 4; ++w) sum += pr[w];
@@ -266,10 +273,19 @@ void attn_fp8_wide_kernel(const AttnArgs a) {
             s_vs[0] = vs[0];
             s_vs[1] = vs[1];
             s_kc = kc;
+            if (__builtin_expect(banded, 0)) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (!band.holds(gload<uint8_t>(sbase + (size_t)t * 64 + 16 * half + 4 * quad + j))) {
+                        s[j] = -INFINITY;
+                        s_vs[j / 2][j % 2] = (_Float16)0.0f;
+                    }
+            }
             if (nan)
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    if (gload<uint8_t>(sbase + (size_t)t * 64 + 16 * half + 4 * quad + j) == FP8_NAN) s[j] = NAN;
+                    if (gload<uint8_t>(sbase + (size_t)t * 64 + 16 * half + 4 * quad + j) == FP8_NAN && s[j] != -INFINITY)
+                        s[j] = NAN;
             if (slow)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
@@ -279,28 +295,87 @@ void attn_fp8_wide_kernel(const AttnArgs a) {
                         s_vs[j / 2][j % 2] = (_Float16)0.0f;  // (0 times a scale of infinity)
                     }
                 }
+        };
+        auto scored = [&]() __attribute__((always_inline)) {
+            masked();
             float top = __builtin_fmaxf(__builtin_fmaxf(s[0], s[1]), __builtin_fmaxf(s[2], s[3]));
             top = top == -INFINITY ? -INFINITY : top * kc;
             if (__any(top > m + MOVE) && lane == 0) sflag[k & 1] = k + 1;
             l_before = l;
-            weigh(k & 1);
+            weigh(k & 1, P0 - (m == -INFINITY ? 0.0f : m));
         };
         if (k > 0) settle(k - 1, flag, w);
         // Half of the waves, one of each SIMD's two, take the values of the tile
         // before first, the others their scores: the matrix cores and the vector
         // units both have work at any time.
-        if (wave >= 4) scored();
+        if (wave >= 4 && !far) scored();
         if (k > 0) values(w, vq);
         fetch_v(t, vq);
         if (__builtin_amdgcn_readfirstlane(__float_as_int(vdown)) != __float_as_int(1.0f))
 #pragma unroll
             for (int db = 0; db < DB; ++db) o[db] *= vdown;
-        if (wave < 4) scored();
+        if (__builtin_expect(far, 0)) {
+            // the row's accumulators at a size of their own, then its maximum, then
+            // V's scales into the weights' exponents: each as all four waves see it
+            auto row_most = [&](float* in, float x) __attribute__((always_inline)) {
+                x = __builtin_fmaxf(x, __shfl_xor(x, 32));
+                if (half == 0) in[wave * 32 + col] = x;
+                lds_barrier();
+#pragma unroll
+                for (int w4 = 0; w4 < 4; ++w4) x = __builtin_fmaxf(x, in[(rb * 4 + w4) * 32 + col]);
+                return x;
+            };
+            float big = 0.0f;
+#pragma unroll
+            for (int db = 0; db < DB; ++db)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) big = __builtin_fmaxf(big, fabsf(o[db][i]));
+            big = row_most(ssum, big);
+            const int up = centre(big);
+            vref = big == 0.0f ? 0 : vref - up;
+            masked();
+            float top = __builtin_fmaxf(__builtin_fmaxf(s[0], s[1]), __builtin_fmaxf(s[2], s[3]));
+            float nm = row_most(smax, top == -INFINITY ? -INFINITY : top * kc);
+            nm = nm > m + MOVE ? nm : m;
+            const float f = m == nm ? 1.0f : __builtin_amdgcn_exp2f(m - nm), off = P0 - (nm == -INFINITY ? 0.0f : nm);
+            m = nm;
+            l *= f;
+            float most = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int vb = (int)(vbytes >> (8 * j)) & 255;
+                s[j] = __builtin_fmaf(s[j], kc, off);
+                l += __builtin_amdgcn_exp2f(s[j]);
+                if (vb != FP8_NAN) most = __builtin_fmaxf(most, s[j] + (float)(vb - vref));
+            }
+            most = row_most(ssum, most);
+            const int rise = most > P0 + MOVE ? (int)__builtin_fminf(ceilf(most - P0), 252.0f) : 0;
+            vref += rise;
+            const int e = up - rise;
+            const float f0 = pow2_biased(e / 2 + 127), f1 = pow2_biased(e - e / 2 + 127);
+#pragma unroll
+            for (int db = 0; db < DB; ++db) o[db] = o[db] * f * f0 * f1;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int vb = (int)(vbytes >> (8 * j)) & 255;
+                s[j] = vb == FP8_NAN && s[j] != -INFINITY ? NAN : s[j] + (float)(vb - vref);
+            }
+            s_kc = 1.0f;
+            s_vs[0] = s_vs[1] = f16x2{(_Float16)1.0f, (_Float16)1.0f};
+            const float sum = l;
+            weigh(k & 1, 0.0f);
+            l = l_before = sum;
+        } else if (wave < 4) {
+            scored();
+        }
+        t = then;
+        cap = next ? next : FP8_NAN;
     };
 
-    if (n > 0) {
+    if (t0 < t1) {
         fetch_k(t0, x, kq);
-        for (int k = 0; k < n; ++k) step(k);
+        int n = 0;
+        while (t < t1) step(n++);
         lds_barrier();
         f16x8 w[2][PL];
         weights(n - 1, w);
@@ -319,7 +394,8 @@ void attn_fp8_wide_kernel(const AttnArgs a) {
     const size_t plane = (size_t)a.n_batch * a.n_head_kv * a.part_rows;
     const __amdgpu_buffer_rsrc_t ro = make_rsrc(a.part_o, 0xffffffffu);
     const __amdgpu_buffer_rsrc_t rm = make_rsrc(a.part_ml, 0xffffffffu);
-    const float up = fp8_scale(vref);
+    const int e2 = vref - 127;
+    const float up0 = pow2_biased(e2 / 2 + 127), up1 = pow2_biased(e2 - e2 / 2 + 127);
     const int i = rb * 32 + col;
     float L = 0.0f;
 #pragma unroll
@@ -330,7 +406,7 @@ void attn_fp8_wide_kernel(const AttnArgs a) {
 #pragma unroll
         for (int e = 0; e < 16; e += 4)
             *reinterpret_cast<f32x4*>(so + i * OP + quad * G::DW + 32 * db + 2 * e + 4 * half) =
-                f32x4{o[db][e], o[db][e + 1], o[db][e + 2], o[db][e + 3]} * f * up;
+                f32x4{o[db][e], o[db][e + 1], o[db][e + 2], o[db][e + 3]} * f * up0 * up1;
     // (a NaN without any finite score must not pass for a row without keys)
     if (a.n_split > 1 && quad == 0 && half == 0 && i < nr)
         store2_sc1(rm, (int)(((size_t)at.split * plane + prow0 + i) * 8), L != L && m == -INFINITY ? 0.0f : m, L);

@@ -16,12 +16,18 @@
 //   f16's 11 bits, an eighth of the output's own rounding.
 // - K's scale enters as its codes are widened: v_cvt_scalef32_pk_f16_fp8 takes
 //   a power of two per lane, and a lane of the A operand is one key.  It is
-//   taken relative to the largest K scale met so far (kref), 2^7 up, which
-//   keeps every code exact to scales 2^22 below it; 2^kref goes into the
-//   factor of the scores.
+//   taken relative to a K scale (kref), 2^7 up, which keeps every code exact to
+//   scales 2^TK below it; 2^kref goes into the factor of the scores.
 // - V's scale multiplies the planes of p, relative to the largest V scale met
-//   so far (vref; the accumulators are rescaled when it rises): powers of two
-//   in f16, the smallest of them subnormal; 2^vref is applied once at the end.
+//   so far (vref; the accumulators are rescaled when it rises): powers of two in
+//   f16, down to 2^-TV, where the planes still hold 21 bits (one plane: 11);
+//   2^vref is applied once at the end.
+// - Scales further apart than that, which a cache need not have but may (a row of
+//   1e30 must not cost queries that do not see it their bits), take a slower way.
+//   A tile is walked again for each band of K scales, with the keys of the others
+//   hidden.  V's scales go into the exponents of the weights, relative to a vref
+//   of each row's own, so that a row's largest product is the measure of its
+//   others; a wave that has met such a V tile stays on this way (`apart`).
 // - m moves only when a score exceeds it by more than 2^MOVE, so p <= 2^(P0 +
 //   MOVE) = 2^15 with p = exp2(s - m + P0), inside f16's range, and the
 //   O rescale is skipped on almost every tile; out does not depend on m.
@@ -53,6 +59,46 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 constexpr float P0 = 8.0f, MOVE = 7.0f;
+constexpr int TK = 22;
+template <int PL>
+constexpr int TV = PL == 2 ? 12 : 16;
+constexpr int TV_RISE = 64;  // a rise of vref that f32 accumulators stand
+
+// Whether a scale byte is one of values (not of a NaN's row or of none) and lies
+// outside far .. 0 below ref.
+__device__ __forceinline__ bool scale_far(int byte, int ref, int far) {
+    return byte > 1 && byte != FP8_NAN && (byte > ref || byte < ref - far);
+}
+// The factor that widens K's codes of scale `byte` in the band that ends at ref.
+__device__ __forceinline__ float band_scale(int byte, int ref) {
+    return (unsigned)(byte - ref + TK) <= (unsigned)TK ? __uint_as_float((uint32_t)(byte - ref + 127 + 7) << 23) : 0.0f;
+}
+// LDS written by lanes of this wave, before others of it read it.
+__device__ __forceinline__ void wave_lds() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+__device__ __forceinline__ int wave_max(int x) {
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) x = max(x, __shfl_xor(x, off));
+    return x;
+}
+// A band of K scales: bytes of values from ref - TK to ref, with NaN rows in the
+// first band of a tile and rows without values in its last.
+struct Band {
+    int ref;
+    bool first, last;
+    __device__ __forceinline__ bool holds(int byte) const {
+        return byte == FP8_NAN ? first : byte <= 1 ? last : byte <= ref && byte >= ref - TK;
+    }
+};
+// The power of two that brings a row's accumulators, the largest of them `big`, to
+// about 2^16 where they are far from it (0: they are 0, or no number).
+__device__ __forceinline__ int centre(float big) {
+    const int e = (int)(__float_as_uint(big) >> 23) - 127;
+    return big == 0.0f || e > 127 || (e >= 8 && e <= 24) ? 0 : 16 - e;
+}
 
 __device__ __forceinline__ f32x16 mfma(const f16x8& a, const f16x8& b, const f32x16& c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
@@ -288,7 +334,8 @@ struct Fp8State {
 
     Acc o[DB];
     float m, l, kc;
-    int kref, vref;
+    int kref, vref;  // (vref: a row's own once `apart`)
+    bool apart;
     float cq;  // |c| / the row's power of two
 
     __device__ __forceinline__ void init(float cq_) {
@@ -297,9 +344,20 @@ struct Fp8State {
 #pragma unroll
             for (int i = 0; i < SPL; ++i) o[db][i] = 0.0f;
         m = -INFINITY;
-        l = kc = 0.0f;
+        l = 0.0f;
+        kc = FLT_MIN;  // (before any stored key; never 0, a hidden score of -infinity has to stay one)
         kref = vref = 0;
+        apart = false;
         cq = cq_;
+    }
+
+    // o times 2^e, |e| <= 252, in two steps
+    __device__ __forceinline__ void scale(int e) {
+        const float a = pow2_biased(e / 2 + 127), b = pow2_biased(e - e / 2 + 127);
+#pragma unroll
+        for (int db = 0; db < DB; ++db) o[db] *= a;
+#pragma unroll
+        for (int db = 0; db < DB; ++db) o[db] *= b;
     }
 
     // kb0, kb1: K's scale bytes of this lane's A rows (32 rows: the same twice);
@@ -307,44 +365,63 @@ struct Fp8State {
     // step) and vcodes(row block, step): 8 codes as two dwords; query(plane,
     // step).  slow: some key may be hidden from some row, then see(i) tells of
     // the lane's i-th key (NP * half + i) whether its row sees it; kbyte(i), its
-    // K scale byte, is asked where the tile has a NaN.  scored() is called once
+    // K scale byte, is asked where the tile has a NaN.  scored(next) is called once
     // K's codes are read.
     template <class KC, class VC, class Q, class See, class KByte, class Scored>
-    __device__ __forceinline__ void tile(int kb0, int kb1, int vb, _Float16* vs, bool slow, KC kcodes, VC vcodes,
+    // cap: the K scales of this walk end there (FP8_NAN: all).  Returns where those
+    // of the tile's next walk end, 0 after its last.
+    __device__ __forceinline__ int tile(int cap, int kb0, int kb1, int vb, _Float16* vs, bool slow, KC kcodes, VC vcodes,
                                          Q query, See see, KByte kbyte, Scored scored) {
         bool nan = false;
         slow = __builtin_amdgcn_readfirstlane(slow);  // (uniform, and known to be: the masks stay behind a branch)
         const int lane = threadIdx.x & 63, half = lane / QR;
-        // ---- scales: relative to the largest so far
-        if (__any(max(kb0, kb1) > kref || vb > vref)) {
-            // (a NaN's byte is larger than any other, so a tile with one comes here)
-            const int k0 = kb0 == FP8_NAN ? 0 : kb0, k1 = kb1 == FP8_NAN ? 0 : kb1;
-            int kt = max(k0, k1), vt = vb == FP8_NAN ? 0 : vb;
+        // ---- scales: within TK of kref and TV of vref, as almost always?  (A NaN's
+        // byte is above, that of a key without values below all others.)
+        int next = 0;
+        Band band{};
+        bool banded = cap != FP8_NAN;
+        if (__any((unsigned)(kb0 - kref + TK) > (unsigned)TK || (KB > 1 && (unsigned)(kb1 - kref + TK) > (unsigned)TK) ||
+                  (unsigned)(vb - vref + TV<PL>) > (unsigned)TV<PL> || apart || banded)) {
+            const int k0 = kb0 > min(cap, FP8_NAN - 1) ? 0 : kb0, k1 = kb1 > min(cap, FP8_NAN - 1) ? 0 : kb1;
+            const int kt = wave_max(max(k0, k1)), vt = wave_max(vb == FP8_NAN ? 0 : vb);
             nan = __any(kb0 == FP8_NAN || kb1 == FP8_NAN || vb == FP8_NAN);
-#pragma unroll
-            for (int off = 32; off > 0; off >>= 1) {
-                kt = max(kt, __shfl_xor(kt, off));
-                vt = max(vt, __shfl_xor(vt, off));
+            if (kt > 1) {
+                kref = kt;
+                kc = __builtin_fmaxf(ldexpf(cq, kref - 127 - 7), FLT_MIN);
             }
-            kref = max(kref, kt);
-            // (never 0: a hidden score of -infinity has to stay one)
-            kc = ldexpf(cq, kref - 127 - 7);
-            kc = kc < FLT_MIN ? FLT_MIN : kc;
-            if (vt > vref) {
-                if (vref > 0) {  // (else o is 0)
+            next = wave_max(max(scale_far(k0, kref, TK) ? k0 : 0, scale_far(k1, kref, TK) ? k1 : 0));
+            banded = banded || next > 0;
+            band = {kref, cap == FP8_NAN, next == 0};
+            if (!apart && vt > vref && !(vref > 1 && vt > vref + TV_RISE)) {
+                if (vref > 1) {  // (else o is 0)
                     const float f = pow2_biased(vref - vt + 127);
 #pragma unroll
                     for (int db = 0; db < DB; ++db) o[db] *= f;
                 }
                 vref = vt;
             }
+            apart = apart || __any(scale_far(vb, vref, TV<PL>));
+            if (apart) {
+                float big = 0.0f;
+#pragma unroll
+                for (int db = 0; db < DB; ++db)
+#pragma unroll
+                    for (int i = 0; i < SPL; ++i) big = __builtin_fmaxf(big, fabsf(o[db][i]));
+#pragma unroll
+                for (int off = QR; off < 64; off <<= 1) big = __builtin_fmaxf(big, __shfl_xor(big, off));
+                const int up = centre(big);
+                scale(up);
+                vref = big == 0.0f ? 0 : vref - up;
+            }
         }
-        if (lane < 32) vs[lane] = (_Float16)(vb == FP8_NAN ? INFINITY : pow2_biased(vb - vref + 127));
-        const float ks0 = pow2_biased(min(kb0 - kref, 0) + 127 + 7), ks1 = pow2_biased(min(kb1 - kref, 0) + 127 + 7);
+        const bool far = __builtin_amdgcn_readfirstlane(apart);
+        if (lane < 32)
+            vs[lane] = (_Float16)(far ? (float)vb : vb == FP8_NAN ? INFINITY : pow2_biased(vb - vref + 127));
 
         // ---- scores of this lane's column
         float s[NP];
         Acc acc[KB] = {};
+        const float ks0 = band_scale(kb0, kref), ks1 = KB > 1 ? band_scale(kb1, kref) : ks0;
 #pragma unroll
         for (int st = 0; st < NS; ++st)
 #pragma unroll
@@ -358,14 +435,21 @@ struct Fp8State {
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
             for (int i = 0; i < SPL; ++i) s[kb * SPL + i] = acc[kb][i];
-        scored();
+        next = __builtin_amdgcn_readfirstlane(next);
+        scored(next);
 
         // ---- masks: scores the row may not use
         uint32_t hidden = 0;
+        banded = __builtin_amdgcn_readfirstlane(banded);
+        if (__builtin_expect(banded, 0)) {
+            slow = true;
+#pragma unroll
+            for (int i = 0; i < NP; ++i) hidden |= band.holds(kbyte(i)) ? 0 : 1u << i;
+        }
         if (slow) {
 #pragma unroll
             for (int i = 0; i < NP; ++i) {
-                const bool ok = see(i);
+                const bool ok = see(i) && !(hidden >> i & 1);
                 hidden |= ok ? 0 : 1u << i;
                 s[i] = ok ? s[i] : -INFINITY;
             }
@@ -380,33 +464,59 @@ struct Fp8State {
 #pragma unroll
         for (int i = 1; i < NP; ++i) top = __builtin_fmaxf(top, s[i]);
         const float ts = top == -INFINITY ? -INFINITY : top * kc;
-        if (__any(ts > m + MOVE)) {
+        float kcl = kc, l_far = 0.0f;
+        if (__any(ts > m + MOVE) || far) {
             float nm = ts;
 #pragma unroll
             for (int off = QR; off < 64; off <<= 1) nm = __builtin_fmaxf(nm, __shfl_xor(nm, off));
             nm = nm > m + MOVE ? nm : m;
-            const float f = m == nm ? 1.0f : __builtin_amdgcn_exp2f(m - nm);
+            float f = m == nm ? 1.0f : __builtin_amdgcn_exp2f(m - nm);
             l *= f;
+            if (far) {
+                // the weights' sum, and V's scales into their exponents, 2^15 at most
+                const float off = P0 - (nm == -INFINITY ? 0.0f : nm);
+                float most = -INFINITY;
+                wave_lds();
+#pragma unroll
+                for (int i = 0; i < NP; ++i) {
+                    const float byte = (float)vs[NP * half + i];
+                    s[i] = __builtin_fmaf(s[i], kc, off);
+                    l_far += __builtin_amdgcn_exp2f(s[i]);
+                    if (byte != (float)FP8_NAN) most = __builtin_fmaxf(most, s[i] + (byte - (float)vref));
+                }
+                l_far += l;
+#pragma unroll
+                for (int o2 = QR; o2 < 64; o2 <<= 1) most = __builtin_fmaxf(most, __shfl_xor(most, o2));
+                const int rise = most > P0 + MOVE ? (int)__builtin_fminf(ceilf(most - P0), 252.0f) : 0;
+                vref += rise;
+                f *= pow2_biased(127 - rise / 2) * pow2_biased(127 - (rise - rise / 2));
+#pragma unroll
+                for (int i = 0; i < NP; ++i) {
+                    const float byte = (float)vs[NP * half + i];
+                    s[i] = byte == (float)FP8_NAN && s[i] != -INFINITY ? NAN : s[i] + (byte - (float)vref);
+                }
+                wave_lds();
+                if (lane < 32) vs[lane] = (_Float16)1.0f;
+                kcl = 1.0f;
+            }
             if (__any(m != -INFINITY))  // (else o is 0)
 #pragma unroll
                 for (int db = 0; db < DB; ++db) o[db] *= f;
             m = nm;
         }
-        const float off = P0 - (m == -INFINITY ? 0.0f : m);
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        const float off = far || m == -INFINITY ? far ? 0.0f : P0 : P0 - m;
+        wave_lds();
+        f16x8 ph[NP / 8], pl[NP / 8];
         f16x8 sc[NP / 8];
 #pragma unroll
         for (int i = 0; i < NP / 8; ++i) sc[i] = *reinterpret_cast<const f16x8*>(vs + NP * half + 8 * i);
         if (slow)  // (a hidden key's p is 0; a scale of infinity would still make it NaN)
 #pragma unroll
             for (int i = 0; i < NP; ++i) sc[i / 8][i % 8] = hidden >> i & 1 ? (_Float16)0.0f : sc[i / 8][i % 8];
-        f16x8 ph[NP / 8], pl[NP / 8];
 #pragma unroll
         for (int i = 0; i < NP; i += 2) {
-            const f32x2 p = {__builtin_amdgcn_exp2f(__builtin_fmaf(s[i], kc, off)),
-                             __builtin_amdgcn_exp2f(__builtin_fmaf(s[i + 1], kc, off))};
+            const f32x2 p = {__builtin_amdgcn_exp2f(__builtin_fmaf(s[i], kcl, off)),
+                             __builtin_amdgcn_exp2f(__builtin_fmaf(s[i + 1], kcl, off))};
             const f16x2 hi = __builtin_convertvector(p, f16x2);
             if constexpr (PL == 1) {
                 // the sum is of the weights that the product takes
@@ -427,6 +537,7 @@ struct Fp8State {
             ph[i] *= sc[i];
             if constexpr (PL == 2) pl[i] *= sc[i];
         }
+        if (far) l = l_far;
         // ---- O^T += V^T P^T
         constexpr int DG = DB < 4 ? DB : 4;  // row blocks in turn: their MFMAs do not wait for each other
 #pragma unroll
@@ -445,9 +556,8 @@ struct Fp8State {
                     for (int k = 0; k < DG; ++k) o[d0 + k] = mfma(v8[k], pl[st], o[d0 + k]);
             }
         // (the next tile's V scales are written after this tile's reads)
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        wave_lds();
+        return next;
     }
 
     // l over the lanes that share a column
@@ -459,7 +569,7 @@ struct Fp8State {
     }
     // o's weight next to a state of maximum M, 2^vref (V's common factor) included
     __device__ __forceinline__ float weight(float M) const {
-        return (m == -INFINITY ? (l != l ? l : 0.0f) : __builtin_amdgcn_exp2f(m - M)) * fp8_scale(vref);
+        return ldexpf(m == -INFINITY ? (l != l ? l : 0.0f) : __builtin_amdgcn_exp2f(m - M), vref - 127);
     }
     // the dim of o[db][i], i a multiple of 4: four consecutive dims from there
     __device__ static __forceinline__ int dim(int db, int i, int half) {
