@@ -139,32 +139,41 @@ void attn_fp8_kernel(const AttnArgs a) {
             for (int s = 0; s < T::NS; ++s) q[p][s] = staged(p, s);
 
     T st;
-    st.init(fabsf(a.c) * srow[col]);
-    for (int t = t_first, cap = FP8_NAN; t < t1;) {
-        int then = t;
-        const int next = st.tile(
-            cap, x.kb0, x.kb1, x.vb, svs + wave * 32, !tile_visible(a, S.nk, t, q_lo, q_hi),
-            [&](int kb, int s) {
-                const u32x4& w = x.k[kb * (G::KCH / 2) + s / 2];
-                return u32x2{w[s % 2 * 2], w[s % 2 * 2 + 1]};
-            },
-            [&](int db, int s) {
-                const int i = (db * (T::NP / 8) + s) * 2;
-                return u32x2{x.v[i], x.v[i + 1]};
-            },
-            [&](int p, int s) { return G::BIG ? staged(p, s) : q[p][G::BIG ? 0 : s]; },
-            [&](int i) {
-                const int key = 32 * t + T::NP * half + i;
-                return (key < S.nk) & visible(my_pos, key, 0, 0, a.window, a.prefix);
-            },
-            [&](int i) { return (int)gload<uint8_t>(sbase + (size_t)t * 64 + T::NP * half + i); },
-            [&](int again) {
-                then = again ? t : t + NW;
-                fetch_k(then, x);
-            });
-        fetch_v(then, x);
-        t = then;
-        cap = next ? next : FP8_NAN;
+    auto walk = [&](auto far) __attribute__((always_inline)) {
+        st.init(fabsf(a.c) * srow[col]);
+        for (int t = t_first, cap = FP8_NAN; t < t1;) {
+            int then = t;
+            const int next = st.template tile<decltype(far)::value>(
+                cap, x.kb0, x.kb1, x.vb, svs + wave * 32, !tile_visible(a, S.nk, t, q_lo, q_hi),
+                [&](int kb, int s) {
+                    const u32x4& w = x.k[kb * (G::KCH / 2) + s / 2];
+                    return u32x2{w[s % 2 * 2], w[s % 2 * 2 + 1]};
+                },
+                [&](int db, int s) {
+                    const int i = (db * (T::NP / 8) + s) * 2;
+                    return u32x2{x.v[i], x.v[i + 1]};
+                },
+                [&](int p, int s) { return G::BIG ? staged(p, s) : q[p][G::BIG ? 0 : s]; },
+                [&](int i) {
+                    const int key = 32 * t + T::NP * half + i;
+                    return (key < S.nk) & visible(my_pos, key, 0, 0, a.window, a.prefix);
+                },
+                [&](int i) { return (int)gload<uint8_t>(sbase + (size_t)t * 64 + T::NP * half + i); },
+                [&](int again) {
+                    then = again ? t : t + NW;
+                    fetch_k(then, x);
+                });
+            if (!decltype(far)::value && next < 0) return false;
+            fetch_v(then, x);
+            t = then;
+            cap = next ? next : FP8_NAN;
+        }
+        return true;
+    };
+    if (!walk(std::false_type{})) {
+        fetch_k(t_first, x);
+        fetch_v(t_first, x);
+        walk(std::true_type{});
     }
     if constexpr (G::BIG) __syncthreads();  // (the merge area lies over the query rows)
     fp8_finish<HD, QR, PL, NW>(a, S, at, st, r0, reinterpret_cast<float*>(lds), sm, sl, sr, stick);

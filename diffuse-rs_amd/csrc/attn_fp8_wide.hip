@@ -115,14 +115,21 @@ void attn_fp8_wide_kernel(const AttnArgs a) {
     __syncthreads();  // (the partial scores lie over the query rows)
 
     f32x16 o[DB];
-#pragma unroll
-    for (int db = 0; db < DB; ++db)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) o[db][i] = 0.0f;
-    float m = -INFINITY, l = 0.0f;  // row col's maximum; this lane's part of its sum
-    int kref = 0, vref = 0;  // (vref: a row's own once `apart`)
+    float m, l;         // row col's maximum; this lane's part of its sum
+    int kref, vref;     // (vref: a row's own once `apart`)
     bool apart = false;
-    float kc = FLT_MIN;
+    float kc;
+    auto init = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[db][i] = 0.0f;
+        m = -INFINITY;
+        l = 0.0f;
+        kref = vref = 0;
+        kc = FLT_MIN;
+    };
+    init();
     // the tile whose weights wait in LDS: its scores and what turns them into weights
     float s[4], s_kc = 0.0f, l_before = 0.0f;
     f16x2 s_vs[2];
@@ -201,33 +208,39 @@ void attn_fp8_wide_kernel(const AttnArgs a) {
     // Walk k of this workgroup: tile t's scores, the values of the walk before, its
     // weights.  (cap and t as of Fp8State::tile and its loop.)
     int t = t0, cap = FP8_NAN;
-    auto step = [&](int k) __attribute__((always_inline)) {
+    auto step = [&](auto far_way, int k) __attribute__((always_inline)) {
+        constexpr bool FAR = decltype(far_way)::value;
         // ---- K's and V's scales, the partial scores
         bool nan = false;
         float vdown = 1.0f;
         int next = 0;
         Band band{};
-        bool banded = cap != FP8_NAN;
+        bool banded = FAR && cap != FP8_NAN;
         if (__any((unsigned)(x.kb - kref + TK) > (unsigned)TK || (unsigned)(x.vb - vref + TV<PL>) > (unsigned)TV<PL> ||
-                  apart || banded)) {
+                  (FAR && (apart || banded)))) {
             // (the same decisions in every wave: each sees all 64 bytes)
             const int k0 = x.kb > min(cap, FP8_NAN - 1) ? 0 : x.kb;
             const int kt = wave_max(k0), vt = wave_max(x.vb == FP8_NAN ? 0 : x.vb);
             nan = __any(x.kb == FP8_NAN || x.vb == FP8_NAN);
-            if (kt > 1) {
+            if (kt > kref || __any(scale_far(k0, kref, TK)) || (FAR && kt > 1)) {
                 kref = kt;
                 kc = __builtin_fmaxf(ldexpf(cq, kref - 127 - 7), FLT_MIN);
             }
-            next = wave_max(scale_far(k0, kref, TK) ? k0 : 0);
-            banded = banded || next > 0;
-            band = {kref, cap == FP8_NAN, next == 0};
-            if (!apart && vt > vref && !(vref > 1 && vt > vref + TV_RISE)) {
+            if constexpr (FAR) {
+                next = wave_max(scale_far(k0, kref, TK) ? k0 : 0);
+                banded = banded || next > 0;
+                band = {kref, cap == FP8_NAN, next == 0};
+            } else if (__builtin_expect(__any(scale_far(k0, kref, TK) || scale_far(x.vb, max(vref, vt), TV<PL>)) ||
+                                            (vref > 1 && vt > vref + TV_RISE), 0)) {
+                return false;
+            }
+            if (!(FAR && apart) && vt > vref && !(vref > 1 && vt > vref + TV_RISE)) {
                 if (vref > 1) vdown = pow2_biased(vref - vt + 127);
                 vref = vt;
             }
-            apart = apart || __any(scale_far(x.vb, vref, TV<PL>));
+            if constexpr (FAR) apart = apart || __any(scale_far(x.vb, vref, TV<PL>));
         }
-        const bool far = __builtin_amdgcn_readfirstlane(apart);
+        const bool far = FAR && __builtin_amdgcn_readfirstlane(apart);
         const bool slow = __builtin_amdgcn_readfirstlane(!tile_visible(a, nk, t, q_lo, q_hi));
         const uint32_t vbytes = x.vq;
         f16x2 vs[2];  // V's scales of the four keys
@@ -245,7 +258,7 @@ void attn_fp8_wide_kernel(const AttnArgs a) {
 #pragma unroll
             for (int p = 0; p < PL; ++p) acc = mfma(k8, q[p][st], acc);
         }
-        next = __builtin_amdgcn_readfirstlane(next);
+        if constexpr (FAR) next = __builtin_amdgcn_readfirstlane(next);
         const int then = next ? t : t + 1;
         fetch_k(then, x, kq);
         char* const mine = part + (k & 1) * G::PART + wave * 4096 + lane * 16;
@@ -273,7 +286,7 @@ void attn_fp8_wide_kernel(const AttnArgs a) {
             s_vs[0] = vs[0];
             s_vs[1] = vs[1];
             s_kc = kc;
-            if (__builtin_expect(banded, 0)) {
+            if (FAR && banded) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
                     if (!band.holds(gload<uint8_t>(sbase + (size_t)t * 64 + 16 * half + 4 * quad + j))) {
@@ -314,7 +327,7 @@ void attn_fp8_wide_kernel(const AttnArgs a) {
         if (__builtin_amdgcn_readfirstlane(__float_as_int(vdown)) != __float_as_int(1.0f))
 #pragma unroll
             for (int db = 0; db < DB; ++db) o[db] *= vdown;
-        if (__builtin_expect(far, 0)) {
+        if (far) {
             // the row's accumulators at a size of their own, then its maximum, then
             // V's scales into the weights' exponents: each as all four waves see it
             auto row_most = [&](float* in, float x) __attribute__((always_inline)) {
@@ -370,12 +383,25 @@ void attn_fp8_wide_kernel(const AttnArgs a) {
         }
         t = then;
         cap = next ? next : FP8_NAN;
+        return true;
     };
 
     if (t0 < t1) {
         fetch_k(t0, x, kq);
         int n = 0;
-        while (t < t1) step(n++);
+        bool ok = true;
+        while (t < t1 && ok) ok = step(std::false_type{}, n++);
+        if (__builtin_expect(!ok, 0)) {
+            // scales too far apart for the common way: from the start, on the other
+            // (all waves decide alike, before a walk's first access to LDS)
+            lds_barrier();
+            if (tid < 2) sflag[tid] = 0;
+            lds_barrier();
+            init();
+            t = t0;
+            fetch_k(t0, x, kq);
+            for (n = 0; t < t1;) step(std::true_type{}, n++);
+        }
         lds_barrier();
         f16x8 w[2][PL];
         weights(n - 1, w);

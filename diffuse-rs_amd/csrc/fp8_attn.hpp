@@ -23,11 +23,13 @@
 //   f16, down to 2^-TV, where the planes still hold 21 bits (one plane: 11);
 //   2^vref is applied once at the end.
 // - Scales further apart than that, which a cache need not have but may (a row of
-//   1e30 must not cost queries that do not see it their bits), take a slower way.
+//   1e30 must not cost queries that do not see it their bits), take a slower way
+//   (FAR), on which a wave that meets them starts again; the common loop carries
+//   nothing of it (as branches of one loop it cost every call 6-17 %).
 //   A tile is walked again for each band of K scales, with the keys of the others
 //   hidden.  V's scales go into the exponents of the weights, relative to a vref
 //   of each row's own, so that a row's largest product is the measure of its
-//   others; a wave that has met such a V tile stays on this way (`apart`).
+//   others (`apart`, from the first V tile that needs it).
 // - m moves only when a score exceeds it by more than 2^MOVE, so p <= 2^(P0 +
 //   MOVE) = 2^15 with p = exp2(s - m + P0), inside f16's range, and the
 //   O rescale is skipped on almost every tile; out does not depend on m.
@@ -367,9 +369,10 @@ struct Fp8State {
     // the lane's i-th key (NP * half + i) whether its row sees it; kbyte(i), its
     // K scale byte, is asked where the tile has a NaN.  scored(next) is called once
     // K's codes are read.
-    template <class KC, class VC, class Q, class See, class KByte, class Scored>
-    // cap: the K scales of this walk end there (FP8_NAN: all).  Returns where those
-    // of the tile's next walk end, 0 after its last.
+    // Without FAR: returns -1, with the state spoilt, where scales lie too far apart,
+    // else 0.  With it: cap, where the K scales of this walk end (FP8_NAN: all);
+    // returns where those of the tile's next walk end, 0 after its last.
+    template <bool FAR, class KC, class VC, class Q, class See, class KByte, class Scored>
     __device__ __forceinline__ int tile(int cap, int kb0, int kb1, int vb, _Float16* vs, bool slow, KC kcodes, VC vcodes,
                                          Q query, See see, KByte kbyte, Scored scored) {
         bool nan = false;
@@ -379,20 +382,26 @@ struct Fp8State {
         // byte is above, that of a key without values below all others.)
         int next = 0;
         Band band{};
-        bool banded = cap != FP8_NAN;
+        bool banded = FAR && cap != FP8_NAN;
         if (__any((unsigned)(kb0 - kref + TK) > (unsigned)TK || (KB > 1 && (unsigned)(kb1 - kref + TK) > (unsigned)TK) ||
-                  (unsigned)(vb - vref + TV<PL>) > (unsigned)TV<PL> || apart || banded)) {
+                  (unsigned)(vb - vref + TV<PL>) > (unsigned)TV<PL> || (FAR && (apart || banded)))) {
             const int k0 = kb0 > min(cap, FP8_NAN - 1) ? 0 : kb0, k1 = kb1 > min(cap, FP8_NAN - 1) ? 0 : kb1;
             const int kt = wave_max(max(k0, k1)), vt = wave_max(vb == FP8_NAN ? 0 : vb);
             nan = __any(kb0 == FP8_NAN || kb1 == FP8_NAN || vb == FP8_NAN);
-            if (kt > 1) {
+            if (kt > kref || __any(scale_far(k0, kref, TK) || scale_far(k1, kref, TK)) || (FAR && kt > 1)) {
                 kref = kt;
                 kc = __builtin_fmaxf(ldexpf(cq, kref - 127 - 7), FLT_MIN);
             }
-            next = wave_max(max(scale_far(k0, kref, TK) ? k0 : 0, scale_far(k1, kref, TK) ? k1 : 0));
-            banded = banded || next > 0;
-            band = {kref, cap == FP8_NAN, next == 0};
-            if (!apart && vt > vref && !(vref > 1 && vt > vref + TV_RISE)) {
+            if constexpr (FAR) {
+                next = wave_max(max(scale_far(k0, kref, TK) ? k0 : 0, scale_far(k1, kref, TK) ? k1 : 0));
+                banded = banded || next > 0;
+                band = {kref, cap == FP8_NAN, next == 0};
+            } else if (__builtin_expect(__any(scale_far(k0, kref, TK) || scale_far(k1, kref, TK) ||
+                                              scale_far(vb, max(vref, vt), TV<PL>)) ||
+                                            (vref > 1 && vt > vref + TV_RISE), 0)) {
+                return -1;
+            }
+            if (!(FAR && apart) && vt > vref && !(vref > 1 && vt > vref + TV_RISE)) {
                 if (vref > 1) {  // (else o is 0)
                     const float f = pow2_biased(vref - vt + 127);
 #pragma unroll
@@ -400,8 +409,8 @@ struct Fp8State {
                 }
                 vref = vt;
             }
-            apart = apart || __any(scale_far(vb, vref, TV<PL>));
-            if (apart) {
+            if constexpr (FAR) apart = apart || __any(scale_far(vb, vref, TV<PL>));
+            if (FAR && apart) {
                 float big = 0.0f;
 #pragma unroll
                 for (int db = 0; db < DB; ++db)
@@ -414,7 +423,7 @@ struct Fp8State {
                 vref = big == 0.0f ? 0 : vref - up;
             }
         }
-        const bool far = __builtin_amdgcn_readfirstlane(apart);
+        const bool far = FAR && __builtin_amdgcn_readfirstlane(apart);
         if (lane < 32)
             vs[lane] = (_Float16)(far ? (float)vb : vb == FP8_NAN ? INFINITY : pow2_biased(vb - vref + 127));
 
@@ -435,13 +444,12 @@ struct Fp8State {
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
             for (int i = 0; i < SPL; ++i) s[kb * SPL + i] = acc[kb][i];
-        next = __builtin_amdgcn_readfirstlane(next);
+        if constexpr (FAR) next = __builtin_amdgcn_readfirstlane(next);
         scored(next);
 
         // ---- masks: scores the row may not use
         uint32_t hidden = 0;
-        banded = __builtin_amdgcn_readfirstlane(banded);
-        if (__builtin_expect(banded, 0)) {
+        if (FAR && __builtin_amdgcn_readfirstlane(banded)) {
             slow = true;
 #pragma unroll
             for (int i = 0; i < NP; ++i) hidden |= band.holds(kbyte(i)) ? 0 : 1u << i;
@@ -557,7 +565,7 @@ struct Fp8State {
             }
         // (the next tile's V scales are written after this tile's reads)
         wave_lds();
-        return next;
+        return FAR ? next : 0;
     }
 
     // l over the lanes that share a column
