@@ -163,14 +163,13 @@ void attn_fp8_kernel(const AttnArgs a) {
                     then = again ? t : t + NW;
                     fetch_k(then, x);
                 });
-            if (!decltype(far)::value && next < 0) return false;
             fetch_v(then, x);
             t = then;
             cap = next ? next : FP8_NAN;
         }
-        return true;
     };
-    if (!walk(std::false_type{})) {
+    walk(std::false_type{});
+    if (__builtin_expect(__builtin_amdgcn_readfirstlane(st.bad), 0)) {
         fetch_k(t_first, x);
         fetch_v(t_first, x);
         walk(std::true_type{});

@@ -117,7 +117,7 @@ void attn_fp8_wide_kernel(const AttnArgs a) {
     f32x16 o[DB];
     float m, l;         // row col's maximum; this lane's part of its sum
     int kref, vref;     // (vref: a row's own once `apart`)
-    bool apart = false;
+    bool apart = false, bad = false;
     float kc;
     auto init = [&]() __attribute__((always_inline)) {
 #pragma unroll
@@ -232,7 +232,7 @@ void attn_fp8_wide_kernel(const AttnArgs a) {
                 band = {kref, cap == FP8_NAN, next == 0};
             } else if (__builtin_expect(__any(scale_far(k0, kref, TK) || scale_far(x.vb, max(vref, vt), TV<PL>)) ||
                                             (vref > 1 && vt > vref + TV_RISE), 0)) {
-                return false;
+                bad = true;
             }
             if (!(FAR && apart) && vt > vref && !(vref > 1 && vt > vref + TV_RISE)) {
                 if (vref > 1) vdown = pow2_biased(vref - vt + 127);
@@ -383,24 +383,23 @@ void attn_fp8_wide_kernel(const AttnArgs a) {
         }
         t = then;
         cap = next ? next : FP8_NAN;
-        return true;
     };
 
     if (t0 < t1) {
         fetch_k(t0, x, kq);
         int n = 0;
-        bool ok = true;
-        while (t < t1 && ok) ok = step(std::false_type{}, n++);
-        if (__builtin_expect(!ok, 0)) {
+        while (t < t1) step(std::false_type{}, n++);
+        if (__builtin_expect(__builtin_amdgcn_readfirstlane(bad), 0)) {
             // scales too far apart for the common way: from the start, on the other
-            // (all waves decide alike, before a walk's first access to LDS)
+            // (all waves decide alike)
             lds_barrier();
             if (tid < 2) sflag[tid] = 0;
             lds_barrier();
             init();
             t = t0;
             fetch_k(t0, x, kq);
-            for (n = 0; t < t1;) step(std::true_type{}, n++);
+            n = 0;
+            while (t < t1) step(std::true_type{}, n++);
         }
         lds_barrier();
         f16x8 w[2][PL];

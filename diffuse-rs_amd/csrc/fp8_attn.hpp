@@ -337,7 +337,7 @@ struct Fp8State {
     Acc o[DB];
     float m, l, kc;
     int kref, vref;  // (vref: a row's own once `apart`)
-    bool apart;
+    bool apart, bad;  // (bad: scales too far apart without FAR, the state is worth nothing)
     float cq;  // |c| / the row's power of two
 
     __device__ __forceinline__ void init(float cq_) {
@@ -349,7 +349,7 @@ struct Fp8State {
         l = 0.0f;
         kc = FLT_MIN;  // (before any stored key; never 0, a hidden score of -infinity has to stay one)
         kref = vref = 0;
-        apart = false;
+        apart = bad = false;
         cq = cq_;
     }
 
@@ -369,9 +369,8 @@ struct Fp8State {
     // the lane's i-th key (NP * half + i) whether its row sees it; kbyte(i), its
     // K scale byte, is asked where the tile has a NaN.  scored(next) is called once
     // K's codes are read.
-    // Without FAR: returns -1, with the state spoilt, where scales lie too far apart,
-    // else 0.  With it: cap, where the K scales of this walk end (FP8_NAN: all);
-    // returns where those of the tile's next walk end, 0 after its last.
+    // With FAR: cap, where the K scales of this walk end (FP8_NAN: all); returns where
+    // those of the tile's next walk end, 0 after its last.
     template <bool FAR, class KC, class VC, class Q, class See, class KByte, class Scored>
     __device__ __forceinline__ int tile(int cap, int kb0, int kb1, int vb, _Float16* vs, bool slow, KC kcodes, VC vcodes,
                                          Q query, See see, KByte kbyte, Scored scored) {
@@ -399,7 +398,7 @@ struct Fp8State {
             } else if (__builtin_expect(__any(scale_far(k0, kref, TK) || scale_far(k1, kref, TK) ||
                                               scale_far(vb, max(vref, vt), TV<PL>)) ||
                                             (vref > 1 && vt > vref + TV_RISE), 0)) {
-                return -1;
+                bad = true;
             }
             if (!(FAR && apart) && vt > vref && !(vref > 1 && vt > vref + TV_RISE)) {
                 if (vref > 1) {  // (else o is 0)
