@@ -10,6 +10,18 @@
 // loads run under the rest of the step and a tile ahead costs no registers.
 // Few workgroups split the keys further; the last of a row block to finish
 // joins them.
+//
+// What bounds it.  One row over a long cache: the stream of the codes (f32 row,
+// 32/8 heads of 128, 131072 keys: 268 MB in 53 us, 5.0 TB/s, where a copy reaches
+// 5.2).  Few tiles: latencies in a row, arguments 1 us, query rows 1, first tiles
+// 2-4, the waves' meeting 2 (256 f32 rows, 32 heads, 768 keys: 13 us, of which
+// 5.5 are the products' and 4 the bytes').  Many tiles: the vector units, 226
+// instructions a tile and wave at 4.3-6.6 clk beside 16 or 32 MFMAs of 32 (4096
+// bf16 rows, 32 heads, causal: 138 GFLOP in 200 us, 690 TFLOP/s; counters: vector
+// units 57-62 %, matrix cores 30 % of the time, which nearly add up).  Tried
+// there without gain: three waves a SIMD (199 against 200 us), 64 rows a wave so
+// that codes are widened once for two blocks (265, registers), tiles shared
+// through LDS (255-290), waves on different rows (215-222).
 #include "fp8_attn.hpp"
 
 #include <algorithm>

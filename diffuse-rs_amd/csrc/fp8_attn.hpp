@@ -1,5 +1,5 @@
 // fp8_attn.hpp -- what the attention kernels of DR_PRECISION_FP8 layers share
-// (attn_fp8.hip): loading and splitting query rows, the
+// (attn_fp8.hip, attn_fp8_wide.hip): loading and splitting query rows, the
 // widening of codes, one key tile's scores, softmax and values, the output rows.
 //
 // With codes k, v and scales 2^ek, 2^ev of a position, and c = scale * log2 e:
@@ -24,8 +24,8 @@
 //   2^vref is applied once at the end.
 // - Scales further apart than that, which a cache need not have but may (a row of
 //   1e30 must not cost queries that do not see it their bits), take a slower way
-//   (FAR), on which a wave that meets them starts again; the common loop carries
-//   nothing of it (as branches of one loop it cost every call 6-17 %).
+//   (FAR), on which a wave that has met them starts again; the common loop only
+//   notes them (as branches of one loop that way cost every call 6-17 %).
 //   A tile is walked again for each band of K scales, with the keys of the others
 //   hidden.  V's scales go into the exponents of the weights, relative to a vref
 //   of each row's own, so that a row's largest product is the measure of its

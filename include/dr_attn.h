@@ -148,8 +148,9 @@ void dr_pass_destroy(dr_pass* pass);
 
 /*
  * StepCache -- src/model/cache.rs:25-115.  Per layer, per batch slot, K and V
- * for every sequence position 0..n_total, stored as bf16 in HBM (K row-major
- * per KV head, V transposed per KV head).  StepCache::new (:44-54) takes
+ * for every sequence position 0..n_total, in HBM: as bf16 (K row-major per KV
+ * head, V transposed per KV head) unless a layer's precision says otherwise
+ * (dr_cache_set_precision).  StepCache::new (:44-54) takes
  * per-layer strides n_head_kv * head_dim (forward.rs:267); here the two
  * factors are given separately.  n_batch > 1 holds several independent
  * streams (e.g. the conditional and unconditional CFG streams, each of which
@@ -530,9 +531,9 @@ int dr_ctx_set_kernel(dr_ctx* ctx, int kernel);
  * DR_DTYPE_BF16: q points at bf16 rows of the same shape (uint16 bit
  * patterns), read by the per-wave-stream kernel, which applies the Q
  * epilogue and the scale to them as to f32 rows, and on DR_PRECISION_FP8
- * layers by theirs.  Calls on other layers that that kernel cannot run (head dims other than 128 / 256, hi/lo layers, RoPE below full
- * rotary, forced tile shapes) fail with DR_ERR_UNSUPPORTED before any
- * store. */
+ * layers by theirs.  Calls on other layers that the per-wave-stream kernel
+ * cannot run (head dims other than 128 / 256, hi/lo layers, RoPE below full
+ * rotary, forced tile shapes) fail with DR_ERR_UNSUPPORTED before any store. */
 #define DR_DTYPE_F32 0
 #define DR_DTYPE_BF16 1
 int dr_ctx_set_q_dtype(dr_ctx* ctx, int dtype);
