@@ -425,7 +425,8 @@ void attn_fp8_wide_kernel(const AttnArgs a) {
     const size_t plane = (size_t)a.n_batch * a.n_head_kv * a.part_rows;
     const __amdgpu_buffer_rsrc_t ro = make_rsrc(a.part_o, 0xffffffffu);
     const __amdgpu_buffer_rsrc_t rm = make_rsrc(a.part_ml, 0xffffffffu);
-    const int e2 = vref - 127;
+    // (split rows meet at 2^-LOW)
+    const int e2 = vref - 127 - (a.n_split > 1 ? LOW : 0);
     const float up0 = pow2_biased(e2 / 2 + 127), up1 = pow2_biased(e2 - e2 / 2 + 127);
     const int i = rb * 32 + col;
     float L = 0.0f;
@@ -440,7 +441,7 @@ void attn_fp8_wide_kernel(const AttnArgs a) {
                 f32x4{o[db][e], o[db][e + 1], o[db][e + 2], o[db][e + 3]} * f * up0 * up1;
     // (a NaN without any finite score must not pass for a row without keys)
     if (a.n_split > 1 && quad == 0 && half == 0 && i < nr)
-        store2_sc1(rm, (int)(((size_t)at.split * plane + prow0 + i) * 8), L != L && m == -INFINITY ? 0.0f : m, L);
+        store2_sc1(rm, (int)(((size_t)at.split * plane + prow0 + i) * 8), L != L && m == -INFINITY ? 0.0f : m, L * pow2_biased(127 - LOW));
     __syncthreads();
     for (int p = tid; p < nr * (HD / 4); p += 512) {
         const int i = p / (HD / 4), d = p % (HD / 4) * 4;

@@ -64,6 +64,9 @@ constexpr float P0 = 8.0f, MOVE = 7.0f;
 constexpr int TK = 22;
 template <int PL>
 constexpr int TV = PL == 2 ? 12 : 16;
+// Rows meet at 2^-LOW of themselves: sums of weights that start at 2^P0 would take
+// values above 1e33 out of f32 before the division by the weights' sum.
+constexpr int LOW = 16;
 constexpr int TV_RISE = 64;  // a rise of vref that f32 accumulators stand
 
 // Whether a scale byte is one of values (not of a NaN's row or of none) and lies
@@ -574,9 +577,10 @@ struct Fp8State {
         for (int off = QR; off < 64; off <<= 1) t += __shfl_xor(t, off);
         return t;
     }
-    // o's weight next to a state of maximum M, 2^vref (V's common factor) included
+    // o's weight next to a state of maximum M, 2^vref (V's common factor) included,
+    // and 2^-LOW, as for the sums
     __device__ __forceinline__ float weight(float M) const {
-        return ldexpf(m == -INFINITY ? (l != l ? l : 0.0f) : __builtin_amdgcn_exp2f(m - M), vref - 127);
+        return ldexpf(m == -INFINITY ? (l != l ? l : 0.0f) : __builtin_amdgcn_exp2f(m - M), vref - 127 - LOW);
     }
     // the dim of o[db][i], i a multiple of 4: four consecutive dims from there
     __device__ static __forceinline__ int dim(int db, int i, int half) {
@@ -770,7 +774,7 @@ __device__ __forceinline__ void fp8_finish(const AttnArgs& a, const AttnSlot& S,
 #pragma unroll
         for (int k = 0; k < NW; ++k) {
             const float mw = sm[k * QR + col], lw = sl[k * QR + col];
-            L += mw == -INFINITY ? (lw != lw ? lw : 0.0f) : lw * __builtin_amdgcn_exp2f(mw - M);
+            L += mw == -INFINITY ? (lw != lw ? lw : 0.0f) : lw * __builtin_amdgcn_exp2f(mw - M - (float)LOW);
         }
         sr[col] = M;
         sr[QR + col] = L;

@@ -134,3 +134,18 @@ def test_positions_never_stored(dev, shape, bf16):
     run(dev, p, wave, bf16, prefix=n, store=store)
     run(dev, p, wave, bf16, window=12, store=store)
     run(dev, p, wave, bf16, window=12, prefix=60, store=store, split=2)
+
+
+@BF16
+@SHAPES
+@pytest.mark.parametrize("size", [1e35, 1e-33])
+def test_the_ends_of_the_range(dev, shape, size, bf16):
+    """Outputs near the largest and the smallest numbers: rows of that size, sums
+    of a few hundred weights over them."""
+    h, hkv, hd, wave = shape
+    rng = np.random.default_rng(hd + wave + 4)
+    p = Problem(rng, h, hkv, hd, 260, range(200, 240))
+    p.v *= np.float32(size)
+    run(dev, p, wave, bf16)
+    run(dev, p, wave, bf16, prefix=230, split=3)
+    run(dev, p, wave, bf16, window=1)
