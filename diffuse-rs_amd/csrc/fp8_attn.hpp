@@ -84,10 +84,17 @@ __device__ __forceinline__ void wave_lds() {
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
+// The largest of 64 lanes' values, uniform: along each row of 16 lanes, then row to
+// row, by DPP (a chain of 6 vector instructions; shuffles through LDS take 6 round
+// trips).
 __device__ __forceinline__ int wave_max(int x) {
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) x = max(x, __shfl_xor(x, off));
-    return x;
+    x = max(x, __builtin_amdgcn_update_dpp(x, x, 0x111, 0xf, 0xf, false));  // row_shr:1
+    x = max(x, __builtin_amdgcn_update_dpp(x, x, 0x112, 0xf, 0xf, false));  // row_shr:2
+    x = max(x, __builtin_amdgcn_update_dpp(x, x, 0x114, 0xf, 0xf, false));  // row_shr:4
+    x = max(x, __builtin_amdgcn_update_dpp(x, x, 0x118, 0xf, 0xf, false));  // row_shr:8
+    x = max(x, __builtin_amdgcn_update_dpp(x, x, 0x142, 0xa, 0xf, false));  // row_bcast:15
+    x = max(x, __builtin_amdgcn_update_dpp(x, x, 0x143, 0xc, 0xf, false));  // row_bcast:31
+    return __builtin_amdgcn_readlane(x, 63);
 }
 // A band of K scales: bytes of values from ref - TK to ref, with NaN rows in the
 // first band of a tile and rows without values in its last.
