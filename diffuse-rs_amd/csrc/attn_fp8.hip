@@ -14,7 +14,7 @@
 // What bounds it.  One row over a long cache: the stream of the codes (f32 row,
 // 32/8 heads of 128, 131072 keys: 268 MB in 53 us, 5.0 TB/s, where a copy reaches
 // 5.2).  Few tiles: latencies in a row, arguments 1 us, query rows 1, first tiles
-// 2-4, the waves' meeting 2 (256 f32 rows, 32 heads, 768 keys: 13 us, of which
+// 2-4, the waves' meeting 2 (256 f32 rows, 32 heads, 768 keys: 12-13 us, of which
 // 5.5 are the products' and 4 the bytes').  Many tiles: the vector units, 226
 // instructions a tile and wave at 4.3-6.6 clk beside 16 or 32 MFMAs of 32 (4096
 // bf16 rows, 32 heads, causal: 138 GFLOP in 200 us, 690 TFLOP/s; counters: vector
@@ -234,6 +234,9 @@ hipError_t launch_hd(const LaunchPlan& p, const AttnArgs& a, hipStream_t st) {
 // split often, and 64 rows are dear to join: 32 rows over 32768 keys 117 / 147.)
 //
 // Waves: 8 where a workgroup per CU is all there is, else 4, two workgroups per CU.
+// 8 / 4 waves: 256 f32 rows x 32 heads of 128 over 768 keys (256 workgroups) 13.8 /
+// 14.7 us, 512 x 16 heads over 2553 29.0 / 32.1; 300 x 32/8 heads over 2000 (304)
+// 40.4 / 34.2, 1000 bf16 rows (1000) 66 / 54.
 //
 // Key splits.  A step of a workgroup (one tile of each wave, or of the wide kernel)
 // takes `step` us, a split's join reads its rows of floats at 13000 a us, and a join
@@ -241,7 +244,7 @@ hipError_t launch_hd(const LaunchPlan& p, const AttnArgs& a, hipStream_t st) {
 // sqrt(steps * step * 13000 / floats).  More workgroups than CUs only wait for each
 // other (16 rows x 8 heads of 256 dims over 32768 keys: 16 splits 38 us, 32 61).
 // A split for every tile and CU, as cheap single rows take it, costs more rows up to
-// twice the time (5 rows x 4 heads of 512 dims, 4352 keys: 34 splits 44 us, 9 33).
+// twice the time (5 rows x 16/2 heads of 512 dims, 4352 keys: 34 splits 44 us, 9 33).
 LaunchPlan plan_fp8(int hd_tile, int n_batch, int n_head_kv, int group, int max_nq, int max_nk, int mask, int n_cu,
                     int force_split, int force_rows, int max_tickets) {
     LaunchPlan p{};
