@@ -585,9 +585,12 @@ struct Fp8State {
         return t;
     }
     // o's weight next to a state of maximum M, 2^vref (V's common factor) included,
-    // and 2^-LOW, as for the sums
-    __device__ __forceinline__ float weight(float M) const {
-        return ldexpf(m == -INFINITY ? (l != l ? l : 0.0f) : __builtin_amdgcn_exp2f(m - M), vref - 127 - LOW);
+    // and 2^-LOW, as for the sums: two factors, since for the smallest rows their
+    // product is subnormal, which would cost o's bits (1e-36: all but 7)
+    __device__ __forceinline__ f32x2 weight(float M) const {
+        const int e = vref - 127 - LOW;
+        const float w = m == -INFINITY ? (l != l ? l : 0.0f) : __builtin_amdgcn_exp2f(m - M);
+        return f32x2{w * pow2_biased(e / 2 + 127), pow2_biased(e - e / 2 + 127)};
     }
     // the dim of o[db][i], i a multiple of 4: four consecutive dims from there
     __device__ static __forceinline__ int dim(int db, int i, int half) {
@@ -786,13 +789,13 @@ __device__ __forceinline__ void fp8_finish(const AttnArgs& a, const AttnSlot& S,
         sr[col] = M;
         sr[QR + col] = L;
     }
-    const float f = st.weight(M);
+    const f32x2 f = st.weight(M);
 #pragma unroll
     for (int db = 0; db < T::DB; ++db)
 #pragma unroll
         for (int i = 0; i < T::SPL; i += 4)
             *reinterpret_cast<f32x4*>(so + (wave * QR + col) * OP + T::dim(db, i, half)) =
-                f32x4{st.o[db][i] * f, st.o[db][i + 1] * f, st.o[db][i + 2] * f, st.o[db][i + 3] * f};
+                f32x4{st.o[db][i], st.o[db][i + 1], st.o[db][i + 2], st.o[db][i + 3]} * f[0] * f[1];
     __syncthreads();
     const int nr = min(QR, S.nq * a.group - r0), items = nr * (HD / 4);
     // four values of row i, relative to its maximum

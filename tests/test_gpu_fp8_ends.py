@@ -1,0 +1,68 @@
+"""Attention over DR_PRECISION_FP8 layers at the ends of what f32 holds: rows so
+small that their scale is the smallest.  Needs an MI355X."""
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import pytest
+
+import dr_attn as dr
+from fp8_reference import attend, bound, check, stored
+from helpers import bf16_round
+
+from test_gpu_fp8_attention import Problem, empty_rows, put_rows, rows_of
+from test_gpu_fp8_far_scales import BF16, SHAPES, visible
+from test_gpu_fp8_wide import wave_rows
+from test_gpu_parity import dev, say, torch  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+
+def run(dev, p, wave, bf16, window=None, prefix=None, split=0, scale=None, more=None):
+    """A call checked row by row against the bound of the keys that it sees (as
+    for scales far apart), `more(i, seen keys)` added to it, and a floor for rows
+    near f32's smallest numbers: up to 8 waves' parts and their sums in up to 3
+    splits, and the splits' sum, are each rounded to 2^-150 at worst, less than
+    64 roundings of a row whose weights add up to 2^-8 or more: 2^-136."""
+    scale = 1 / math.sqrt(p.hd) if scale is None else scale
+    if bf16:
+        p.q = bf16_round(p.q)
+    cache = dr.StepCache(dev.ctx, p.n, [p.hkv], [p.hd], precision=[dr.PRECISION_FP8])
+    cache.store(0, dr.Pass(dev.ctx, range(p.n)), dev.put(p.k), dev.put(p.v))
+    out = empty_rows(dev, p.q.size, bf16)
+    dev.ctx.set_split(split)
+    with wave_rows(dev, wave), rows_of(dev, bf16):
+        try:
+            cache.attention(0, [(put_rows(dev, p.q, bf16), out, dr.Pass(dev.ctx, p.pos))], p.h, sliding_window=window,
+                            causal_prefix=prefix, scale=scale)
+        finally:
+            dev.ctx.set_split(0)
+    got = dev.get(out.float()).reshape(p.q.shape)
+    k, v = stored(p.k), stored(p.v)
+    see = visible(p.n, p.pos, window, prefix)
+    worst = 0.0
+    for i in range(len(p.pos)):
+        ki, vi = k[see[i]], v[see[i]]
+        want, weighted = attend(p.q[i:i + 1], ki, vi, [0], scale)
+        tol = bound(p.q[i:i + 1], ki, np.zeros_like(vi), weighted, want, scale, bf16) + weighted * p.n * 2.0 ** -24
+        tol = tol + 2.0 ** -136 + (0.0 if more is None else more(i, see[i]))
+        worst = max(worst, check(got[i:i + 1], want, tol, f"row {i}"))
+    say(f"  {worst:.3f} of the bound")
+
+
+# ---- rows of the smallest scale
+
+
+@BF16
+@SHAPES
+@pytest.mark.parametrize("size", [1e-34, 1e-35])
+def test_small_outputs(dev, shape, size, bf16):
+    """Nothing but V rows near the smallest numbers."""
+    h, hkv, hd, wave = shape
+    rng = np.random.default_rng(hd + wave + 2)
+    p = Problem(rng, h, hkv, hd, 300, range(240, 300))
+    p.v *= np.float32(size)
+    run(dev, p, wave, bf16)
+    run(dev, p, wave, bf16, window=100, split=3)
