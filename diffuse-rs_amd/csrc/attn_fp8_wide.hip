@@ -228,7 +228,7 @@ void attn_fp8_wide_kernel(const AttnArgs a) {
             const int k0 = x.kb > min(cap, FP8_NAN - 1) ? 0 : x.kb;
             const int kt = wave_max(k0), vt = wave_max(x.vb == FP8_NAN ? 0 : x.vb);
             nan = __any(x.kb == FP8_NAN || x.vb == FP8_NAN);
-            if (kt > kref || __any(scale_far(k0, kref, TK)) || (FAR && kt > 1)) {
+            if (kt > kref || __any(scale_far(k0, kref, TK)) || (FAR && kt > 0)) {
                 kref = kt;
                 kc = __builtin_fmaxf(ldexpf(cq, kref - 127 - 7), FLT_MIN);
             }

@@ -69,10 +69,10 @@ constexpr int TV = PL == 2 ? 12 : 16;
 constexpr int LOW = 16;
 constexpr int TV_RISE = 64;  // a rise of vref that f32 accumulators stand
 
-// Whether a scale byte is one of values (not of a NaN's row or of none) and lies
+// Whether a scale byte is one of values (not of a NaN's row or of zeros) and lies
 // outside far .. 0 below ref.
 __device__ __forceinline__ bool scale_far(int byte, int ref, int far) {
-    return byte > 1 && byte != FP8_NAN && (byte > ref || byte < ref - far);
+    return byte > 0 && byte != FP8_NAN && (byte > ref || byte < ref - far);
 }
 // The factor that widens K's codes of scale `byte` in the band that ends at ref.
 __device__ __forceinline__ float band_scale(int byte, int ref) {
@@ -97,12 +97,12 @@ __device__ __forceinline__ int wave_max(int x) {
     return __builtin_amdgcn_readlane(x, 63);
 }
 // A band of K scales: bytes of values from ref - TK to ref, with NaN rows in the
-// first band of a tile and rows without values in its last.
+// first band of a tile and rows of zeros in its last.
 struct Band {
     int ref;
     bool first, last;
     __device__ __forceinline__ bool holds(int byte) const {
-        return byte == FP8_NAN ? first : byte <= 1 ? last : byte <= ref && byte >= ref - TK;
+        return byte == FP8_NAN ? first : byte == 0 ? last : byte <= ref && byte >= ref - TK;
     }
 };
 // The power of two that brings a row's accumulators, the largest of them `big`, to
@@ -388,7 +388,7 @@ struct Fp8State {
         slow = __builtin_amdgcn_readfirstlane(slow);  // (uniform, and known to be: the masks stay behind a branch)
         const int lane = threadIdx.x & 63, half = lane / QR;
         // ---- scales: within TK of kref and TV of vref, as almost always?  (A NaN's
-        // byte is above, that of a key without values below all others.)
+        // byte is above, that of a row of zeros below all others.)
         int next = 0;
         Band band{};
         bool banded = FAR && cap != FP8_NAN;
@@ -397,7 +397,7 @@ struct Fp8State {
             const int k0 = kb0 > min(cap, FP8_NAN - 1) ? 0 : kb0, k1 = kb1 > min(cap, FP8_NAN - 1) ? 0 : kb1;
             const int kt = wave_max(max(k0, k1)), vt = wave_max(vb == FP8_NAN ? 0 : vb);
             nan = __any(kb0 == FP8_NAN || kb1 == FP8_NAN || vb == FP8_NAN);
-            if (kt > kref || __any(scale_far(k0, kref, TK) || scale_far(k1, kref, TK)) || (FAR && kt > 1)) {
+            if (kt > kref || __any(scale_far(k0, kref, TK) || scale_far(k1, kref, TK)) || (FAR && kt > 0)) {
                 kref = kt;
                 kc = __builtin_fmaxf(ldexpf(cq, kref - 127 - 7), FLT_MIN);
             }

@@ -5,9 +5,9 @@
 // two 2^e and are held as e4m3 codes (x / 2^e to nearest, ties to even).  With
 // a = max |x|: e = floor(log2 a) - 8, one more where a's mantissa exceeds 1.75,
 // so a / 2^e <= 448, the largest e4m3 value, and nothing saturates; e >= -126.
-// The scale byte is e + 127; 0 is a position never stored (codes 0) and
-// FP8_NAN marks a row with a NaN or an infinity, which has no 8 bit form: its
-// codes are 0 and all of it reads back as NaN.
+// The scale byte is e + 127; 0 is a row of zeros, stored or never stored, so that
+// 1 and above always mean values; FP8_NAN marks a row with a NaN or an infinity,
+// which has no 8 bit form: its codes are 0 and all of it reads back as NaN.
 // The block is a single position because a denoise step rewrites single
 // positions: a scale shared by more of them would make each store read and
 // requantise its neighbours, and the contents depend on the order of stores.
@@ -32,11 +32,12 @@ constexpr int FP8_NAN = 255;
 // larger than every number).
 __device__ __forceinline__ int fp8_scale_byte(uint32_t bits) {
     if (bits >= 0x7f800000u) return FP8_NAN;
+    if (bits == 0) return 0;
     const int e = (int)(bits >> 23) - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
     return e < 1 ? 1 : e;
 }
 
-// 2^-e of a scale byte (1..247): x times it is exact but for results far below
+// 2^-e of a scale byte (0..247): x times it is exact but for results far below
 // the smallest code.
 __device__ __forceinline__ float fp8_inverse(int byte) { return __uint_as_float((uint32_t)(254 - byte) << 23); }
 

@@ -57,6 +57,24 @@ def run(dev, p, wave, bf16, window=None, prefix=None, split=0, scale=None, more=
 
 @BF16
 @SHAPES
+def test_keys_of_the_smallest_scale(dev, shape, bf16):
+    """K rows of the smallest scale whose scores a large query makes ordinary, in
+    tiles that they share with larger ones out of sight."""
+    h, hkv, hd, wave = shape
+    rng = np.random.default_rng(hd + wave + 1)
+    p = Problem(rng, h, hkv, hd, 300, range(140, 200))
+    p.q *= np.float32(2.0 ** 119)
+    p.k *= np.float32(2.0 ** -120)
+    assert np.abs(p.k).max() <= 1.75 * 2.0 ** -118
+    run(dev, p, wave, bf16)
+    p.k[:100] *= np.float32(2.0 ** 110)
+    p.k[220:] *= np.float32(2.0 ** 110)
+    run(dev, p, wave, bf16, window=20)
+    run(dev, p, wave, bf16, window=20, split=2)
+
+
+@BF16
+@SHAPES
 @pytest.mark.parametrize("size", [1e-34, 1e-35])
 def test_small_outputs(dev, shape, size, bf16):
     """Nothing but V rows near the smallest numbers."""
