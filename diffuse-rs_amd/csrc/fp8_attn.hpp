@@ -407,11 +407,11 @@ struct Fp8State {
                 band = {kref, cap == FP8_NAN, next == 0};
             } else if (__builtin_expect(__any(scale_far(k0, kref, TK) || scale_far(k1, kref, TK) ||
                                               scale_far(vb, max(vref, vt), TV<PL>)) ||
-                                            (vref > 1 && vt > vref + TV_RISE), 0)) {
+                                            (vref > 0 && vt > vref + TV_RISE), 0)) {
                 bad = true;
             }
-            if (!(FAR && apart) && vt > vref && !(vref > 1 && vt > vref + TV_RISE)) {
-                if (vref > 1) {  // (else o is 0)
+            if (!(FAR && apart) && vt > vref && !(vref > 0 && vt > vref + TV_RISE)) {
+                if (vref > 0) {  // (else o is 0)
                     const float f = pow2_biased(vref - vt + 127);
 #pragma unroll
                     for (int db = 0; db < DB; ++db) o[db] *= f;

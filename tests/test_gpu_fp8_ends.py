@@ -18,6 +18,10 @@ from test_gpu_parity import dev, say, torch  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
+SMALL = pytest.mark.parametrize("size", [1.2e-36, 1e-40])  # (most rows' largest values below 1.75 * 2^-118: the smallest scale)
+NARROW = pytest.mark.parametrize("shape", [(4, 2, 64, 32), (4, 2, 64, 16), (4, 2, 128, 32), (4, 2, 128, 16), (4, 2, 256, 16),
+                                           (4, 2, 512, 16), (6, 3, 80, 32)], ids=str)
+
 
 
 def run(dev, p, wave, bf16, window=None, prefix=None, split=0, scale=None, more=None):
@@ -25,7 +29,9 @@ def run(dev, p, wave, bf16, window=None, prefix=None, split=0, scale=None, more=
     for scales far apart), `more(i, seen keys)` added to it, and a floor for rows
     near f32's smallest numbers: up to 8 waves' parts and their sums in up to 3
     splits, and the splits' sum, are each rounded to 2^-150 at worst, less than
-    64 roundings of a row whose weights add up to 2^-8 or more: 2^-136."""
+    64 roundings of a row whose weights add up to 2^-8 or more: 2^-136.  (bf16's
+    subnormals are 2^-126 / 2^7 = 2^-133 apart, so a row of them is off by half of
+    that where the relative 2^-8 says less.)"""
     scale = 1 / math.sqrt(p.hd) if scale is None else scale
     if bf16:
         p.q = bf16_round(p.q)
@@ -47,12 +53,30 @@ def run(dev, p, wave, bf16, window=None, prefix=None, split=0, scale=None, more=
         ki, vi = k[see[i]], v[see[i]]
         want, weighted = attend(p.q[i:i + 1], ki, vi, [0], scale)
         tol = bound(p.q[i:i + 1], ki, np.zeros_like(vi), weighted, want, scale, bf16) + weighted * p.n * 2.0 ** -24
-        tol = tol + 2.0 ** -136 + (0.0 if more is None else more(i, see[i]))
+        tol = tol + 2.0 ** -136 + (2.0 ** -134 if bf16 else 0.0) + (0.0 if more is None else more(i, see[i]))
         worst = max(worst, check(got[i:i + 1], want, tol, f"row {i}"))
     say(f"  {worst:.3f} of the bound")
 
 
 # ---- rows of the smallest scale
+
+
+@BF16
+@NARROW
+@SMALL
+def test_ordinary_values_after_the_smallest(dev, shape, size, bf16):
+    """V rows of the smallest scale in the first tiles of every wave, ordinary ones
+    after them: queries that see both, and some that see the small ones alone."""
+    h, hkv, hd, wave = shape
+    rng = np.random.default_rng(hd + wave)
+    p = Problem(rng, h, hkv, hd, 600, [200, 210, 255, 300, 330, *range(580, 600)])
+    p.v[:256] *= np.float32(size)
+    assert (np.abs(p.v[:256]).max(-1) <= 1.75 * 2.0 ** -118).mean() > 0.9
+    run(dev, p, wave, bf16)
+    run(dev, p, wave, bf16, prefix=600)
+    run(dev, p, wave, bf16, prefix=600, split=2)
+    p.v = np.ascontiguousarray(p.v[::-1])
+    run(dev, p, wave, bf16, prefix=600, split=3)
 
 
 @BF16
@@ -75,7 +99,7 @@ def test_keys_of_the_smallest_scale(dev, shape, bf16):
 
 @BF16
 @SHAPES
-@pytest.mark.parametrize("size", [1e-34, 1e-35])
+@pytest.mark.parametrize("size", [1e-34, 1e-35, 1.2e-36])
 def test_small_outputs(dev, shape, size, bf16):
     """Nothing but V rows near the smallest numbers."""
     h, hkv, hd, wave = shape
