@@ -237,11 +237,11 @@ void attn_fp8_wide_kernel(const AttnArgs a) {
                 banded = banded || next > 0;
                 band = {kref, cap == FP8_NAN, next == 0};
             } else if (__builtin_expect(__any(scale_far(k0, kref, TK) || scale_far(x.vb, max(vref, vt), TV<PL>)) ||
-                                            (vref > 1 && vt > vref + TV_RISE), 0)) {
+                                            (vref > 0 && vt > vref + TV_RISE), 0)) {
                 bad = true;
             }
-            if (!(FAR && apart) && vt > vref && !(vref > 1 && vt > vref + TV_RISE)) {
-                if (vref > 1) vdown = pow2_biased(vref - vt + 127);
+            if (!(FAR && apart) && vt > vref && !(vref > 0 && vt > vref + TV_RISE)) {
+                if (vref > 0) vdown = pow2_biased(vref - vt + 127);
                 vref = vt;
             }
             if constexpr (FAR) apart = apart || __any(scale_far(x.vb, vref, TV<PL>));

@@ -19,8 +19,6 @@ from test_gpu_parity import dev, say, torch  # noqa: F401
 pytestmark = pytest.mark.gpu
 
 SMALL = pytest.mark.parametrize("size", [1.2e-36, 1e-40])  # (most rows' largest values below 1.75 * 2^-118: the smallest scale)
-NARROW = pytest.mark.parametrize("shape", [(4, 2, 64, 32), (4, 2, 64, 16), (4, 2, 128, 32), (4, 2, 128, 16), (4, 2, 256, 16),
-                                           (4, 2, 512, 16), (6, 3, 80, 32)], ids=str)
 
 
 
@@ -62,7 +60,7 @@ def run(dev, p, wave, bf16, window=None, prefix=None, split=0, scale=None, more=
 
 
 @BF16
-@NARROW
+@SHAPES
 @SMALL
 def test_ordinary_values_after_the_smallest(dev, shape, size, bf16):
     """V rows of the smallest scale in the first tiles of every wave, ordinary ones
