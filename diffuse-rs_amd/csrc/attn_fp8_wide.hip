@@ -122,7 +122,7 @@ void attn_fp8_wide_kernel(const AttnArgs a) {
 
     f32x16 o[DB];
     float m, l;         // row col's maximum; this lane's part of its sum
-    int kref, vref;     // (vref: a row's own once `apart`)
+    int kref, vref, vfirst;  // (as of Fp8State)
     bool apart = false, bad = false;
     float kc;
     auto init = [&]() __attribute__((always_inline)) {
@@ -132,7 +132,7 @@ void attn_fp8_wide_kernel(const AttnArgs a) {
             for (int i = 0; i < 16; ++i) o[db][i] = 0.0f;
         m = -INFINITY;
         l = 0.0f;
-        kref = vref = 0;
+        kref = vref = vfirst = 0;
         kc = FLT_MIN;
     };
     init();
@@ -232,16 +232,20 @@ void attn_fp8_wide_kernel(const AttnArgs a) {
                 kref = kt;
                 kc = __builtin_fmaxf(ldexpf(cq, kref - 127 - 7), FLT_MIN);
             }
+            const bool steep = vfirst > 0 && vt > vfirst + TV_RISE;
             if constexpr (FAR) {
                 next = wave_max(scale_far(k0, kref, TK) ? k0 : 0);
                 banded = banded || next > 0;
                 band = {kref, cap == FP8_NAN, next == 0};
             } else if (__builtin_expect(__any(scale_far(k0, kref, TK) || scale_far(x.vb, max(vref, vt), TV<PL>)) ||
-                                            (vref > 0 && vt > vref + TV_RISE), 0)) {
+                                            steep, 0)) {
                 bad = true;
             }
-            if (!(FAR && apart) && vt > vref && !(vref > 0 && vt > vref + TV_RISE)) {
-                if (vref > 0) vdown = pow2_biased(vref - vt + 127);
+            if (!(FAR && apart) && vt > vref && !steep) {
+                if (vref > 0)
+                    vdown = pow2_biased(vref - vt + 127);
+                else
+                    vfirst = vt;
                 vref = vt;
             }
             if constexpr (FAR) apart = apart || __any(scale_far(x.vb, vref, TV<PL>));

@@ -67,7 +67,9 @@ constexpr int TV = PL == 2 ? 12 : 16;
 // Rows meet at 2^-LOW of themselves: sums of weights that start at 2^P0 would take
 // values above 1e33 out of f32 before the division by the weights' sum.
 constexpr int LOW = 16;
-constexpr int TV_RISE = 64;  // a rise of vref that f32 accumulators stand
+// How far vref may rise in all: the sums of a row that sees only the first tiles
+// sink by as much (2^8 at least at first, f32 holds them whole to 2^-102).
+constexpr int TV_RISE = 64;
 
 // Whether a scale byte is one of values (not of a NaN's row or of zeros) and lies
 // outside far .. 0 below ref.
@@ -346,7 +348,7 @@ struct Fp8State {
 
     Acc o[DB];
     float m, l, kc;
-    int kref, vref;  // (vref: a row's own once `apart`)
+    int kref, vref, vfirst;  // (vref: a row's own once `apart`; vfirst: where it rose from 0 to)
     bool apart, bad;  // (bad: scales too far apart without FAR, the state is worth nothing)
     float cq;  // |c| / the row's power of two
 
@@ -358,7 +360,7 @@ struct Fp8State {
         m = -INFINITY;
         l = 0.0f;
         kc = FLT_MIN;  // (before any stored key; never 0, a hidden score of -infinity has to stay one)
-        kref = vref = 0;
+        kref = vref = vfirst = 0;
         apart = bad = false;
         cq = cq_;
     }
@@ -401,20 +403,22 @@ struct Fp8State {
                 kref = kt;
                 kc = __builtin_fmaxf(ldexpf(cq, kref - 127 - 7), FLT_MIN);
             }
+            const bool steep = vfirst > 0 && vt > vfirst + TV_RISE;
             if constexpr (FAR) {
                 next = wave_max(max(scale_far(k0, kref, TK) ? k0 : 0, scale_far(k1, kref, TK) ? k1 : 0));
                 banded = banded || next > 0;
                 band = {kref, cap == FP8_NAN, next == 0};
             } else if (__builtin_expect(__any(scale_far(k0, kref, TK) || scale_far(k1, kref, TK) ||
-                                              scale_far(vb, max(vref, vt), TV<PL>)) ||
-                                            (vref > 0 && vt > vref + TV_RISE), 0)) {
+                                              scale_far(vb, max(vref, vt), TV<PL>)) || steep, 0)) {
                 bad = true;
             }
-            if (!(FAR && apart) && vt > vref && !(vref > 0 && vt > vref + TV_RISE)) {
-                if (vref > 0) {  // (else o is 0)
+            if (!(FAR && apart) && vt > vref && !steep) {
+                if (vref > 0) {
                     const float f = pow2_biased(vref - vt + 127);
 #pragma unroll
                     for (int db = 0; db < DB; ++db) o[db] *= f;
+                } else {  // (o is 0)
+                    vfirst = vt;
                 }
                 vref = vt;
             }

@@ -1,5 +1,6 @@
 """Attention over DR_PRECISION_FP8 layers at the ends of what f32 holds: rows so
-small that their scale is the smallest.  Needs an MI355X."""
+small that their scale is the smallest, sizes that grow from tile to tile.  Needs
+an MI355X."""
 from __future__ import annotations
 
 import math
@@ -106,3 +107,20 @@ def test_small_outputs(dev, shape, size, bf16):
     p.v *= np.float32(size)
     run(dev, p, wave, bf16)
     run(dev, p, wave, bf16, window=100, split=3)
+
+
+# ---- sizes that grow
+
+
+@BF16
+@SHAPES
+def test_values_that_grow_in_steps(dev, shape, bf16):
+    """V rows that grow 2^60 at a time, each step within what the accumulators
+    stand: a query that sees the first of them alone keeps its bits beside one
+    that sees them all."""
+    h, hkv, hd, wave = shape
+    rng = np.random.default_rng(hd + wave + 3)
+    p = Problem(rng, h, hkv, hd, 1024, [10, 100, 255, 256, 500, 511, 700, 1023])
+    p.v *= np.exp2(-100.0 + 60 * (np.arange(1024) // 256)).astype(np.float32)[:, None, None]
+    run(dev, p, wave, bf16, prefix=1024)
+    run(dev, p, wave, bf16, prefix=1024, split=1)
