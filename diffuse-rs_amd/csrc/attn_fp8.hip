@@ -52,8 +52,8 @@ void attn_fp8_kernel(const AttnArgs a) {
     using T = Fp8State<HD, QR, PL>;
     extern __shared__ __align__(16) char lds[];
     _Float16* const sq = reinterpret_cast<_Float16*>(lds);  // [PL][QR][QP]
-    float* const srow = reinterpret_cast<float*>(lds + G::BODY);
-    float* const sm = srow + QR;
+    int* const srow = reinterpret_cast<int*>(lds + G::BODY);
+    float* const sm = reinterpret_cast<float*>(srow + QR);
     float* const sl = sm + NW * QR;
     float* const sr = sl + NW * QR;
     _Float16* const svs = reinterpret_cast<_Float16*>(sr + 2 * QR);  // [NW][32]
@@ -152,7 +152,7 @@ void attn_fp8_kernel(const AttnArgs a) {
 
     T st;
     auto walk = [&](auto far) __attribute__((always_inline)) {
-        st.init(fabsf(a.c) * srow[col]);
+        st.init(a.c, srow[col]);
         for (int t = t_first, cap = FP8_NAN; t < t1;) {
             int then = t;
             const int next = st.template tile<decltype(far)::value>(

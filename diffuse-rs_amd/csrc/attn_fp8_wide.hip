@@ -50,8 +50,8 @@ void attn_fp8_wide_kernel(const AttnArgs a) {
     extern __shared__ __align__(16) char lds[];
     char* const part = lds;
     char* const pbuf = lds + 2 * G::PART;
-    float* const srow = reinterpret_cast<float*>(lds + G::BODY);  // [ROWS]
-    float* const smax = srow + G::ROWS;                           // [NW][32]
+    int* const srow = reinterpret_cast<int*>(lds + G::BODY);          // [ROWS]
+    float* const smax = reinterpret_cast<float*>(srow + G::ROWS);  // [NW][32]
     float* const ssum = smax + NW * 32;                           // [NW][32]
     int* const sflag = reinterpret_cast<int*>(ssum + NW * 32);    // [2]
     int* const stick = sflag + 4;
@@ -117,7 +117,7 @@ void attn_fp8_wide_kernel(const AttnArgs a) {
             q[p][s] = *reinterpret_cast<const f16x8*>(reinterpret_cast<_Float16*>(lds) +
                                                       ((size_t)p * G::ROWS + rb * 32 + col) * G::QP + d);
         }
-    const float cq = fabsf(a.c) * srow[32 * rb + col];
+    const int eq = srow[32 * rb + col];
     __syncthreads();  // (the partial scores lie over the query rows)
 
     f32x16 o[DB];
@@ -230,7 +230,7 @@ void attn_fp8_wide_kernel(const AttnArgs a) {
             nan = __any(x.kb == FP8_NAN || x.vb == FP8_NAN);
             if (kt > kref || __any(scale_far(k0, kref, TK)) || (FAR && kt > 0)) {
                 kref = kt;
-                kc = __builtin_fmaxf(ldexpf(cq, kref - 127 - 7), FLT_MIN);
+                kc = __builtin_fmaxf(ldexpf(fabsf(a.c), eq + kref - 127 - 7), FLT_MIN);
             }
             const bool steep = vfirst > 0 && vt > vfirst + TV_RISE;
             if constexpr (FAR) {

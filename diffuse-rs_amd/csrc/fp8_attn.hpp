@@ -246,9 +246,10 @@ __device__ __forceinline__ void load_query(const AttnArgs& a, const AttnSlot& S,
 }
 
 // The power of two that brings a row's largest magnitude to 2^14..2^15 (up, with
-// the sign of c), and its inverse; a row with a NaN or an infinity becomes NaN.
+// the sign of c; 2^127 at most), and its inverse's exponent (the inverse itself may
+// be subnormal); a row with a NaN or an infinity becomes NaN.
 template <int LPR>
-__device__ __forceinline__ void query_scale(const AttnArgs& a, const f32x4 (&y)[4], float& up, float& down) {
+__device__ __forceinline__ void query_scale(const AttnArgs& a, const f32x4 (&y)[4], float& up, int& down) {
     uint32_t top = 0;
 #pragma unroll
     for (int e = 0; e < 16; ++e) top = max(top, __float_as_uint(y[e / 4][e % 4]) & 0x7fffffffu);
@@ -258,7 +259,7 @@ __device__ __forceinline__ void query_scale(const AttnArgs& a, const f32x4 (&y)[
     const int ex = min(268 - (int)(top >> 23), 254);
     up = bad ? __uint_as_float(0x7fc00000u) : pow2_biased(ex);
     if (a.c < 0.0f) up = -up;
-    down = pow2_biased(bad ? 127 : 254 - ex);
+    down = bad ? 0 : 127 - ex;
 }
 
 // Values 8 h .. 8 h + 7 of a run, scaled, as f16 planes.
@@ -311,14 +312,15 @@ struct Fp8Queries {
             load_query<HD>(a, S, qi, g * a.group + r - qi * a.group, (int)threadIdx.x % LPR * 16, y[p]);
         }
     }
-    // scaled by a power of two each (inverse to srow), split into PL planes of f16
-    // in sq [PL][QR][QP]
-    __device__ __forceinline__ void stage(const AttnArgs& a, _Float16* sq, float* srow) const {
+    // scaled by a power of two each (its inverse's exponent to srow), split into PL
+    // planes of f16 in sq [PL][QR][QP]
+    __device__ __forceinline__ void stage(const AttnArgs& a, _Float16* sq, int* srow) const {
         const int tid = threadIdx.x, d0 = tid % LPR * 16;
 #pragma unroll
         for (int p = 0; p < PASSES; ++p) {
             const int i = p * PER + tid / LPR;
-            float up, down;
+            float up;
+            int down;
             query_scale<LPR>(a, y[p], up, down);
             if (i < QR) {
                 if (tid % LPR == 0) srow[i] = down;
@@ -350,9 +352,10 @@ struct Fp8State {
     float m, l, kc;
     int kref, vref, vfirst;  // (vref: a row's own once `apart`; vfirst: where it rose from 0 to)
     bool apart, bad;  // (bad: scales too far apart without FAR, the state is worth nothing)
-    float cq;  // |c| / the row's power of two
+    float c;  // |c|, and the exponent of the inverse of the row's power of two
+    int eq;
 
-    __device__ __forceinline__ void init(float cq_) {
+    __device__ __forceinline__ void init(float c_, int eq_) {
 #pragma unroll
         for (int db = 0; db < DB; ++db)
 #pragma unroll
@@ -362,7 +365,8 @@ struct Fp8State {
         kc = FLT_MIN;  // (before any stored key; never 0, a hidden score of -infinity has to stay one)
         kref = vref = vfirst = 0;
         apart = bad = false;
-        cq = cq_;
+        c = fabsf(c_);
+        eq = eq_;
     }
 
     // o times 2^e, |e| <= 252, in two steps
@@ -401,7 +405,7 @@ struct Fp8State {
             nan = __any(kb0 == FP8_NAN || kb1 == FP8_NAN || vb == FP8_NAN);
             if (kt > kref || __any(scale_far(k0, kref, TK) || scale_far(k1, kref, TK)) || (FAR && kt > 0)) {
                 kref = kt;
-                kc = __builtin_fmaxf(ldexpf(cq, kref - 127 - 7), FLT_MIN);
+                kc = __builtin_fmaxf(ldexpf(c, eq + kref - 127 - 7), FLT_MIN);
             }
             const bool steep = vfirst > 0 && vt > vfirst + TV_RISE;
             if constexpr (FAR) {

@@ -1,6 +1,6 @@
 """Attention over DR_PRECISION_FP8 layers at the ends of what f32 holds: rows so
-small that their scale is the smallest, sizes that grow from tile to tile.  Needs
-an MI355X."""
+small that their scale is the smallest, sizes that grow from tile to tile, query
+rows near f32's smallest numbers.  Needs an MI355X."""
 from __future__ import annotations
 
 import math
@@ -124,3 +124,22 @@ def test_values_that_grow_in_steps(dev, shape, bf16):
     p.v *= np.exp2(-100.0 + 60 * (np.arange(1024) // 256)).astype(np.float32)[:, None, None]
     run(dev, p, wave, bf16, prefix=1024)
     run(dev, p, wave, bf16, prefix=1024, split=1)
+
+
+# ---- small queries
+
+
+@BF16
+@SHAPES
+@pytest.mark.parametrize("e", [105, 113, 120])
+def test_small_queries_of_large_keys(dev, shape, e, bf16):
+    """Query rows around 2^-e, K rows around 2^e, and the other way round."""
+    h, hkv, hd, wave = shape
+    rng = np.random.default_rng(hd + wave + e)
+    p = Problem(rng, h, hkv, hd, 200, range(150, 200))
+    q, k = p.q, p.k
+    p.q, p.k = q * np.float32(2.0 ** -e), k * np.float32(2.0 ** e)
+    run(dev, p, wave, bf16)
+    run(dev, p, wave, bf16, window=60, split=2)
+    p.q, p.k = q * np.float32(2.0 ** e), k * np.float32(2.0 ** -e)
+    run(dev, p, wave, bf16)
