@@ -20,8 +20,10 @@
 //   scales 2^TK below it; 2^kref goes into the factor of the scores.
 // - V's scale multiplies the planes of p, relative to the largest V scale met
 //   so far (vref; the accumulators are rescaled when it rises): powers of two in
-//   f16, down to 2^-TV, where the planes still hold 21 bits (one plane: 11);
-//   2^vref is applied once at the end.
+//   f16, down to 2^-TV; 2^vref is applied once at the end.  The planes end at
+//   2^-24, so a weight so scaled is off by 2^-24 (one plane: 2^-25) at most, where
+//   the row's largest is 2^P0 or more: by 2^-22 (2^-19) of that largest beside a
+//   V row 2^TV larger, seen or not, and by 2^-34 (2^-35) among rows of one scale.
 // - Scales further apart than that, which a cache need not have but may (a row of
 //   1e30 must not cost queries that do not see it their bits), take a slower way
 //   (FAR), on which a wave that has met them starts again; the common loop only
@@ -32,7 +34,11 @@
 //   others (`apart`, from the first V tile that needs it).
 // - m moves only when a score exceeds it by more than 2^MOVE, so p <= 2^(P0 +
 //   MOVE) = 2^15 with p = exp2(s - m + P0), inside f16's range, and the
-//   O rescale is skipped on almost every tile; out does not depend on m.
+//   O rescale is skipped on almost every tile; out does not depend on m.  A
+//   larger P0 keeps more of light weights, a smaller MOVE rescales more often:
+//   P0 8 / 10 / 11 / 12, 256 bf16 rows x 16/8 heads of 256 in a window of 1024
+//   17.4 / 18.1 / 18.2 / 18.5 us, 256 f32 rows x 16/2 heads of 512 over 4352 keys
+//   94 / 95 / 92 / 99, 256 f32 rows x 32 heads of 128 over 768 13.5 / 13.6 / 13.6 / 13.8.
 //
 // S^T = K Q^T and O^T = V^T P^T: a lane owns one query column of both, so the
 // softmax statistics are per lane, and with the keys of a tile assigned to A
@@ -60,15 +66,15 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
-constexpr float P0 = 8.0f, MOVE = 7.0f;
+constexpr float P0 = 10.0f, MOVE = 5.0f;
 constexpr int TK = 22;
 template <int PL>
 constexpr int TV = PL == 2 ? 12 : 16;
 // Rows meet at 2^-LOW of themselves: sums of weights that start at 2^P0 would take
 // values above 1e33 out of f32 before the division by the weights' sum.
-constexpr int LOW = 16;
+constexpr int LOW = 18;
 // How far vref may rise in all: the sums of a row that sees only the first tiles
-// sink by as much (2^8 at least at first, f32 holds them whole to 2^-102).
+// sink by as much (2^P0 or more at first; f32 holds them whole down to 2^-102).
 constexpr int TV_RISE = 64;
 
 // Whether a scale byte is one of values (not of a NaN's row or of zeros) and lies

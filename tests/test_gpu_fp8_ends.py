@@ -1,6 +1,7 @@
 """Attention over DR_PRECISION_FP8 layers at the ends of what f32 holds: rows so
 small that their scale is the smallest, sizes that grow from tile to tile, query
-rows near f32's smallest numbers.  Needs an MI355X."""
+rows near f32's smallest numbers, and rows out of sight that are larger than
+those in sight by less than what takes the slow way.  Needs an MI355X."""
 from __future__ import annotations
 
 import math
@@ -143,3 +144,39 @@ def test_small_queries_of_large_keys(dev, shape, e, bf16):
     run(dev, p, wave, bf16, window=60, split=2)
     p.q, p.k = q * np.float32(2.0 ** e), k * np.float32(2.0 ** -e)
     run(dev, p, wave, bf16)
+
+
+# ---- larger rows out of sight
+
+
+@BF16
+@SHAPES
+def test_light_keys_beside_a_larger_row_out_of_sight(dev, shape, bf16):
+    """One key takes almost all of a row's weight, the others, alike, about 2^-12
+    of it; dims in which the heavy key's value is 0 are theirs alone.  In their
+    tile lies a V row that no query sees, 2^12 times as large (bf16 rows 2^16).
+
+    A weight times its scale, relative to the largest scale met, is rounded to
+    f16 planes whose last bit is 2^-24: off by 2^-24 (two planes) or 2^-25, in
+    units in which the row's largest weight is 2^10 at least.  So a key adds at
+    most 2^-34 (2^-35) of its value times the ratio of the scales, over the sum
+    of weights relative to the largest."""
+    h, hkv, hd, wave = shape
+    rng = np.random.default_rng(hd + wave + 4)
+    p = Problem(rng, h, hkv, hd, 32, range(12, 31))
+    ratio = 16 if bf16 else 12
+    p.v = rng.uniform(-1, 1, p.v.shape).astype(np.float32)
+    p.v[..., hd // 2] = 1.75  # (every row's largest: one scale)
+    p.v[0, :, :hd // 2] = 0
+    p.v[31] *= np.float32(2.0 ** ratio)
+    p.k[:] = 0
+    p.k[:, :, 1] = 1
+    p.k[0, :, 0] = 8  # (a code, so that its score is known)
+    p.q[:] = 0
+    p.q[..., 0] = rng.uniform(0.9, 1.1, p.q.shape[:2]) * 12 * math.log(2) * math.sqrt(hd) / 8
+
+    def more(i, seen):
+        v = np.repeat(np.abs(stored(p.v)[seen]).sum(0), h // hkv, axis=0)[None]
+        return v * 2.0 ** (ratio - (35 if bf16 else 34))
+
+    run(dev, p, wave, bf16, prefix=32, more=more)
