@@ -694,24 +694,33 @@ int dr_cache_set_precision(dr_step_cache* cache, size_t layer, int precision) {
     if (!precision_ok(precision))
         return fail(DR_ERR_INVALID, "dr_cache_set_precision: precision %d is not DR_PRECISION_BF16 (0), "
                     "DR_PRECISION_HILO (1) or DR_PRECISION_FP8 (2)", precision);
-    DR_CHECK(use_device(cache->ctx));
-    // (zero: rows stored before this call carry no lo half, and none of them
-    // passes between the 8 bit planes and the others)
-    DR_CHECK(add_planes(cache, layer, precision, "cache plane allocation"));
     const std::vector<Plane> keep = planes_of(cache, layer, precision);
-    bool waited = false;
+    std::vector<Plane> drop;
     for (int other : {DR_PRECISION_HILO, DR_PRECISION_FP8})
         for (const Plane& pl : planes_of(cache, layer, other)) {
             bool kept = false;
             for (const Plane& k : keep) kept = kept || (k.p16 == pl.p16 && k.p8 == pl.p8);
-            if (kept) continue;
-            for (size_t i = layer * cache->n_batch; i < (layer + 1) * cache->n_batch; ++i) {
-                if (!pl.get(i)) continue;
-                if (!waited) (void)hipStreamSynchronize(cache->ctx->stream);
-                waited = true;
-                (void)hipFree(pl.get(i));
-                pl.set(i, nullptr);
-            }
+            if (!kept) drop.push_back(pl);
+        }
+    const size_t first = layer * cache->n_batch, last = first + cache->n_batch;
+    bool same = true;
+    for (size_t i = first; i < last; ++i) {
+        for (const Plane& pl : keep) same = same && pl.get(i);
+        for (const Plane& pl : drop) same = same && !pl.get(i);
+    }
+    if (same) return DR_OK;  // (nothing asked of the device: a stream may be under capture)
+    DR_CHECK(use_device(cache->ctx));
+    // (zero: rows stored before this call carry no lo half, and none of them
+    // passes between the 8 bit planes and the others)
+    DR_CHECK(add_planes(cache, layer, precision, "cache plane allocation"));
+    bool waited = false;
+    for (const Plane& pl : drop)
+        for (size_t i = first; i < last; ++i) {
+            if (!pl.get(i)) continue;
+            if (!waited) (void)hipStreamSynchronize(cache->ctx->stream);
+            waited = true;
+            (void)hipFree(pl.get(i));
+            pl.set(i, nullptr);
         }
     return DR_OK;
 }
