@@ -709,6 +709,9 @@ int dr_cache_set_precision(dr_step_cache* cache, size_t layer, int precision) {
         for (const Plane& pl : drop) same = same && !pl.get(i);
     }
     if (same) return DR_OK;  // (nothing asked of the device: a stream may be under capture)
+    if (capturing(cache->ctx->stream) || capturing(cache->ctx->own))
+        return fail(DR_ERR_INVALID, "dr_cache_set_precision: the context's stream is under graph capture (a graph "
+                    "would keep planes that this call frees)");
     DR_CHECK(use_device(cache->ctx));
     // (zero: rows stored before this call carry no lo half, and none of them
     // passes between the 8 bit planes and the others)

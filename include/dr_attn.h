@@ -196,7 +196,9 @@ void dr_cache_destroy(dr_step_cache* cache);
  * dr_ctx_set_o_dtype) with 11 bit weights, at any head dim.  The scale limit of
  * bf16 layers applies (dr_cache_create_layers).  Changing a layer to or from
  * DR_PRECISION_FP8 drops the rows it holds (they read as zeros) and frees its
- * planes: a captured hipGraph that uses the layer must not be replayed after. */
+ * planes: a captured hipGraph that uses the layer must not be replayed after,
+ * and while the context's stream is being captured a change is refused
+ * (DR_ERR_INVALID). */
 #define DR_PRECISION_FP8 2
 int dr_cache_set_precision(dr_step_cache* cache, size_t layer, int precision);
 /* dr_cache_create with each layer's score precision given up front

@@ -1,5 +1,6 @@
 """dr_cache_set_precision while a stream is captured into a graph: a call that
-changes nothing does nothing.  Needs an MI355X."""
+changes nothing does nothing, one that would make or free planes is refused and
+leaves the capture and the layer as they were.  Needs an MI355X."""
 from __future__ import annotations
 
 import math
@@ -8,7 +9,6 @@ import numpy as np
 import pytest
 
 import dr_attn as dr
-from fp8_reference import attend, bound, check, stored
 
 from test_gpu_parity import say, torch  # noqa: F401
 
@@ -58,3 +58,17 @@ def ctx_stream(request, torch):
 @pytest.mark.parametrize("kind", KINDS)
 def test_the_same_precision_again(torch, ctx_stream, kind):
     captured_step(torch, *ctx_stream, kind, lambda cache: cache.set_precision(0, kind))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_a_change_under_capture_is_refused(torch, ctx_stream, kind):
+    def change(cache):
+        for other in KINDS:
+            if other != kind:
+                with pytest.raises(dr.DrError) as e:
+                    cache.set_precision(0, other)
+                assert e.value.status == dr.DR_ERR_INVALID and "capture" in str(e.value)
+
+    cache = captured_step(torch, *ctx_stream, kind, change)
+    for other in KINDS:
+        cache.set_precision(0, other)  # (free to change once no stream is captured)
