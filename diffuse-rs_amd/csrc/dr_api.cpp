@@ -890,6 +890,7 @@ static int store_rows(dr_step_cache* cache, size_t layer, size_t batch, const dr
         a.kc = reinterpret_cast<uint16_t*>(cache->k8[at]);
         a.vtc = reinterpret_cast<uint16_t*>(cache->v8[at]);
         a.sc = cache->sc[at];
+        a.n_cu = cache->ctx->n_cu;
     }
     hipError_t e = a.sc ? dr::launch_store_fp8(cache->hd_tile[layer], a, cache->ctx->stream)
                         : dr::launch_store(cache->hd_tile[layer], a, cache->ctx->stream);
@@ -918,6 +919,7 @@ static int gather_rows(dr_step_cache* cache, size_t layer, size_t batch, const i
         a.kc = reinterpret_cast<const uint16_t*>(cache->k8[at]);
         a.vtc = reinterpret_cast<const uint16_t*>(cache->v8[at]);
         a.sc = cache->sc[at];
+        a.n_cu = cache->ctx->n_cu;
     }
     hipError_t e = a.sc ? dr::launch_gather_fp8(cache->hd_tile[layer], a, cache->ctx->stream)
                         : dr::launch_gather(cache->hd_tile[layer], a, cache->ctx->stream);

@@ -117,6 +117,7 @@ struct StoreArgs {
     int rot;             // rotated dims per head
     int pos0;            // >= 0: pos[r] == pos0 + r (contiguous rows), read without a load
     uint8_t* sc;         // launch_store_fp8: scale bytes, kc and vtc being code planes (fp8_common.hpp)
+    int n_cu;            // the same: compute units of the device
 };
 
 struct GatherArgs {
@@ -133,6 +134,7 @@ struct GatherArgs {
     float* out_v;
     const uint8_t* sc;   // launch_gather_fp8: scale bytes, kc and vtc being code planes (fp8_common.hpp)
     int pos0;            // the same: >= 0: pos[r] == pos0 + r, read without a load
+    int n_cu;            // the same: compute units of the device
 };
 
 // The Q/K/V epilogue of attention_block (forward.rs:291-310), in place on

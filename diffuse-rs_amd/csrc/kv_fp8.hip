@@ -349,8 +349,8 @@ int fp8_blocks(int n, int pos0, int per) {
 // rows no cache level holds reads past them (32768 rows x 8 heads of 128, 268 MB:
 // 71 -> 64 us; where L2 or the memory-side cache may still hold them, 256 x 32
 // heads: 4.6 -> 5.5, 8192 x 8: 17.8 -> 19.3).
-Fp8Way pick_way(int n, int pos0, int n_head_kv, int hd) {
-    if (pos0 < 0 || (long)fp8_blocks(n, pos0, 32) * n_head_kv * 2 < 256) return BY_ROWS;
+Fp8Way pick_way(int n, int pos0, int n_head_kv, int hd, int n_cu) {
+    if (pos0 < 0 || (long)fp8_blocks(n, pos0, 32) * n_head_kv * 2 < n_cu) return BY_ROWS;
     return (long)n * n_head_kv * hd >= 16L << 20 ? BY_TILES_STREAM : BY_TILES;
 }
 
@@ -367,7 +367,7 @@ hipError_t store(const StoreArgs& a, hipStream_t st) {
 
 template <int HD>
 hipError_t store(const StoreArgs& a, hipStream_t st) {
-    switch (pick_way(a.n, a.pos0, a.n_head_kv, a.hd)) {
+    switch (pick_way(a.n, a.pos0, a.n_head_kv, a.hd, a.n_cu)) {
         case BY_ROWS: return store<HD, BY_ROWS>(a, st);
         case BY_TILES_STREAM: return store<HD, BY_TILES_STREAM>(a, st);
         default: return store<HD, BY_TILES>(a, st);
@@ -398,7 +398,7 @@ hipError_t launch_store_fp8(int hd_tile, const StoreArgs& a, hipStream_t st) {
 hipError_t launch_gather_fp8(int hd_tile, const GatherArgs& a, hipStream_t st) {
     if (a.n <= 0) return hipSuccess;
     if (!a.sc || (a.pos0 < 0 && !a.pos)) return hipErrorInvalidValue;
-    const bool rows = pick_way(a.n, a.pos0, a.n_head_kv, a.hd) == BY_ROWS;
+    const bool rows = pick_way(a.n, a.pos0, a.n_head_kv, a.hd, a.n_cu) == BY_ROWS;
     switch (hd_tile) {
         case 64: return rows ? gather<64, true>(a, st) : gather<64, false>(a, st);
         case 128: return rows ? gather<128, true>(a, st) : gather<128, false>(a, st);
