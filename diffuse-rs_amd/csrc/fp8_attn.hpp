@@ -253,7 +253,8 @@ __device__ __forceinline__ void load_query(const AttnArgs& a, const AttnSlot& S,
 
 // The power of two that brings a row's largest magnitude to 2^14..2^15 (up, with
 // the sign of c; 2^127 at most), and its inverse's exponent (the inverse itself may
-// be subnormal); a row with a NaN or an infinity becomes NaN.
+// be subnormal); a row with a NaN or an infinity becomes NaN, and so does every row
+// under a scale that is NaN.
 template <int LPR>
 __device__ __forceinline__ void query_scale(const AttnArgs& a, const f32x4 (&y)[4], float& up, int& down) {
     uint32_t top = 0;
@@ -261,7 +262,7 @@ __device__ __forceinline__ void query_scale(const AttnArgs& a, const f32x4 (&y)[
     for (int e = 0; e < 16; ++e) top = max(top, __float_as_uint(y[e / 4][e % 4]) & 0x7fffffffu);
 #pragma unroll
     for (int o = LPR / 2; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o));
-    const bool bad = top >= 0x7f800000u;
+    const bool bad = top >= 0x7f800000u || a.c != a.c;
     const int ex = min(268 - (int)(top >> 23), 254);
     up = bad ? __uint_as_float(0x7fc00000u) : pow2_biased(ex);
     if (a.c < 0.0f) up = -up;

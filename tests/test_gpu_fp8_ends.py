@@ -1,7 +1,8 @@
 """Attention over DR_PRECISION_FP8 layers at the ends of what f32 holds: rows so
 small that their scale is the smallest, sizes that grow from tile to tile, query
-rows near f32's smallest numbers, and rows out of sight that are larger than
-those in sight by less than what takes the slow way.  Needs an MI355X."""
+rows near f32's smallest numbers, rows out of sight that are larger than those
+in sight by less than what takes the slow way, a scale that is no number.  Needs
+an MI355X."""
 from __future__ import annotations
 
 import math
@@ -180,3 +181,17 @@ def test_light_keys_beside_a_larger_row_out_of_sight(dev, shape, bf16):
         return v * 2.0 ** (ratio - (35 if bf16 else 34))
 
     run(dev, p, wave, bf16, prefix=32, more=more)
+
+
+# ---- a scale that is no number
+
+
+@BF16
+@SHAPES
+def test_nan_scale(dev, shape, bf16):
+    """Scores that are NaN: every row is, as on the other layers."""
+    h, hkv, hd, wave = shape
+    rng = np.random.default_rng(hd + wave + 5)
+    p = Problem(rng, h, hkv, hd, 70, range(40, 70))
+    run(dev, p, wave, bf16, scale=math.nan)
+    run(dev, p, wave, bf16, window=20, split=2, scale=math.nan)
