@@ -15,10 +15,12 @@
 // 32/8 heads of 128, 131072 keys: 268 MB in 53 us, 5.0 TB/s, where a copy reaches
 // 5.2).  Few tiles: latencies in a row, arguments 1 us, query rows 1, first tiles
 // 2-4, the waves' meeting 2 (256 f32 rows, 32 heads, 768 keys: 12-13 us, of which
-// 5.5 are the products' and 4 the bytes').  Many tiles: the vector units, 226
+// 5.5 are the products' and 4 the bytes').  Many tiles: the vector units, 233
 // instructions a tile and wave at 4.3-6.6 clk beside 16 or 32 MFMAs of 32 (4096
 // bf16 rows, 32 heads, causal: 138 GFLOP in 200 us, 690 TFLOP/s; counters: vector
-// units 57-62 %, matrix cores 30 % of the time, which nearly add up).  Tried
+// units 61 %, matrix cores 29 % of the time, which nearly add up).  f32 rows at
+// head dim 256 spill 23 registers (256 rows, 16/8 heads, window 1024: 19.2 us,
+// bf16 rows 17.5).  Tried
 // there without gain: three waves a SIMD (199 against 200 us), 64 rows a wave so
 // that codes are widened once for two blocks (265, registers), tiles shared
 // through LDS (255-290), waves on different rows (215-222).
@@ -229,9 +231,12 @@ hipError_t launch_hd(const LaunchPlan& p, const AttnArgs& a, hipStream_t st) {
 // the wide kernel: it starts slower (24 us against 8 of fixed time) but a 32-key
 // tile costs it 1.6 us for 64 rows, where four waves take 2.6 us for four tiles of
 // 16 rows.  Measured, 16-row / wide, f32 rows over 2 KV heads of 512 dims, group 8:
-// 256 rows over 600 keys 27 / 36 us, over 4352 101 / 91, over 32768 680 / 531;
-// 600 rows over 600 keys 69 / 48, over 4352 277 / 243.  (Few row blocks would be
-// split often, and 64 rows are dear to join: 32 rows over 32768 keys 117 / 147.)
+// 256 rows (256 blocks) over 600 keys 25 / 38 us, 1800 49 / 54, 2800 68.5 / 69.2,
+// 3200 75.5 / 74.8, 3800 88.8 / 83.6, 4352 98.6 / 92.3, 32768 680 / 531; 600 rows
+// over 600 keys 69 / 48, over 4352 277 / 243.  So a block for each CU breaks even
+// near 95 tiles; 120 keeps the 16-row kernel up to 6 % too long there.  (Few row
+// blocks would be split often, and 64 rows are dear to join: 32 rows over 32768
+// keys 117 / 147.)
 //
 // Waves: 8 where a workgroup per CU is all there is, else 4, two workgroups per CU.
 // 8 / 4 waves: 256 f32 rows x 32 heads of 128 over 768 keys (256 workgroups) 13.8 /
@@ -241,8 +246,12 @@ hipError_t launch_hd(const LaunchPlan& p, const AttnArgs& a, hipStream_t st) {
 // Key splits.  A step of a workgroup (one tile of each wave, or of the wide kernel)
 // takes `step` us, a split's join reads its rows of floats at 13000 a us, and a join
 // at all about 2 us: so steps / n * step + n * floats / 13000 is smallest at n =
-// sqrt(steps * step * 13000 / floats).  More workgroups than CUs only wait for each
-// other (16 rows x 8 heads of 256 dims over 32768 keys: 16 splits 38 us, 32 61).
+// sqrt(steps * step * 13000 / floats).  More workgroups than CUs mostly wait for
+// each other: 16 rows x 8 heads of 256 dims over 32768 keys (8 row blocks), 16 splits
+// 38 us, 32 61; 1 / 2 / 3 splits of 160 row blocks, 160 rows x 32 heads of 128 over
+// 4096 keys 30.7 / 42.6 / 35.8, 300 x 16 heads over 2553 22.7 / 34.5 / 28.4; of 200 at
+// head dim 256, 4352 keys, 43.5 / 43.9 / 47.7.  (Not always: of 136 there, 130 rows,
+// 43.5 / 41.8 / 33.7, and the rule does not split.)
 // A split for every tile and CU, as cheap single rows take it, costs more rows up to
 // twice the time (5 rows x 16/2 heads of 512 dims, 4352 keys: 34 splits 44 us, 9 33).
 LaunchPlan plan_fp8(int hd_tile, int n_batch, int n_head_kv, int group, int max_nq, int max_nk, int mask, int n_cu,

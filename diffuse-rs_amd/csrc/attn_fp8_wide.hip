@@ -22,7 +22,7 @@
 // 3400; the rest is the latency of LDS behind the barrier (104 KB a tile) and what
 // of the weights no product covers.  256 f32 rows x 16/2 heads of 512 dims, 4352
 // keys: 90-100 us, 36.5 GFLOP (twice that with both planes), of which starting is
-// 9 us and joining the 4 splits 13.
+// 9 us and joining the 4 splits 13.  Two planes spill 7 registers.
 #include "fp8_attn.hpp"
 
 namespace dr {

@@ -1547,7 +1547,8 @@ static int cached_args(dr_step_cache* cache, size_t layer, const dr_batch_item* 
     // 11-23 times it and moves outputs by ~0.24 on a bf16 layer.  Such a call
     // needs a DR_PRECISION_HILO layer, unless the caller forced a kernel
     // family and so asked for bf16 scores.
-    // An 8 bit layer's K is coarser still; only its own kernel reads it.
+    // An 8 bit layer's K is coarser (N(0, 1) rows: outputs off by 2e-2 at the
+    // usual scale, 0.15 at the limit); only its own kernel reads it.
     const bool hilo_layer = cache->klo[layer * cache->n_batch] != nullptr;
     const bool fp8_layer = cache->sc[layer * cache->n_batch] != nullptr;
     a.fp8 = fp8_layer ? 1 : 0;
@@ -1558,10 +1559,13 @@ static int cached_args(dr_step_cache* cache, size_t layer, const dr_batch_item* 
     if (!hilo_layer && !forced &&
         std::fabs(scale) * std::sqrt((double)hd) > MAX_BF16_SCALE)
         return fail(DR_ERR_UNSUPPORTED,
-                    "%s: scale %g is %.1f times 1/sqrt(head_dim %zu), more than bf16 or 8 bit scores hold to the 1e-2 bar; "
+                    "%s: scale %g is %.1f times 1/sqrt(head_dim %zu), %s; "
                     "keep layer %zu at DR_PRECISION_HILO (dr_cache_create_layers, dr_cache_set_precision), or force "
                     "a kernel family (dr_ctx_set_kernel) to accept them",
-                    who, scale, std::fabs(scale) * std::sqrt((double)hd), hd, layer);
+                    who, scale, std::fabs(scale) * std::sqrt((double)hd), hd,
+                    fp8_layer ? "where 8 bit scores move outputs by 0.15 and more"
+                              : "more than bf16 scores hold to the 1e-2 bar",
+                    layer);
     if ((a.q_bf16 || a.o_bf16) && !fp8_layer && ((hd != 128 && hd != 256) || cache->klo[layer * cache->n_batch]))
         return fail(DR_ERR_UNSUPPORTED,
                     "%s: bf16 Q / output rows (dr_ctx_set_q_dtype, dr_ctx_set_o_dtype) need head dim 128 or "

@@ -190,13 +190,30 @@ void dr_cache_destroy(dr_step_cache* cache);
  * stands for NaN.  A position that was never stored reads as zeros.
  * dr_cache_store and the step calls (with their whole epilogue) write such a
  * layer, dr_cache_gather and dr_cache_gather_pass give back the f32 values that
- * it stands for, and every cached attention call reads it: f32 rows with
- * f32-accurate arithmetic on those values, so the cache's own rounding is the
- * only one that counts; bf16 Q and output rows (both: dr_ctx_set_q_dtype,
- * dr_ctx_set_o_dtype) with 11 bit weights, at any head dim.  The scale limit of
- * bf16 layers applies (dr_cache_create_layers).  Changing a layer to or from
- * DR_PRECISION_FP8 drops the rows it holds (they read as zeros) and frees its
- * planes: a captured hipGraph that uses the layer must not be replayed after,
+ * it stands for, and every cached attention call reads it, at any head dim.
+ *
+ * How far outputs are off.  Against the rows that the caller stored: with N(0, 1)
+ * rows and the usual scale 1/sqrt(head_dim) by 3 % of the outputs' own size in the
+ * mean, 16 times a bf16 layer (256 rows over 768 keys of 128: mean-abs 1.8e-3,
+ * max-abs 2.1e-2; bf16 1.1e-4 and 1.4e-3), so such a layer is not held to the 1e-2
+ * / 1e-3 bar of the others; at twice that scale mean-abs 7.6e-3, max-abs 0.15.
+ * Against the values that the codes stand for, f32 rows: what f32 sums are off by,
+ * with Q values held to 2^-22 of themselves or 2^-38 of their row's largest, and
+ * weights to 2^-22 of themselves or 2^-34 of their row's largest, 2^-22 of it
+ * beside V rows, seen or not, up to 2^12 larger.  bf16 Q and output rows (both:
+ * dr_ctx_set_q_dtype, dr_ctx_set_o_dtype): weights of 11 bits, or to 2^-19 of the
+ * row's largest beside V rows up to 2^16 larger.  Scales further apart take a
+ * slower way, where a row's own largest product is the measure: 1.5 to 3.5 times
+ * as long where V's are, up to 7 times where K's are.  Outputs below 2^-118 are
+ * held to 2^-135.
+ *
+ * The scale limit of bf16 layers applies (dr_cache_create_layers).
+ *
+ * Changing a layer to or from DR_PRECISION_FP8 drops the rows it holds (they read
+ * as zeros; dr_cache_split_active does not know, so every position has to be
+ * stored again).  Planes are made before others are freed, so that a failure
+ * leaves the layer as it was: the change needs memory for both.  A captured
+ * hipGraph that uses the layer must not be replayed after a change of precision,
  * and while the context's stream is being captured a change is refused
  * (DR_ERR_INVALID). */
 #define DR_PRECISION_FP8 2
@@ -209,7 +226,8 @@ int dr_cache_set_precision(dr_step_cache* cache, size_t layer, int precision);
  * attention call (dr_attention_cached, _noalloc, _step, _step_epi) on a
  * DR_PRECISION_BF16 or _FP8 layer with |scale| * sqrt(head_dim) > 2 fails with
  * DR_ERR_UNSUPPORTED, since bf16 scores miss the 1e-2 bar there (outputs move
- * by ~0.24 at Gemma's 1.0), unless a kernel family was forced with
+ * by ~0.24 at Gemma's 1.0; 8 bit scores by 0.15 at the limit already), unless a
+ * kernel family was forced with
  * dr_ctx_set_kernel (then the caller accepts bf16 or 8 bit scores). */
 int dr_cache_create_layers(dr_ctx* ctx, size_t n_total, size_t n_layer, const size_t* n_head_kv,
                            const size_t* head_dim, const int* precision, size_t n_batch,
