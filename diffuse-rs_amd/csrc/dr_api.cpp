@@ -1743,14 +1743,14 @@ static int step_impl(dr_step_cache* cache, size_t layer, const dr_step_item* ite
     a.qb = epi->bq;
     a.rope = rope ? rope->d_table : nullptr;
     a.rot = rope ? (int)rope->rope_dim : 0;
+    if (max_nq == 0) return DR_OK;  // (no row to store or to plan for)
     const int mask = mask_of(sliding_window, causal_prefix);
     const int qepi = (epi->bq || rope) ? dr::QEPI_FULL : (epi->q_norm_w ? dr::QEPI_NORM : dr::QEPI_NONE);
     const dr::LaunchPlan p = plan_for(cache->ctx, a, a.hd, max_nq, (int)cache->n_total, mask, qepi);
-    if (max_nq > 0) DR_CHECK(check_q_dtype(a, p, who));  // (before any store)
+    DR_CHECK(check_q_dtype(a, p, who));  // (before any store)
     for (size_t b = 0; b < n_items; ++b)
         DR_CHECK(store_rows(cache, layer, b, items[b].pass, items[b].k, items[b].v, epi->k_norm_w,
                             epi->eps, epi->bk, epi->bv, epi->v_norm, rope, kv_stride));
-    if (max_nq == 0) return DR_OK;
     return launch_plan(cache->ctx, a, p);
 }
 
