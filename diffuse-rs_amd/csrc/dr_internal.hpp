@@ -29,9 +29,10 @@ struct AttnSlot {
     const int* qpos;      // [nq] sequence positions of the queries (device)
     const int* qseq;      // [nq] or nullptr
     const int* qprefix;   // [nq] per-row causal prefix or nullptr
-    const uint16_t* k;    // bf16 bits
-    const uint16_t* vt;   // bf16 bits
+    const uint16_t* k;    // bf16 bits (with AttnArgs::fp8: K's codes)
+    const uint16_t* vt;   // bf16 bits (with AttnArgs::fp8: V's codes)
     const uint16_t* klo;  // K's lo half, bf16(k - bf16(k)), K's layout (the hi/lo kernel) or nullptr
+                          // (with AttnArgs::fp8: the scale bytes)
     const uint16_t* vlo;  // V's lo half in V^T's layout (with klo) or nullptr
     const int* kpos;      // [nk] or nullptr
     const int* kseq;      // [nk] or nullptr
@@ -71,8 +72,8 @@ struct AttnArgs {
     // counter; no split_merge_kernel follows.  The per-wave-stream kernel, and
     // always that of DR_PRECISION_FP8 layers.
     int* ticket;
-    int q_bf16;                    // Q rows are bf16 (the per-wave-stream kernel reads them)
-    int o_bf16;                    // output rows are bf16 (the per-wave-stream kernel writes them)
+    int q_bf16;                    // Q rows are bf16 (the per-wave-stream kernel and 8 bit layers' read them)
+    int o_bf16;                    // output rows are bf16 (the same write them)
     // the Q/K/V epilogue's Q part (forward.rs:291-310): bias before the
     // QK-norm, RoPE after it, at the query rows' positions (qpos)
     const float* qb;               // [n_head*hd] or nullptr
