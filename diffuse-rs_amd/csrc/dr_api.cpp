@@ -1202,6 +1202,178 @@ int dr_quantize_q8k(dr_ctx* ctx, const float* act, size_t n, size_t cols, void* 
     return DR_OK;
 }
 
+// Largest row of microscaled values (32-bit offsets within a tile of 256 rows).
+static constexpr size_t MX_COLS = (size_t)1 << 22;
+
+static int mx_cols(const char* who, const char* what, size_t cols) {
+    if (cols == 0 || cols % 32 != 0 || cols > MX_COLS)
+        return fail(DR_ERR_INVALID, "%s: %s %zu is not a positive multiple of 32 up to %zu", who, what, cols, MX_COLS);
+    return DR_OK;
+}
+
+static int mx_rows(const char* who, const char* what, const dr_mx_rows* r, dr::MxRows& out) {
+    if (!r || !r->codes || !r->scales) return fail(DR_ERR_INVALID, "%s: %s: NULL rows, codes or scales", who, what);
+    if (r->format != DR_MX_E2M1 && r->format != DR_MX_E4M3)
+        return fail(DR_ERR_INVALID, "%s: %s: format %d is neither DR_MX_E2M1 nor DR_MX_E4M3", who, what, r->format);
+    if (((uintptr_t)r->codes & 15) || ((uintptr_t)r->scales & 3))
+        return fail(DR_ERR_INVALID, "%s: %s: codes must be 16-byte and scales 4-byte aligned", who, what);
+    out.codes = static_cast<uint8_t*>(r->codes);
+    out.scales = static_cast<uint8_t*>(r->scales);
+    out.format = r->format;
+    return DR_OK;
+}
+
+static int mx_dtype(const char* who, int dtype) {
+    if (dtype != DR_DTYPE_F32 && dtype != DR_DTYPE_BF16)
+        return fail(DR_ERR_INVALID, "%s: dtype %d is neither DR_DTYPE_F32 nor DR_DTYPE_BF16", who, dtype);
+    return DR_OK;
+}
+
+// rows of x: x_stride (0: cols) elements apart, each 16-byte aligned
+static int mx_stride(const char* who, const void* x, int dtype, size_t cols, size_t& x_stride) {
+    if (x_stride == 0) x_stride = cols;
+    if (x_stride < cols || x_stride % (dtype == DR_DTYPE_F32 ? 4 : 8) || ((uintptr_t)x & 15))
+        return fail(DR_ERR_INVALID, "%s: rows of %zu values, %zu apart, must not overlap and must start 16-byte aligned", who,
+                    cols, x_stride);
+    return DR_OK;
+}
+
+int dr_mx_quantize(dr_ctx* ctx, const void* x, int dtype, size_t n, size_t cols, size_t x_stride, const dr_mx_rows* out) {
+    const char* who = "dr_mx_quantize";
+    if (!ctx) return fail(DR_ERR_INVALID, "%s: ctx is NULL", who);
+    DR_CHECK(mx_dtype(who, dtype));
+    DR_CHECK(mx_cols(who, "cols", cols));
+    if (n == 0) return DR_OK;
+    dr::MxConvertArgs a{};
+    DR_CHECK(mx_rows(who, "out", out, a.rows));
+    if (!x) return fail(DR_ERR_INVALID, "%s: x is NULL", who);
+    DR_CHECK(mx_stride(who, x, dtype, cols, x_stride));
+    if (n > ((size_t)1 << 30) / (cols / 32) || x_stride > SIZE_MAX / 4 / n)
+        return fail(DR_ERR_INVALID, "%s: %zu x %zu too large", who, n, cols);
+    DR_CHECK(use_device(ctx));
+    a.x = x;
+    a.x_stride = x_stride;
+    a.n = (uint32_t)n;
+    a.blocks = (uint32_t)(cols / 32);
+    a.bf16 = dtype == DR_DTYPE_BF16;
+    hipError_t e = dr::launch_mx_quantize(a, ctx->stream);
+    if (e != hipSuccess) return hip_fail(e, "mx_quantize launch");
+    return DR_OK;
+}
+
+int dr_mx_dequantize(dr_ctx* ctx, const dr_mx_rows* rows, size_t n, size_t cols, void* out, int dtype) {
+    const char* who = "dr_mx_dequantize";
+    if (!ctx) return fail(DR_ERR_INVALID, "%s: ctx is NULL", who);
+    DR_CHECK(mx_dtype(who, dtype));
+    DR_CHECK(mx_cols(who, "cols", cols));
+    if (n == 0) return DR_OK;
+    dr::MxConvertArgs a{};
+    DR_CHECK(mx_rows(who, "rows", rows, a.rows));
+    if (!out || ((uintptr_t)out & 15)) return fail(DR_ERR_INVALID, "%s: out is NULL or not 16-byte aligned", who);
+    if (n > ((size_t)1 << 30) / (cols / 32)) return fail(DR_ERR_INVALID, "%s: %zu x %zu too large", who, n, cols);
+    DR_CHECK(use_device(ctx));
+    a.out = out;
+    a.n = (uint32_t)n;
+    a.blocks = (uint32_t)(cols / 32);
+    a.bf16 = dtype == DR_DTYPE_BF16;
+    hipError_t e = dr::launch_mx_dequantize(a, ctx->stream);
+    if (e != hipSuccess) return hip_fail(e, "mx_dequantize launch");
+    return DR_OK;
+}
+
+int dr_rms_norm_mx(dr_ctx* ctx, const void* x, const void* residual, void* sum, int dtype, size_t n, size_t cols,
+                   size_t x_stride, const float* w, float eps, const dr_mx_rows* out) {
+    const char* who = "dr_rms_norm_mx";
+    if (!ctx) return fail(DR_ERR_INVALID, "%s: ctx is NULL", who);
+    DR_CHECK(mx_dtype(who, dtype));
+    DR_CHECK(mx_cols(who, "cols", cols));
+    if (n == 0) return DR_OK;
+    dr::MxNormArgs a{};
+    DR_CHECK(mx_rows(who, "out", out, a.rows));
+    if (!x) return fail(DR_ERR_INVALID, "%s: x is NULL", who);
+    DR_CHECK(mx_stride(who, x, dtype, cols, x_stride));
+    if (((uintptr_t)residual & 15) || ((uintptr_t)sum & 15) || ((uintptr_t)w & 15))
+        return fail(DR_ERR_INVALID, "%s: residual, sum and w must be 16-byte aligned", who);
+    if (sum == x && x_stride != cols)
+        return fail(DR_ERR_INVALID, "%s: sum is x, whose rows are %zu apart and not %zu", who, x_stride, cols);
+    if (n > (size_t)INT32_MAX / 256 || x_stride > SIZE_MAX / 4 / n)
+        return fail(DR_ERR_INVALID, "%s: %zu x %zu too large", who, n, cols);
+    DR_CHECK(use_device(ctx));
+    a.x = x;
+    a.residual = residual;
+    a.sum = sum;
+    a.w = w;
+    a.x_stride = x_stride;
+    a.n = (int)n;
+    a.cols = (int)cols;
+    a.bf16 = dtype == DR_DTYPE_BF16;
+    a.eps = eps;
+    hipError_t e = dr::launch_mx_norm(a, ctx->stream);
+    if (e != hipSuccess) return hip_fail(e, "rms_norm_mx launch");
+    return DR_OK;
+}
+
+// what both products check of their weights and activations
+static int mx_operands(const char* who, const dr_mx_rows* w, size_t rows, size_t cols, const dr_mx_rows* act, size_t n,
+                       dr::MxMatArgs& a) {
+    DR_CHECK(mx_rows(who, "weights", w, a.w));
+    DR_CHECK(mx_rows(who, "act", act, a.act));
+    if (a.w.format != DR_MX_E2M1)
+        return fail(DR_ERR_UNSUPPORTED, "%s: weights of format %d not built (DR_MX_E2M1 = 0)", who, a.w.format);
+    if (rows > (size_t)INT32_MAX / 256 || n > (size_t)INT32_MAX / 256)
+        return fail(DR_ERR_INVALID, "%s: %zu x %zu x %zu too large", who, n, rows, cols);
+    a.rows = (int)rows;
+    a.cols = (int)cols;
+    a.n = (int)n;
+    return DR_OK;
+}
+
+int dr_mx_matmul(dr_ctx* ctx, const dr_mx_rows* w, size_t rows, size_t cols, const dr_mx_rows* act, size_t n, void* out,
+                 const void* residual, int dtype) {
+    const char* who = "dr_mx_matmul";
+    if (!ctx) return fail(DR_ERR_INVALID, "%s: ctx is NULL", who);
+    DR_CHECK(mx_dtype(who, dtype));
+    DR_CHECK(mx_cols(who, "cols", cols));
+    if (n == 0 || rows == 0) return DR_OK;
+    dr::MxMatArgs a{};
+    DR_CHECK(mx_operands(who, w, rows, cols, act, n, a));
+    const uintptr_t to = dtype == DR_DTYPE_F32 ? 3 : 1;
+    if (!out || ((uintptr_t)out & to) || ((uintptr_t)residual & to))
+        return fail(DR_ERR_INVALID, "%s: out is NULL, or out or residual not aligned to its type", who);
+    DR_CHECK(use_device(ctx));
+    a.out = out;
+    a.residual = residual;
+    a.bf16 = dtype == DR_DTYPE_BF16;
+    a.n_cu = ctx->n_cu;
+    hipError_t e = dr::launch_mx_matmul(a, ctx->stream);
+    if (e != hipSuccess) return hip_fail(e, "mx_matmul launch");
+    return DR_OK;
+}
+
+int dr_mx_gated(dr_ctx* ctx, const dr_mx_rows* gate, const dr_mx_rows* up, size_t rows, size_t cols, const dr_mx_rows* act,
+                size_t n, int activation, const dr_mx_rows* out) {
+    const char* who = "dr_mx_gated";
+    if (!ctx) return fail(DR_ERR_INVALID, "%s: ctx is NULL", who);
+    if (activation != DR_ACT_SILU && activation != DR_ACT_GELU)
+        return fail(DR_ERR_INVALID, "%s: activation %d is neither DR_ACT_SILU nor DR_ACT_GELU", who, activation);
+    DR_CHECK(mx_cols(who, "cols", cols));
+    if (n == 0 || rows == 0) return DR_OK;
+    DR_CHECK(mx_cols(who, "rows", rows));
+    dr::MxMatArgs a{};
+    DR_CHECK(mx_operands(who, gate, rows, cols, act, n, a));
+    DR_CHECK(mx_rows(who, "up", up, a.up));
+    if (a.up.format != DR_MX_E2M1)
+        return fail(DR_ERR_UNSUPPORTED, "%s: weights of format %d not built (DR_MX_E2M1 = 0)", who, a.up.format);
+    DR_CHECK(mx_rows(who, "out", out, a.hidden));
+    DR_CHECK(use_device(ctx));
+    a.gated = 1;
+    a.fn = activation;
+    a.n_cu = ctx->n_cu;
+    hipError_t e = dr::launch_mx_matmul(a, ctx->stream);
+    if (e != hipSuccess) return hip_fail(e, "mx_gated launch");
+    return DR_OK;
+}
+
 int dr_cache_update_seq(dr_step_cache* cache, size_t batch, const int32_t* seq, size_t n) {
     if (!cache) return fail(DR_ERR_INVALID, "dr_cache_update_seq: cache is NULL");
     if (batch >= cache->n_batch) return fail(DR_ERR_INVALID, "dr_cache_update_seq: batch %zu >= %zu", batch, cache->n_batch);

@@ -420,4 +420,60 @@ hipError_t launch_quantize_q80(const float* act, int n, int cols, void* out, hip
 // quantize_rows_q8_k into the reference's BlockQ8K layout
 hipError_t launch_quantize_q8k(const float* act, int n, int cols, Q8KBlock* out, hipStream_t st);
 
+// ---- microscaled rows (dr_mx_rows; the format: mx_common.hpp)
+enum MxFormat : int { MX_E2M1 = 0, MX_E4M3 = 1 };
+enum MxAct : int { MX_SILU = 0, MX_GELU = 1 };
+struct MxRows {
+    uint8_t* codes;
+    uint8_t* scales;
+    int format;
+};
+// bytes between the scale rows, and of a row of codes
+constexpr size_t mx_pitch(size_t cols) { return (cols / 32 + 3) / 4 * 4; }
+constexpr size_t mx_row_bytes(int format, size_t cols) { return format == MX_E2M1 ? cols / 2 : cols; }
+
+// dr_mx_quantize, dr_mx_dequantize
+struct MxConvertArgs {
+    const void* x;  // quantise: the rows, x_stride elements apart
+    void* out;      // dequantise: contiguous rows
+    MxRows rows;
+    size_t x_stride;
+    uint32_t n, blocks;  // rows, blocks of a row; n * blocks < 2^30
+    int bf16;            // x, out: bf16 rather than f32
+};
+hipError_t launch_mx_quantize(const MxConvertArgs& a, hipStream_t st);
+hipError_t launch_mx_dequantize(const MxConvertArgs& a, hipStream_t st);
+
+// dr_rms_norm_mx
+struct MxNormArgs {
+    const void* x;         // rows x_stride elements apart
+    const void* residual;  // contiguous rows, or nullptr
+    void* sum;             // contiguous rows, or nullptr
+    const float* w;        // gain, or nullptr
+    MxRows rows;
+    size_t x_stride;
+    int n, cols;
+    int bf16;  // x, residual, sum
+    float eps;
+};
+hipError_t launch_mx_norm(const MxNormArgs& a, hipStream_t st);
+
+// dr_mx_matmul, dr_mx_gated: weights E2M1 [rows][cols], activations [n][cols]
+struct MxMatArgs {
+    MxRows w;   // gated: the gate projection
+    MxRows up;  // gated
+    MxRows act;
+    int rows, cols, n;
+    int gated;
+    // product
+    void* out;             // [n][rows]
+    const void* residual;  // the same, or nullptr
+    int bf16;              // out, residual
+    // gated
+    MxRows hidden;  // [n][rows]
+    int fn;         // MxAct
+    int n_cu;
+};
+hipError_t launch_mx_matmul(const MxMatArgs& a, hipStream_t st);
+
 }  // namespace dr

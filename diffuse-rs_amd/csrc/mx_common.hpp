@@ -1,0 +1,136 @@
+// mx_common.hpp -- microscaled rows (dr_mx_rows), shared by mx_rows.hip
+// (quantisation, norm) and the products of mx_few.hip and mx_tile.hip.
+//
+// 32 consecutive values of a row are a block: they share 2^e, held as the byte
+// e + 127 (255: the whole block stands for NaN), and each is an E2M1 (4 bit) or
+// E4M3 (8 bit) code times 2^e.  With a = max |x| of the block, e is the smallest
+// that keeps a / 2^e within the largest code (6 or 448), so nothing saturates;
+// e >= -126, which keeps 2^-e a normal f32 number (blocks of zeros have e = -126).
+// Codes are to nearest, ties to even.
+//   codes   [n][cols / 2] bytes (value 2 j in the low half of byte j), or [n][cols]
+//   scales  [n][mx_pitch(cols)]: one byte per block, rows at multiples of 4 bytes
+//           so that four blocks' bytes are one aligned load; the bytes between
+//           a row's last block and the next row are neither read as scales nor
+//           written.
+#pragma once
+
+#include "dr_internal.hpp"
+
+namespace dr {
+namespace {
+
+constexpr int MX_NAN = 255;
+
+using bf16x2 = __bf16 __attribute__((ext_vector_type(2)));
+using bf16x8m = __bf16 __attribute__((ext_vector_type(8)));
+using f32x2m = float __attribute__((ext_vector_type(2)));
+using f32x4m = float __attribute__((ext_vector_type(4)));
+using u32x4m = uint32_t __attribute__((ext_vector_type(4)));
+using u32x2m = uint32_t __attribute__((ext_vector_type(2)));
+
+// Scale byte of a block whose largest magnitude has the bit pattern `bits` (sign
+// cleared; compared as integers, so a NaN is larger than an infinity, and that
+// larger than every number).
+template <int FMT>
+__device__ __forceinline__ int mx_scale_byte(uint32_t bits) {
+    if (bits >= 0x7f800000u) return MX_NAN;
+    const int top = FMT == MX_E2M1 ? 2 : 8;
+    const uint32_t frac = FMT == MX_E2M1 ? 0x400000u : 0x600000u;  // of 6 = 1.5 * 2^2 and 448 = 1.75 * 2^8
+    const int e = (int)(bits >> 23) - top + ((bits & 0x7fffffu) > frac ? 1 : 0);
+    return e < 1 ? 1 : e;
+}
+
+// 2^e of a scale byte as f32, NaN for MX_NAN.
+__device__ __forceinline__ float mx_scale(int byte) {
+    return __uint_as_float(byte == 0 ? 0x400000u : byte == MX_NAN ? 0x7fc00000u : (uint32_t)byte << 23);
+}
+
+// The codes of 8 values with their block's scale byte: 4 bytes (E2M1) or 8.
+// Dividing by a power of two is exact but for results far below the smallest code.
+template <int FMT>
+__device__ __forceinline__ u32x2m mx_encode8(const float (&x)[8], int byte) {
+    u32x2m c = {0, 0};
+    if (byte == MX_NAN) return c;
+    if constexpr (FMT == MX_E2M1) {
+        const float s = __uint_as_float((uint32_t)byte << 23);
+        c[0] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c[0], x[0], x[1], s, 0);
+        c[0] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c[0], x[2], x[3], s, 1);
+        c[0] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c[0], x[4], x[5], s, 2);
+        c[0] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c[0], x[6], x[7], s, 3);
+    } else {
+        const float inv = __uint_as_float((uint32_t)(254 - byte) << 23);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            int w = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * h] * inv, x[4 * h + 1] * inv, 0, false);
+            c[h] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[4 * h + 2] * inv, x[4 * h + 3] * inv, w, true);
+        }
+    }
+    return c;
+}
+
+// The f32 values of 8 codes.
+template <int FMT>
+__device__ __forceinline__ void mx_decode8(u32x2m c, int byte, float (&x)[8]) {
+    const float s = mx_scale(byte);
+    f32x2m p[4];
+    if constexpr (FMT == MX_E2M1) {
+        p[0] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c[0], 1.0f, 0);
+        p[1] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c[0], 1.0f, 1);
+        p[2] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c[0], 1.0f, 2);
+        p[3] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c[0], 1.0f, 3);
+    } else {
+        p[0] = __builtin_amdgcn_cvt_pk_f32_fp8((int)c[0], false);
+        p[1] = __builtin_amdgcn_cvt_pk_f32_fp8((int)c[0], true);
+        p[2] = __builtin_amdgcn_cvt_pk_f32_fp8((int)c[1], false);
+        p[3] = __builtin_amdgcn_cvt_pk_f32_fp8((int)c[1], true);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = p[i / 2][i % 2] * s;
+}
+
+// The largest of a value over a quad of lanes.
+__device__ __forceinline__ uint32_t quad_max(uint32_t v) {
+    v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xf, 0xf, true));  // lanes 1 0 3 2
+    return max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xf, 0xf, true));  // lanes 2 3 0 1
+}
+
+__device__ __forceinline__ uint16_t mx_bf16(float x) { return __builtin_bit_cast(uint16_t, (__bf16)x); }
+__device__ __forceinline__ float mx_f32(uint32_t bf16_bits) { return __uint_as_float(bf16_bits << 16); }
+
+// 8 consecutive f32 or bf16 values (16-byte aligned).
+template <bool BF16>
+__device__ __forceinline__ void load8(const void* base, size_t at, float (&x)[8]) {
+    if constexpr (BF16) {
+        const u32x4m v = *reinterpret_cast<const u32x4m*>(static_cast<const uint16_t*>(base) + at);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[2 * i] = mx_f32(v[i] & 0xffff), x[2 * i + 1] = __uint_as_float(v[i] & 0xffff0000u);
+    } else {
+        const f32x4m* p = reinterpret_cast<const f32x4m*>(static_cast<const float*>(base) + at);
+        const f32x4m a = p[0], b = p[1];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = a[i], x[4 + i] = b[i];
+    }
+}
+template <bool BF16>
+__device__ __forceinline__ void store8(void* base, size_t at, const float (&x)[8]) {
+    if constexpr (BF16) {
+        u32x4m v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = mx_bf16(x[2 * i]) | (uint32_t)mx_bf16(x[2 * i + 1]) << 16;
+        *reinterpret_cast<u32x4m*>(static_cast<uint16_t*>(base) + at) = v;
+    } else {
+        f32x4m* p = reinterpret_cast<f32x4m*>(static_cast<float*>(base) + at);
+        p[0] = f32x4m{x[0], x[1], x[2], x[3]};
+        p[1] = f32x4m{x[4], x[5], x[6], x[7]};
+    }
+}
+
+// x / (1 + e^-x), and gelu in its tanh form: 0.5 x (1 + tanh z) = x / (1 + e^-2z),
+// z = sqrt(2 / pi) (x + 0.044715 x^3), which keeps its digits where tanh is near -1.
+__device__ __forceinline__ float mx_act(float x, int fn) {
+    const float z = fn == MX_SILU ? x : 1.5957691216057308f * (x + 0.044715f * x * x * x);
+    return x / (1.0f + expf(-z));
+}
+
+}  // namespace
+}  // namespace dr

@@ -107,6 +107,10 @@ class CLaunchInfo(ctypes.Structure):
     ]
 
 
+class CMxRows(ctypes.Structure):
+    _fields_ = [("codes", ctypes.c_void_p), ("scales", ctypes.c_void_p), ("format", ctypes.c_int)]
+
+
 class DrError(RuntimeError):
     def __init__(self, status: int, message: str):
         super().__init__(f"{STATUS_NAMES.get(status, status)}: {message}")
@@ -157,6 +161,12 @@ _SIGS = {
     "dr_quantize_q8k": (_I, [_VP, _VP, _SZ, _SZ, _VP]),
     "dr_quantize_q8_0": (_I, [_VP, _VP, _SZ, _SZ, _VP]),
     "dr_qmatmul_post_norm": (_I, [_VP, _I, _VP, _SZ, _SZ, _VP, _SZ, _VP, _VP, _VP, _F]),
+    "dr_mx_quantize": (_I, [_VP, _VP, _I, _SZ, _SZ, _SZ, ctypes.POINTER(CMxRows)]),
+    "dr_mx_dequantize": (_I, [_VP, ctypes.POINTER(CMxRows), _SZ, _SZ, _VP, _I]),
+    "dr_rms_norm_mx": (_I, [_VP, _VP, _VP, _VP, _I, _SZ, _SZ, _SZ, _VP, _F, ctypes.POINTER(CMxRows)]),
+    "dr_mx_matmul": (_I, [_VP, ctypes.POINTER(CMxRows), _SZ, _SZ, ctypes.POINTER(CMxRows), _SZ, _VP, _VP, _I]),
+    "dr_mx_gated": (_I, [_VP, ctypes.POINTER(CMxRows), ctypes.POINTER(CMxRows), _SZ, _SZ, ctypes.POINTER(CMxRows), _SZ,
+                         _I, ctypes.POINTER(CMxRows)]),
     "dr_pass_destroy": (None, [_VP]),
     "dr_cache_create": (_I, [_VP, _SZ, _SZ, c_size_p, c_size_p, _SZ, ctypes.POINTER(_VP)]),
     "dr_cache_create_layers": (_I, [_VP, _SZ, _SZ, c_size_p, c_size_p, _VP, _SZ, ctypes.POINTER(_VP)]),
@@ -686,3 +696,53 @@ def quantize_q8_0(ctx: Context, act, n: int, cols: int, out) -> None:
     """quantize_row_q8_0 (matmul.rs:73-82) into n * cols/32 BlockQ8_0
     (34 bytes each) at device pointer / tensor out."""
     _check(ctx.lib.dr_quantize_q8_0(ctx.h, _ptr(act), n, cols, _ptr(out)))
+
+
+MX_E2M1, MX_E4M3 = 0, 1  # dr_mx_rows.format
+ACT_SILU, ACT_GELU = 0, 1  # dr_mx_gated
+
+
+def mx_pitch(cols: int) -> int:
+    """Bytes between the scale rows of microscaled rows of ``cols`` values: one
+    byte per 32 values, rows at multiples of 4 bytes."""
+    return (cols // 32 + 3) // 4 * 4
+
+
+class MxRows:
+    """dr_mx_rows: device tensors (or addresses) of microscaled rows' codes
+    ([n][cols / 2] bytes for MX_E2M1, [n][cols] for MX_E4M3) and scale bytes
+    ([n][mx_pitch(cols)])."""
+
+    def __init__(self, codes, scales, format: int):
+        self.codes, self.scales, self.format = codes, scales, format  # (held: the struct has their addresses)
+        self.c = CMxRows(_ptr(codes), _ptr(scales), format)
+
+
+def mx_quantize(ctx: Context, x, n: int, cols: int, out: MxRows, dtype: int = DTYPE_F32, stride: int = 0) -> None:
+    """f32 or bf16 rows, ``stride`` elements apart (0: cols), into microscaled rows (dr_mx_quantize)."""
+    _check(ctx.lib.dr_mx_quantize(ctx.h, _ptr(x), dtype, n, cols, stride, out.c))
+
+
+def mx_dequantize(ctx: Context, rows: MxRows, n: int, cols: int, out, dtype: int = DTYPE_F32) -> None:
+    """The values that microscaled rows stand for, f32 or bf16 (dr_mx_dequantize)."""
+    _check(ctx.lib.dr_mx_dequantize(ctx.h, rows.c, n, cols, _ptr(out), dtype))
+
+
+def rms_norm_mx(ctx: Context, x, n: int, cols: int, out: MxRows, w=None, eps: float = 1e-6, residual=None, total=None,
+                dtype: int = DTYPE_F32, stride: int = 0) -> None:
+    """x + residual (into ``total`` where given), its RMSNorm with the gain w,
+    quantised into ``out`` (dr_rms_norm_mx)."""
+    _check(ctx.lib.dr_rms_norm_mx(ctx.h, _ptr(x), _ptr(residual) or None, _ptr(total) or None, dtype, n, cols, stride,
+                                  _ptr(w) or None, eps, out.c))
+
+
+def mx_matmul(ctx: Context, w: MxRows, rows: int, cols: int, act: MxRows, n: int, out, residual=None,
+              dtype: int = DTYPE_F32) -> None:
+    """out = act w^T + residual with 4 bit weights (dr_mx_matmul)."""
+    _check(ctx.lib.dr_mx_matmul(ctx.h, w.c, rows, cols, act.c, n, _ptr(out), _ptr(residual) or None, dtype))
+
+
+def mx_gated(ctx: Context, gate: MxRows, up: MxRows, rows: int, cols: int, act: MxRows, n: int, out: MxRows,
+             activation: int = ACT_SILU) -> None:
+    """The gated projections: f(act gate^T) * (act up^T), quantised (dr_mx_gated)."""
+    _check(ctx.lib.dr_mx_gated(ctx.h, gate.c, up.c, rows, cols, act.c, n, activation, out.c))

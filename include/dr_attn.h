@@ -495,6 +495,74 @@ int dr_quantize_q8k(dr_ctx* ctx, const float* act, size_t n, size_t cols, void* 
  * qs[32] = round(x / d) half away from zero), 2-byte aligned. */
 int dr_quantize_q8_0(dr_ctx* ctx, const float* act, size_t n, size_t cols, void* out);
 
+/* ---- the feed-forward after the attention, on microscaled rows (no counterpart
+ * in the reference, whose weights are GGUF blocks and whose activations Q8_K or
+ * Q8_0 blocks; the steps are those of its ffn_block, src/model/forward.rs:354-542:
+ * norm, gate and up projections, SiLU or GeGLU, down projection, residual).
+ *
+ * A microscaled row is cut into blocks of 32 consecutive values that share a
+ * power of two 2^e; each value is a code times 2^e.  DR_MX_E2M1: 4 bit codes (0,
+ * 0.5, 1, 1.5, 2, 3, 4, 6 and a sign), value 2 j in the low half of byte j.
+ * DR_MX_E4M3: 8 bit codes, magnitudes up to 448.  codes: [n][cols / 2] or [n][cols]
+ * bytes, 16-byte aligned.  scales: one byte e + 127 per block, rows ceil(cols / 32
+ * / 4) * 4 bytes apart (no gaps where cols is a multiple of 128), 4-byte aligned;
+ * byte 255 makes its block NaN, and bytes in a gap are neither read as scales nor
+ * written.  This is the OCP MX layout (MXFP4, MXFP8 E4M3): rows quantised elsewhere
+ * can be used.  Rows quantised here: e is the smallest, at least -126, that keeps
+ * the block's largest magnitude within the largest code (6, 448), so that nothing
+ * saturates; codes to nearest, ties to even; a block with a NaN or an infinity
+ * stands for NaN.  cols is a multiple of 32, at most 2^22.
+ *
+ * All calls enqueue on the context's stream, allocate nothing and use no
+ * workspace, so they can be captured into a hipGraph.  n == 0 (rows == 0) writes
+ * nothing.  An output must not overlap an input other than where said. */
+#define DR_MX_E2M1 0
+#define DR_MX_E4M3 1
+typedef struct {
+    void* codes;   /* device */
+    void* scales;  /* device */
+    int format;    /* DR_MX_E2M1 or DR_MX_E4M3 */
+} dr_mx_rows;
+
+/* x [n][cols] (DR_DTYPE_F32 or _BF16, rows x_stride elements apart, 0: cols; rows
+ * start 16-byte aligned) -> out. */
+int dr_mx_quantize(dr_ctx* ctx, const void* x, int dtype, size_t n, size_t cols, size_t x_stride,
+                   const dr_mx_rows* out);
+/* The values that rows stand for -> out [n][cols] (DR_DTYPE_F32, or _BF16, which
+ * holds every code exactly; 16-byte aligned).  Values past the type's largest
+ * (a block near f32's, rounded up) read back as infinities, values below its
+ * smallest rounded. */
+int dr_mx_dequantize(dr_ctx* ctx, const dr_mx_rows* rows, size_t n, size_t cols, void* out, int dtype);
+
+/* The residual's addition, RMSNorm and quantisation in one pass:
+ *   h = x + residual, rounded to dtype      (residual NULL: h = x)
+ *   sum = h                                 (NULL: not written)
+ *   out = codes of h / sqrt(mean(h^2) + eps) * w   (w: device, [cols] f32; NULL: ones)
+ * as rms_norm (src/model/ops.rs:7-104) of the new residual stream, which forward.rs
+ * makes before each block's projections.  x, residual and sum are dtype
+ * (DR_DTYPE_F32 or _BF16); x has rows x_stride elements apart (0: cols), residual
+ * and sum are [n][cols]; sum may be x (then x_stride is cols) or residual.  The
+ * squares are summed in f32 over the held h. */
+int dr_rms_norm_mx(dr_ctx* ctx, const void* x, const void* residual, void* sum, int dtype, size_t n, size_t cols,
+                   size_t x_stride, const float* w, float eps, const dr_mx_rows* out);
+
+/* out[t][r] = sum_k w[r][k] act[t][k] + residual[t][r]: w DR_MX_E2M1 [rows][cols], act
+ * [n][cols] of either format, out and residual (NULL: none; may be out) [n][rows] of
+ * dtype DR_DTYPE_F32 or _BF16. */
+int dr_mx_matmul(dr_ctx* ctx, const dr_mx_rows* w, size_t rows, size_t cols, const dr_mx_rows* act, size_t n,
+                 void* out, const void* residual, int dtype);
+
+/* The gated projections with their activation, in one kernel:
+ *   out = codes of f(act gate^T) * (act up^T)
+ * gate and up DR_MX_E2M1 [rows][cols], act [n][cols] of either format, out [n][rows] of
+ * either format (rows a multiple of 32).  f: DR_ACT_SILU x / (1 + e^-x)
+ * (silu_mul, ops.rs:282-350), DR_ACT_GELU 0.5 x (1 + tanh(sqrt(2 / pi) (x + 0.044715
+ * x^3))) (GeGLU, ops.rs:126-138). */
+#define DR_ACT_SILU 0
+#define DR_ACT_GELU 1
+int dr_mx_gated(dr_ctx* ctx, const dr_mx_rows* gate, const dr_mx_rows* up, size_t rows, size_t cols,
+                const dr_mx_rows* act, size_t n, int activation, const dr_mx_rows* out);
+
 /* Launch configuration of the last attention kernel this context enqueued
  * (for measurement): key splits across workgroups, workgroups, waves per
  * workgroup, keys per tile, head-dim tile, 32-row query blocks and key
