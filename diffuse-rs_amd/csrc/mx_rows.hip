@@ -55,13 +55,35 @@ __global__ __launch_bounds__(256) void mx_dequantize_kernel(const MxConvertArgs 
     store8<BF16>(a.out, (size_t)u * 8, x);
 }
 
+// The root of a row's mean square: sums of eight f32 squares are added in 64 bits
+// (as the reference sums them), so that the factor is off by its own rounding alone:
+// an f32 sum's few 2^-24 move ten times as many values past a border between codes.
+template <int WAVES>
+__device__ __forceinline__ float row_factor(double ss, double (&part)[WAVES], const MxNormArgs& a) {
+#pragma unroll
+    for (int d = 32; d; d >>= 1) ss += __shfl_xor(ss, d);
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = ss;
+    __syncthreads();
+    ss = 0.0;
+#pragma unroll
+    for (int i = 0; i < WAVES; ++i) ss += part[i];
+    return (float)(1.0 / sqrt(ss / (double)a.cols + (double)a.eps));
+}
+__device__ __forceinline__ float squares8(const float (&h)[8]) {
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s = fmaf(h[i], h[i], s);
+    return s;
+}
+
 // One workgroup per row; a row of up to 16384 values stays in registers.
 template <int FMT, bool BF16, int NV>
 __global__ __launch_bounds__(256) void mx_norm_kernel(const MxNormArgs a) {
-    __shared__ float s_part[4];
+    __shared__ double s_part[4];
     const size_t row = blockIdx.x;
     const size_t xo = row * a.x_stride, ro = row * (size_t)a.cols;
-    float h[NV][8], ss = 0.0f;
+    float h[NV][8];
+    double ss = 0.0;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
         const int at = (v * 256 + (int)threadIdx.x) * 8;
@@ -81,15 +103,9 @@ __global__ __launch_bounds__(256) void mx_norm_kernel(const MxNormArgs a) {
             }
         }
         if (a.sum) store8<BF16>(a.sum, ro + at, h[v]);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) ss += h[v][i] * h[v][i];
+        ss += squares8(h[v]);
     }
-#pragma unroll
-    for (int d = 32; d; d >>= 1) ss += __shfl_xor(ss, d);
-    if ((threadIdx.x & 63) == 0) s_part[threadIdx.x >> 6] = ss;
-    __syncthreads();
-    ss = (s_part[0] + s_part[1]) + (s_part[2] + s_part[3]);
-    const float scale = 1.0f / sqrtf(ss / (float)a.cols + a.eps);
+    const float scale = row_factor(ss, s_part, a);
     const size_t pitch = mx_pitch(a.cols), code_row = row * mx_row_bytes(FMT, a.cols);
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
@@ -118,7 +134,7 @@ __global__ __launch_bounds__(256) void mx_norm_kernel(const MxNormArgs a) {
 // one (it may lie over x or the residual).
 template <int FMT, bool BF16>
 __global__ __launch_bounds__(1024) void mx_norm_long_kernel(const MxNormArgs a) {
-    __shared__ float s_part[16];
+    __shared__ double s_part[16];
     const size_t row = blockIdx.x;
     const size_t xo = row * a.x_stride, ro = row * (size_t)a.cols;
     auto row8 = [&](int at, float (&h)[8]) {
@@ -132,24 +148,14 @@ __global__ __launch_bounds__(1024) void mx_norm_long_kernel(const MxNormArgs a) 
             if constexpr (BF16) h[i] = mx_f32(mx_bf16(h[i]));
         }
     };
-    float ss = 0.0f;
+    double ss = 0.0;
     for (int at = (int)threadIdx.x * 8; at < a.cols; at += 8192) {
         float h[8];
         row8(at, h);
         if (a.sum) store8<BF16>(a.sum, ro + at, h);
-        float s8 = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) s8 += h[i] * h[i];
-        ss += s8;
+        ss += squares8(h);
     }
-#pragma unroll
-    for (int d = 32; d; d >>= 1) ss += __shfl_xor(ss, d);
-    if ((threadIdx.x & 63) == 0) s_part[threadIdx.x >> 6] = ss;
-    __syncthreads();
-    ss = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) ss += s_part[i];
-    const float scale = 1.0f / sqrtf(ss / (float)a.cols + a.eps);
+    const float scale = row_factor(ss, s_part, a);
     const size_t pitch = mx_pitch(a.cols), code_row = row * mx_row_bytes(FMT, a.cols);
     for (int at = (int)threadIdx.x * 8; at < a.cols; at += 8192) {
         float h[8], w[8] = {1, 1, 1, 1, 1, 1, 1, 1};
