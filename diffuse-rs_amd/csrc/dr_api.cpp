@@ -1320,7 +1320,7 @@ static int mx_operands(const char* who, const dr_mx_rows* w, size_t rows, size_t
     DR_CHECK(mx_rows(who, "act", act, a.act));
     if (a.w.format != DR_MX_E2M1)
         return fail(DR_ERR_UNSUPPORTED, "%s: weights of format %d not built (DR_MX_E2M1 = 0)", who, a.w.format);
-    if (rows > (size_t)INT32_MAX / 256 || n > (size_t)INT32_MAX / 256)
+    if (rows > (size_t)INT32_MAX / 256 || n > (size_t)INT32_MAX / 256 || (rows + 15) / 16 * ((n + 15) / 16) > (size_t)INT32_MAX)
         return fail(DR_ERR_INVALID, "%s: %zu x %zu x %zu too large", who, n, rows, cols);
     a.rows = (int)rows;
     a.cols = (int)cols;
@@ -1344,6 +1344,7 @@ int dr_mx_matmul(dr_ctx* ctx, const dr_mx_rows* w, size_t rows, size_t cols, con
     a.out = out;
     a.residual = residual;
     a.bf16 = dtype == DR_DTYPE_BF16;
+    a.vec = (((uintptr_t)out | (uintptr_t)residual) & 15) == 0;
     a.n_cu = ctx->n_cu;
     hipError_t e = dr::launch_mx_matmul(a, ctx->stream);
     if (e != hipSuccess) return hip_fail(e, "mx_matmul launch");

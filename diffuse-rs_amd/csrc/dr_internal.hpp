@@ -469,11 +469,13 @@ struct MxMatArgs {
     void* out;             // [n][rows]
     const void* residual;  // the same, or nullptr
     int bf16;              // out, residual
+    int vec;               // both 16-byte aligned
     // gated
     MxRows hidden;  // [n][rows]
     int fn;         // MxAct
     int n_cu;
 };
 hipError_t launch_mx_matmul(const MxMatArgs& a, hipStream_t st);
+hipError_t launch_mx_tile(const MxMatArgs& a, hipStream_t st);
 
 }  // namespace dr

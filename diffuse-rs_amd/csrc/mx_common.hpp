@@ -132,5 +132,16 @@ __device__ __forceinline__ float mx_act(float x, int fn) {
     return x / (1.0f + expf(-z));
 }
 
+// One sum of a product, with its residual, at element `at` of out.
+__device__ __forceinline__ void put_sum(const MxMatArgs& a, size_t at, float x) {
+    if (a.bf16) {
+        if (a.residual) x += mx_f32(static_cast<const uint16_t*>(a.residual)[at]);
+        static_cast<uint16_t*>(a.out)[at] = mx_bf16(x);
+    } else {
+        if (a.residual) x += static_cast<const float*>(a.residual)[at];
+        static_cast<float*>(a.out)[at] = x;
+    }
+}
+
 }  // namespace
 }  // namespace dr

@@ -48,7 +48,8 @@ __global__ __launch_bounds__(512) void mx_few_kernel(const MxMatArgs a) {
     __shared__ __align__(16) float s_sum[8][MT][16 * ROW];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, g = lane >> 4;
-    const int strip = blockIdx.x * FT * 16, tok0 = blockIdx.y * 16;
+    const int strips = (a.rows + FT * 16 - 1) / (FT * 16);
+    const int tg = blockIdx.x / strips, strip = (blockIdx.x - tg * strips) * FT * 16, tok0 = tg * 16;
     const int nblk = a.cols / 32, steps = (nblk + 15) / 16;
     const size_t pitch = mx_pitch(a.cols), w_row = a.cols / 2, a_row = mx_row_bytes(AF, a.cols);
 
@@ -123,15 +124,7 @@ __global__ __launch_bounds__(512) void mx_few_kernel(const MxMatArgs a) {
         for (int e = threadIdx.x; e < MT * 256; e += 512) {
             const int f = e % (MT * 16), t = e / (MT * 16);
             if (strip + f >= a.rows || tok0 + t >= a.n) continue;
-            float x = total(f / 16, f % 16, t);
-            const size_t at = (size_t)(tok0 + t) * a.rows + strip + f;
-            if (a.bf16) {
-                if (a.residual) x += mx_f32(static_cast<const uint16_t*>(a.residual)[at]);
-                static_cast<uint16_t*>(a.out)[at] = mx_bf16(x);
-            } else {
-                if (a.residual) x += static_cast<const float*>(a.residual)[at];
-                static_cast<float*>(a.out)[at] = x;
-            }
+            put_sum(a, (size_t)(tok0 + t) * a.rows + strip + f, total(f / 16, f % 16, t));
         }
     } else {
         static_assert(!GATED || MT == 4, "a strip is one block of the output");
@@ -163,9 +156,9 @@ template <int AF>
 hipError_t few(const MxMatArgs& a, hipStream_t st) {
     const unsigned tg = (unsigned)((a.n + 15) / 16);
     if (a.gated)
-        hipLaunchKernelGGL((mx_few_kernel<AF, true, 4>), dim3((unsigned)(a.rows / 32), tg), dim3(512), 0, st, a);
+        hipLaunchKernelGGL((mx_few_kernel<AF, true, 4>), dim3(tg * (unsigned)(a.rows / 32)), dim3(512), 0, st, a);
     else
-        hipLaunchKernelGGL((mx_few_kernel<AF, false, 1>), dim3((unsigned)((a.rows + 15) / 16), tg), dim3(512), 0, st, a);
+        hipLaunchKernelGGL((mx_few_kernel<AF, false, 1>), dim3(tg * (unsigned)((a.rows + 15) / 16)), dim3(512), 0, st, a);
     return hipGetLastError();
 }
 
@@ -173,6 +166,8 @@ hipError_t few(const MxMatArgs& a, hipStream_t st) {
 
 hipError_t launch_mx_matmul(const MxMatArgs& a, hipStream_t st) {
     if (a.n <= 0 || a.rows <= 0) return hipSuccess;
+    // f32 sums of 8 bit codes: the bf16 MFMA's
+    if (a.n > 16 && (a.gated || a.bf16 || a.act.format == MX_E2M1)) return launch_mx_tile(a, st);
     return a.act.format == MX_E2M1 ? few<MX_E2M1>(a, st) : few<MX_E4M3>(a, st);
 }
 

@@ -1,0 +1,307 @@
+// mx_tile.hip -- products of E2M1 weights with microscaled activations, many
+// rows: tiles staged through LDS, the block-scaled MFMA.
+//
+// v_mfma_scale_f32_16x16x128_f8f6f4 multiplies 16 x 128 by 128 x 16 codes, each
+// 32 of a row scaled by a power of two: no value is unpacked.  Lane (r, g) =
+// (lane % 16, lane / 16) holds of row r: 4 bit codes: block g (16 bytes); 8 bit
+// codes: values 16 g .. 16 g + 15 and 64 more (the 16-byte pieces g and 4 + g of
+// the 128); and block g's scale byte.  The weights are the A operand, so a lane's
+// four sums are consecutive output columns of one activation row.
+//
+// A workgroup's tile of BM weight rows by BN activation rows goes over the
+// columns in steps of 128.  Codes and scales of a step come by LDS DMA, 16 bytes
+// (codes) or four scale bytes a lane, STAGES - 1 steps ahead; columns behind a
+// row's end and rows behind the last are out of the buffer's range and read as 0
+// codes.
+#include "mx_common.hpp"
+
+namespace dr {
+namespace {
+
+using i32x8m = int __attribute__((ext_vector_type(8)));
+
+constexpr int OUT_OF_RANGE = 1 << 30;  // past every tile's bytes (256 rows of 2^21 at most)
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_rsrc(const void* base, size_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, (int)bytes, 0x00020000);
+}
+// lane i: 16 (4) bytes at rsrc + voff + soff -> LDS byte address lds + 16 (4) i.  Inline
+// asm without outputs, so that the compiler does not make every LDS read wait for it;
+// the kernel's own waits order them.  (M0 needs a wait state; nothing else here uses it.)
+__device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t r, uint32_t lds, int voff, int soff) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(voff), "s"(r), "s"(soff)
+                 : "memory");
+#endif
+}
+__device__ __forceinline__ void dma4(__amdgpu_buffer_rsrc_t r, uint32_t lds, int voff, int soff) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds" ::"s"(lds), "v"(voff), "s"(r), "s"(soff)
+                 : "memory");
+#endif
+}
+template <int N>
+__device__ __forceinline__ void wait_vm() {
+    static_assert(N >= 0 && N < 64, "vmcnt");
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void barrier_lds() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// A workgroup of WM x WN waves, each with Q groups of 64 weight rows by TN tiles
+// of 16 activation rows.  Group q of a wave is rows of `w` (gated: odd groups
+// are rows of `up`, of the same output columns as the group before).  Tile i, row
+// 4 g + e of a group is its weight row 16 g + 4 i + e, so that lane group g's sums
+// over the four tiles are 16 consecutive output columns.
+template <int AF_, bool GATED_, int WM_, int Q_, int WN_, int TN_, int STAGES_>
+struct TileGeom {
+    static constexpr int AF = AF_, WM = WM_, Q = Q_, WN = WN_, TN = TN_, STAGES = STAGES_;
+    static constexpr bool GATED = GATED_;
+    static constexpr int WAVES = WM * WN, THREADS = 64 * WAVES;
+    static constexpr int GROUPS = WM * Q;                     // of 64 weight rows
+    static constexpr int COLS = GROUPS * 64 / (GATED ? 2 : 1);  // output columns
+    static constexpr int BN = WN * TN * 16;
+    static constexpr int ROW_B = AF == MX_E4M3 ? 128 : 64;    // bytes of an activation row and step
+    static constexpr int W_BYTES = GROUPS * 64 * 64, A_BYTES = BN * ROW_B;
+    static constexpr int NW = W_BYTES / 1024, NA = A_BYTES / 1024;  // DMA instructions of a step
+    static constexpr int NSW = GROUPS, NSA = (BN + 63) / 64;        // of its scales
+    static constexpr int NI_W = NW / WAVES, NI_A = NA / WAVES;
+    static constexpr int NI_S = (NSW + NSA + WAVES - 1) / WAVES, NI = NI_W + NI_A + NI_S;  // of a wave
+    static constexpr int S_OFF = W_BYTES + A_BYTES, STAGE = S_OFF + NI_S * WAVES * 256;
+    static constexpr int LDS = STAGE * STAGES;
+    static_assert(NW % WAVES == 0 && NA % WAVES == 0, "every wave issues the same number");
+    static_assert(!GATED || Q % 2 == 0, "gate and up groups pair up in a wave");
+    static_assert(LDS <= 160 * 1024, "LDS");
+};
+
+template <class G>
+__global__ __launch_bounds__(G::THREADS, 512 / G::THREADS * 2) void mx_tile_kernel(const MxMatArgs a, int n_m, int n_n) {
+    extern __shared__ __align__(16) uint8_t s_mem[];
+    constexpr int AF = G::AF, Q = G::Q, TN = G::TN;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r = lane & 15, g = lane >> 4;
+    // Workgroups go to the 8 XCDs in turn: each XCD takes a run of tiles, 4 along
+    // the weights by as many as there are along the activations, whose rows its L2
+    // then holds.
+    int mt, nt;
+    {
+        const int total = n_m * n_n, id = blockIdx.x, x = id & 7, per = total >> 3, rest = total & 7;
+        const int lin = x * per + min(x, rest) + (id >> 3);
+        const int band = lin / (4 * n_n), in = lin - band * 4 * n_n, wide = min(4, n_m - 4 * band);
+        nt = __builtin_amdgcn_readfirstlane(in / wide);  // (divided on the vector unit)
+        mt = __builtin_amdgcn_readfirstlane(4 * band + in - nt * wide);
+    }
+    const int nblk = a.cols / 32, steps = (nblk + 3) / 4;
+    const int pitch = (int)mx_pitch(a.cols), w_row = a.cols / 2, a_row = (int)mx_row_bytes(AF, a.cols);
+    const int col0 = mt * G::COLS, tok0 = nt * G::BN;
+
+    const int cols_in = min(G::COLS, a.rows - col0), toks_in = min(G::BN, a.n - tok0);
+    // first output column (within the tile) of weight group q
+    auto group_col = [](int q) { return G::GATED ? (q >> 1) * 64 : q * 64; };
+    // 16-byte pieces of a step.  64-byte rows: piece c of row R lies at slot c ^ (R / 4 % 4),
+    // 128-byte rows: at c ^ (R / 2 % 8): 16 lanes of a read touch every bank once.
+    // (buffers over the tile's rows; an instruction's is the wave's own choice)
+    __amdgpu_buffer_rsrc_t rw[G::NI_W], rs[G::NI_S];
+    const __amdgpu_buffer_rsrc_t ra = tile_rsrc(a.act.codes + (size_t)tok0 * a_row, (size_t)toks_in * a_row);
+    int vw[G::NI_W], bw[G::NI_W], va[G::NI_A], ba[G::NI_A];
+#pragma unroll
+    for (int k = 0; k < G::NI_W; ++k) {  // instruction j: tile j % 4 of group j / 4
+        const int j = wave * G::NI_W + k, R = lane >> 2, c = (lane & 3) ^ ((R >> 2) & 3);
+        const int row = group_col(j >> 2) + 16 * (R >> 2) + 4 * (j & 3) + (R & 3);
+        vw[k] = row * w_row + c * 16;
+        bw[k] = c;
+        rw[k] = tile_rsrc((G::GATED && (j & 4) ? a.up.codes : a.w.codes) + (size_t)col0 * w_row, (size_t)cols_in * w_row);
+    }
+#pragma unroll
+    for (int k = 0; k < G::NI_A; ++k) {
+        const int j = wave * G::NI_A + k;
+        if constexpr (AF == MX_E4M3) {  // 8 rows
+            const int R = j * 8 + (lane >> 3), c = (lane & 7) ^ ((R >> 1) & 7);
+            va[k] = R * a_row + c * 16;
+            ba[k] = c >> 1;
+        } else {  // 16 rows
+            const int R = j * 16 + (lane >> 2), c = (lane & 3) ^ ((R >> 2) & 3);
+            va[k] = R * a_row + c * 16;
+            ba[k] = c;
+        }
+    }
+    // scales: instruction j < NSW: group j's, dword r * 4 + i that of tile i, row r; then
+    // 64 activation rows' in the same order
+    int vs[G::NI_S];
+#pragma unroll
+    for (int k = 0; k < G::NI_S; ++k) {
+        const int j = wave * G::NI_S + k, R = lane >> 2, i = lane & 3;
+        vs[k] = j < G::NSW ? (group_col(j) + 16 * (R >> 2) + 4 * i + (R & 3)) * pitch : ((j - G::NSW) * 64 + i * 16 + R) * pitch;
+        if (j >= G::NSW && (j - G::NSW) * 64 + i * 16 + R >= G::BN) vs[k] = OUT_OF_RANGE;  // (every wave issues the same number)
+        const uint8_t* const base = j >= G::NSW ? a.act.scales : G::GATED && (j & 1) ? a.up.scales : a.w.scales;
+        rs[k] = tile_rsrc(base + (size_t)(j >= G::NSW ? tok0 : col0) * pitch, (size_t)(j >= G::NSW ? toks_in : cols_in) * pitch);
+    }
+
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)s_mem;
+    auto request = [&](int t, uint32_t at) __attribute__((always_inline)) {
+        const int left = nblk - 4 * t;  // blocks from here on (none: every lane out of range)
+#pragma unroll
+        for (int k = 0; k < G::NI_W; ++k)
+            dma16(rw[k], at + (wave * G::NI_W + k) * 1024, bw[k] < left ? vw[k] : OUT_OF_RANGE, t * 64);
+#pragma unroll
+        for (int k = 0; k < G::NI_A; ++k)
+            dma16(ra, at + G::W_BYTES + (wave * G::NI_A + k) * 1024, ba[k] < left ? va[k] : OUT_OF_RANGE, t * G::ROW_B);
+#pragma unroll
+        for (int k = 0; k < G::NI_S; ++k)
+            dma4(rs[k], at + G::S_OFF + (wave * G::NI_S + k) * 256, left > 0 ? vs[k] : OUT_OF_RANGE, t * 4);
+    };
+    const int wm = wave % G::WM, wn = wave / G::WM;
+    f32x4m acc[Q][4][TN] = {};
+    // byte offsets of this wave's operands within a stage
+    const int at_w = wm * Q * 4096 + r * 64 + ((g ^ ((r >> 2) & 3)) * 16);
+    const int at_a = AF == MX_E4M3 ? G::W_BYTES + wn * TN * 2048 + r * 128 + ((g ^ ((r >> 1) & 7)) * 16)
+                                   : G::W_BYTES + wn * TN * 1024 + r * 64 + ((g ^ ((r >> 2) & 3)) * 16);
+    const int at_sw = G::S_OFF + wm * Q * 256 + r * 16;
+    const int at_sa = G::S_OFF + G::NSW * 256 + (wn * TN / 4) * 256 + r * 16 + (wn * TN % 4) * 4;
+
+    auto multiply = [&](int t, const uint8_t* st) __attribute__((always_inline)) {
+        // the scale byte of block g; behind a row's last block the codes are 0 and so is this
+        const uint32_t sel = 4 * t + g < nblk ? 0x0c0c0c00u | g : 0x0c0c0c0cu;
+        i32x8m oa[TN];
+        uint32_t sa[TN];
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+            const u32x4m lo = *reinterpret_cast<const u32x4m*>(st + at_a + j * 16 * G::ROW_B);
+            oa[j] = i32x8m{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], 0, 0, 0, 0};
+            if constexpr (AF == MX_E4M3) {
+                const u32x4m hi = *reinterpret_cast<const u32x4m*>(st + (at_a ^ 64) + j * 16 * G::ROW_B);
+                oa[j][4] = (int)hi[0], oa[j][5] = (int)hi[1], oa[j][6] = (int)hi[2], oa[j][7] = (int)hi[3];
+            }
+            sa[j] = __builtin_amdgcn_perm(0, *reinterpret_cast<const uint32_t*>(st + at_sa + j * 4), sel);
+        }
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+            const u32x4m s4 = *reinterpret_cast<const u32x4m*>(st + at_sw + q * 256);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const u32x4m w = *reinterpret_cast<const u32x4m*>(st + at_w + q * 4096 + i * 1024);
+                const i32x8m ow = i32x8m{(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
+                const int sw = (int)__builtin_amdgcn_perm(0, s4[i], sel);
+#pragma unroll
+                for (int j = 0; j < TN; ++j)
+                    acc[q][i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(ow, oa[j], acc[q][i][j], 4, AF == MX_E4M3 ? 0 : 4,
+                                                                                     0, sw, 0, (int)sa[j]);
+            }
+        }
+    };
+
+#pragma unroll
+    for (int s = 0; s < G::STAGES - 1; ++s) request(s, lds0 + s * G::STAGE);
+    int cur = 0;
+    for (int t = 0; t < steps; ++t) {
+        // this wave's pieces of step t are there; behind the barrier everybody's, and
+        // everybody has read step t - 1, whose place is free
+        wait_vm<(G::STAGES - 2) * G::NI>();
+        barrier_lds();
+        const int next = cur == 0 ? G::STAGES - 1 : cur - 1;
+        request(t + G::STAGES - 1, lds0 + next * G::STAGE);
+        multiply(t, s_mem + cur * G::STAGE);
+        cur = cur == G::STAGES - 1 ? 0 : cur + 1;
+    }
+    wait_vm<0>();
+
+    // lane (r, g): activation row r of each tile, 16 columns of each group
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+        const int tok = tok0 + (wn * TN + j) * 16 + r;
+        if constexpr (!G::GATED) {
+#pragma unroll
+            for (int q = 0; q < Q; ++q) {
+                const int c0 = col0 + (wm * Q + q) * 64 + 16 * g;
+                if (tok >= a.n || c0 >= a.rows) continue;
+                const size_t at = (size_t)tok * a.rows + c0;
+                const int in = min(16, a.rows - c0);
+                const bool whole = in == 16 && ((a.rows & 7) == 0) && a.vec;
+#pragma unroll
+                for (int i = 0; i < 4; i += 2) {
+                    float x[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[e] = acc[q][i + e / 4][j][e % 4];
+                    if (whole) {
+                        float y[8];
+                        if (a.bf16) {
+                            if (a.residual) {
+                                load8<true>(a.residual, at + 4 * i, y);
+#pragma unroll
+                                for (int e = 0; e < 8; ++e) x[e] += y[e];
+                            }
+                            store8<true>(a.out, at + 4 * i, x);
+                        } else {
+                            if (a.residual) {
+                                load8<false>(a.residual, at + 4 * i, y);
+#pragma unroll
+                                for (int e = 0; e < 8; ++e) x[e] += y[e];
+                            }
+                            store8<false>(a.out, at + 4 * i, x);
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            if (4 * i + e < in) put_sum(a, at + 4 * i + e, x[e]);
+                    }
+                }
+            }
+        } else {
+#pragma unroll
+            for (int q = 0; q < Q; q += 2) {
+                const int c0 = col0 + (wm * Q + q) / 2 * 64 + 16 * g;
+                float x[2][8];
+                uint32_t m = 0;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const float v = mx_act(acc[q][e / 4][j][e % 4], a.fn) * acc[q + 1][e / 4][j][e % 4];
+                    x[e / 8][e % 8] = v;
+                    m = max(m, __float_as_uint(v) & 0x7fffffffu);
+                }
+                m = max(m, (uint32_t)__shfl_xor((int)m, 16));  // a block: 16 columns of two lane groups
+                if (tok >= a.n || c0 >= a.rows) continue;
+                uint8_t* const to = a.hidden.codes + (size_t)tok * mx_row_bytes(a.hidden.format, a.rows);
+                int byte;
+                if (a.hidden.format == MX_E2M1) {
+                    byte = mx_scale_byte<MX_E2M1>(m);
+                    *reinterpret_cast<u32x2m*>(to + c0 / 2) = u32x2m{mx_encode8<MX_E2M1>(x[0], byte)[0], mx_encode8<MX_E2M1>(x[1], byte)[0]};
+                } else {
+                    byte = mx_scale_byte<MX_E4M3>(m);
+                    const u32x2m lo = mx_encode8<MX_E4M3>(x[0], byte), hi = mx_encode8<MX_E4M3>(x[1], byte);
+                    *reinterpret_cast<u32x4m*>(to + c0) = u32x4m{lo[0], lo[1], hi[0], hi[1]};
+                }
+                if ((g & 1) == 0) a.hidden.scales[(size_t)tok * mx_pitch(a.rows) + c0 / 32] = (uint8_t)byte;
+            }
+        }
+    }
+}
+
+template <class G>
+hipError_t tile(const MxMatArgs& a, hipStream_t st) {
+    const int n_m = (a.rows + G::COLS - 1) / G::COLS, n_n = (a.n + G::BN - 1) / G::BN;
+    const hipError_t e =
+        hipFuncSetAttribute(reinterpret_cast<const void*>(mx_tile_kernel<G>), hipFuncAttributeMaxDynamicSharedMemorySize, G::LDS);
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL((mx_tile_kernel<G>), dim3((unsigned)(n_m * n_n)), dim3(G::THREADS), G::LDS, st, a, n_m, n_n);
+    return hipGetLastError();
+}
+
+template <int AF, bool GATED>
+hipError_t tiles(const MxMatArgs& a, hipStream_t st) {
+    constexpr int BIG = AF == MX_E4M3 ? 3 : 4;
+    const long cols = GATED ? 2l * a.rows : a.rows;
+    const long big = (cols + 255) / 256 * ((a.n + 255) / 256);
+    if (big >= a.n_cu / 2) return tile<TileGeom<AF, GATED, 2, 2, 4, 4, BIG>>(a, st);
+    if constexpr (GATED)
+        return tile<TileGeom<AF, GATED, 1, 2, 4, 2, 3>>(a, st);
+    else
+        return tile<TileGeom<AF, GATED, 1, 1, 4, 1, 4>>(a, st);
+}
+
+}  // namespace
+
+hipError_t launch_mx_tile(const MxMatArgs& a, hipStream_t st) {
+    if (a.act.format == MX_E4M3) return a.gated ? tiles<MX_E4M3, true>(a, st) : tiles<MX_E4M3, false>(a, st);
+    return a.gated ? tiles<MX_E2M1, true>(a, st) : tiles<MX_E2M1, false>(a, st);
+}
+
+}  // namespace dr
