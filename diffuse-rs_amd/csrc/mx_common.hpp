@@ -1,5 +1,5 @@
 // mx_common.hpp -- microscaled rows (dr_mx_rows), shared by mx_rows.hip
-// (quantisation, norm) and the products of mx_few.hip and mx_tile.hip.
+// (quantisation, norm) and the products of mx_ring.hip and mx_tile.hip.
 //
 // 32 consecutive values of a row are a block: they share 2^e, held as the byte
 // e + 127 (255: the whole block stands for NaN), and each is an E2M1 (4 bit) or
@@ -88,6 +88,20 @@ __device__ __forceinline__ void mx_decode8(u32x2m c, int byte, float (&x)[8]) {
     for (int i = 0; i < 8; ++i) x[i] = p[i / 2][i % 2] * s;
 }
 
+// The codes of 4 values: 2 bytes (E2M1) or 4.
+template <int FMT>
+__device__ __forceinline__ uint32_t mx_encode4(const float (&x)[4], int byte) {
+    if (byte == MX_NAN) return 0;
+    if constexpr (FMT == MX_E2M1) {
+        const float s = __uint_as_float((uint32_t)byte << 23);
+        return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(__builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0, x[0], x[1], s, 0), x[2], x[3], s, 1);
+    } else {
+        const float inv = __uint_as_float((uint32_t)(254 - byte) << 23);
+        const int w = __builtin_amdgcn_cvt_pk_fp8_f32(x[0] * inv, x[1] * inv, 0, false);
+        return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[2] * inv, x[3] * inv, w, true);
+    }
+}
+
 // The largest of a value over a quad of lanes.
 __device__ __forceinline__ uint32_t quad_max(uint32_t v) {
     v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xf, 0xf, true));  // lanes 1 0 3 2
@@ -130,6 +144,59 @@ __device__ __forceinline__ void store8(void* base, size_t at, const float (&x)[8
 __device__ __forceinline__ float mx_act(float x, int fn) {
     const float z = fn == MX_SILU ? x : 1.5957691216057308f * (x + 0.044715f * x * x * x);
     return x / (1.0f + expf(-z));
+}
+
+// ---- staging through LDS (mx_ring.hip, mx_tile.hip)
+
+using i32x8m = int __attribute__((ext_vector_type(8)));
+
+constexpr int OUT_OF_RANGE = 1 << 30;  // at or past every tile's end (256 rows of 2^22 bytes at most)
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_rsrc(const void* base, size_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, (int)bytes, 0x00020000);
+}
+// lane i: 16 (4) bytes at rsrc + voff + soff -> LDS byte address lds + 16 (4) i; 0 where voff
+// lies past the buffer's end.  Inline asm without outputs, so that the compiler does not
+// make every LDS read wait for it; the kernels' own waits order them.  (M0 needs a wait
+// state; nothing else here uses it.)
+__device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t r, uint32_t lds, int voff, int soff) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(voff), "s"(r), "s"(soff)
+                 : "memory");
+#endif
+}
+__device__ __forceinline__ void dma4(__amdgpu_buffer_rsrc_t r, uint32_t lds, int voff, int soff) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds" ::"s"(lds), "v"(voff), "s"(r), "s"(soff)
+                 : "memory");
+#endif
+}
+template <int N>
+__device__ __forceinline__ void wait_vm() {
+    static_assert(N >= 0 && N < 64, "vmcnt");
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+// this wave's LDS reads and writes are done
+__device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+// a barrier that leaves LDS DMA in flight
+__device__ __forceinline__ void barrier_lds() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+__device__ __forceinline__ uint32_t lds_address(const void* p) {
+    return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t*)p;
+}
+
+// Place in the order of tiles of workgroup id of `total`: workgroups go to the 8 XCDs
+// in turn, and each XCD takes a run of consecutive places, whose operands its L2 shares.
+__device__ __forceinline__ int xcd_order(int id, int total) {
+    const int x = id & 7, per = total >> 3, rest = total & 7;
+    return x * per + min(x, rest) + (id >> 3);
+}
+
+// 16-byte piece c of row R of a staged tile lies at slot c ^ turn(R): the 16 lanes that
+// read a piece of 16 rows together then touch every bank once.  ROW: bytes of a row,
+// 64, 128 or 256.
+template <int ROW>
+__device__ __forceinline__ int turn(int R) {
+    return ROW == 64 ? (R >> 2) & 3 : ROW == 128 ? (R >> 1) & 7 : R & 15;
 }
 
 // One sum of a product, with its residual, at element `at` of out.

@@ -1,0 +1,309 @@
+// mx_ring.hip -- products of E2M1 weights with microscaled activations, few rows:
+// a workgroup's waves share a strip of weight rows and up to 64 activation rows
+// and split the columns; each wave streams its own part through LDS, and the
+// sums are joined there at the end, in a fixed order.
+//
+// With few rows the weights' bytes bound the product, or the latency of the few
+// steps a workgroup takes: what counts is how many bytes are under way.  Each wave
+// keeps STAGES - 1 steps of weights, activations and scales in flight by LDS DMA
+// (whole rows of 64 or 128 bytes, consecutive lanes on consecutive bytes), waits for
+// nobody but its own loads and meets the others once, at the end.
+//
+// EXACT: both operands are turned into bf16, which holds every code times its
+// power of two exactly, and multiplied by the bf16 MFMA, whose sums keep f32's
+// bits: the block-scaled MFMA lines the products of a step up with the largest and
+// drops what lies about 2^19 below it (with 8 bit codes: relative errors of 4e-6 to
+// 5e-5 against 1e-7, measured over 4096 columns; none with 4 bit codes, whose
+// products span less).  Taken for f32 outputs, and wherever the conversions hide
+// behind the loads.  A product does not depend on the order of the columns, so
+// the MFMA's k index is whatever both operands agree on: lane group g takes block g
+// of a step's four, and instruction j multiplies the blocks' values 8 j .. 8 j + 7.
+#include "mx_common.hpp"
+
+namespace dr {
+namespace {
+
+__device__ __forceinline__ bf16x8m join(bf16x2 a, bf16x2 b, bf16x2 c, bf16x2 d) {
+    return bf16x8m{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+// A block's 32 values as four operands.
+__device__ __forceinline__ void operands4(const u32x4m& c, float s, bf16x8m (&o)[4]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        o[j] = join(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c[j], s, 0), __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c[j], s, 1),
+                    __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c[j], s, 2), __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c[j], s, 3));
+}
+__device__ __forceinline__ void operands8(const u32x4m (&c)[2], float s, bf16x8m (&o)[4]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const uint32_t a = c[j / 2][2 * (j & 1)], b = c[j / 2][2 * (j & 1) + 1];
+        o[j] = join(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, s, false), __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, s, true),
+                    __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, s, false), __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, s, true));
+    }
+}
+
+// MT tiles of 16 weight rows (gated: the first half of the gate, the second of the up
+// projection, of the same output columns) by NT tiles of 16 activation rows, of which
+// AR are staged (a multiple of 4; fewer than 16 with one tile); steps of SK * 128 columns.
+template <int AF_, bool GATED_, bool EXACT_, int MT_, int NT_, int AR_, int SK_, int STAGES_, int WAVES_>
+struct RingGeom {
+    static constexpr int AF = AF_, MT = MT_, NT = NT_, AR = AR_, SK = SK_, STAGES = STAGES_, WAVES = WAVES_;
+    static constexpr bool GATED = GATED_, EXACT = EXACT_;
+    static constexpr int FT = GATED ? MT / 2 : MT;  // tiles of output columns
+    static constexpr int W_ROW = SK * 64, A_ROW = SK * (AF == MX_E4M3 ? 128 : 64);  // bytes of a row and step
+    static constexpr int NW = MT * 16 * W_ROW / 1024;                               // DMA instructions of a step
+    static constexpr int NA = (AR * A_ROW + 1023) / 1024;
+    static constexpr int NSM = (FT * 16 * SK + 63) / 64;  // scales of one matrix
+    static constexpr int NSW = GATED ? 2 * NSM : NSM, NSA = (AR * SK + 63) / 64;
+    static constexpr int NI = NW + NA + NSW + NSA;
+    static constexpr int A_OFF = NW * 1024, SW_OFF = A_OFF + NA * 1024, SA_OFF = SW_OFF + NSW * 256, STAGE = SA_OFF + NSA * 256;
+    static constexpr int TILE = 16 * 20;  // floats of a tile of sums: rows of 16 and 4 apart
+    static constexpr int RING = STAGE * STAGES * WAVES, SUMS = WAVES * MT * NT * TILE * 4;
+    static constexpr int LDS = RING > SUMS ? RING : SUMS;
+    static_assert(LDS <= 160 * 1024, "LDS");
+    static_assert(!GATED || FT % 2 == 0, "whole blocks of output columns");
+    static_assert((STAGES - 1) * NI < 64, "vmcnt");
+    static_assert(NT * 16 == AR || (NT == 1 && (AR == 4 || AR == 8)), "staged rows");
+};
+
+template <class G>
+__global__ __launch_bounds__(64 * G::WAVES) void mx_ring_kernel(const MxMatArgs a, int groups) {
+    extern __shared__ __align__(16) uint8_t s_mem[];
+    constexpr int AF = G::AF, MT = G::MT, NT = G::NT, SK = G::SK, WAVES = G::WAVES;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r = lane & 15, g = lane >> 4;
+    // (an XCD takes a strip's groups of activation rows one after the other)
+    const int lin = xcd_order(blockIdx.x, gridDim.x), strip = __builtin_amdgcn_readfirstlane(lin / groups);
+    const int col0 = strip * G::FT * 16, tok0 = __builtin_amdgcn_readfirstlane(lin - strip * groups) * NT * 16;
+    const int nblk = a.cols / 32, steps = (nblk + 4 * SK - 1) / (4 * SK);
+    const int pitch = (int)mx_pitch(a.cols), w_row = a.cols / 2, a_row = (int)mx_row_bytes(AF, a.cols);
+    const int cols_in = min(G::FT * 16, a.rows - col0), toks_in = min(G::NT * 16, a.n - tok0);
+
+    const __amdgpu_buffer_rsrc_t rw = tile_rsrc(a.w.codes + (size_t)col0 * w_row, (size_t)cols_in * w_row);
+    const __amdgpu_buffer_rsrc_t rws = tile_rsrc(a.w.scales + (size_t)col0 * pitch, (size_t)cols_in * pitch);
+    const __amdgpu_buffer_rsrc_t ru = tile_rsrc((G::GATED ? a.up : a.w).codes + (size_t)col0 * w_row, (size_t)cols_in * w_row);
+    const __amdgpu_buffer_rsrc_t rus = tile_rsrc((G::GATED ? a.up : a.w).scales + (size_t)col0 * pitch, (size_t)cols_in * pitch);
+    const __amdgpu_buffer_rsrc_t ra = tile_rsrc(a.act.codes + (size_t)tok0 * a_row, (size_t)toks_in * a_row);
+    const __amdgpu_buffer_rsrc_t ras = tile_rsrc(a.act.scales + (size_t)tok0 * pitch, (size_t)toks_in * pitch);
+
+    // Lane addresses of a step's pieces (row in the strip, piece in the row).
+    constexpr int W_LANES = G::W_ROW / 16, A_LANES = G::A_ROW / 16;  // lanes of a row
+    constexpr int W_ROWS = 64 / W_LANES, A_ROWS = 64 / A_LANES;      // rows of an instruction
+    constexpr int NWM = G::FT * 16 / W_ROWS;                         // instructions of one matrix
+    int vw[NWM], bw[NWM], va[G::NA], ba[G::NA], vsw[G::NSM], vsa[G::NSA];
+#pragma unroll
+    for (int k = 0; k < NWM; ++k) {
+        const int R = k * W_ROWS % 16 + lane / W_LANES, c = (lane % W_LANES) ^ turn<G::W_ROW>(R);
+        vw[k] = (R + k * W_ROWS / 16 * 16) * w_row + c * 16;
+        bw[k] = c;
+    }
+#pragma unroll
+    for (int k = 0; k < G::NA; ++k) {
+        const int R = k * A_ROWS % 16 + lane / A_LANES, c = (lane % A_LANES) ^ turn<G::A_ROW>(R);
+        va[k] = R + k * A_ROWS / 16 * 16 < G::AR ? (R + k * A_ROWS / 16 * 16) * a_row + c * 16 : OUT_OF_RANGE;
+        ba[k] = AF == MX_E4M3 ? c >> 1 : c;
+    }
+    // scale bytes: dword SK * R + s is row R's of the step's 128 columns s
+    const int ss = lane % SK;
+#pragma unroll
+    for (int k = 0; k < G::NSM; ++k) {
+        const int R = (k * 64 + lane) / SK;
+        vsw[k] = R < G::FT * 16 ? R * pitch + ss * 4 : OUT_OF_RANGE;
+    }
+#pragma unroll
+    for (int k = 0; k < G::NSA; ++k) {
+        const int R = (k * 64 + lane) / SK;
+        vsa[k] = R < G::AR ? R * pitch + ss * 4 : OUT_OF_RANGE;
+    }
+    const uint32_t ring = lds_address(s_mem) + wave * G::STAGES * G::STAGE;
+    auto request = [&](int t, uint32_t at) __attribute__((always_inline)) {
+        const int left = nblk - 4 * SK * t;  // blocks from here on (none: every lane out of range)
+#pragma unroll
+        for (int k = 0; k < G::NW; ++k)
+            dma16(k >= NWM ? ru : rw, at + k * 1024, bw[k % NWM] < left ? vw[k % NWM] : OUT_OF_RANGE, t * G::W_ROW);
+#pragma unroll
+        for (int k = 0; k < G::NA; ++k) dma16(ra, at + G::A_OFF + k * 1024, ba[k] < left ? va[k] : OUT_OF_RANGE, t * G::A_ROW);
+#pragma unroll
+        for (int k = 0; k < G::NSW; ++k)
+            dma4(k >= G::NSM ? rus : rws, at + G::SW_OFF + k * 256, 4 * ss < left ? vsw[k % G::NSM] : OUT_OF_RANGE, t * SK * 4);
+#pragma unroll
+        for (int k = 0; k < G::NSA; ++k)
+            dma4(ras, at + G::SA_OFF + k * 256, 4 * ss < left ? vsa[k] : OUT_OF_RANGE, t * SK * 4);
+    };
+
+    f32x4m acc[MT][NT] = {};
+    auto multiply = [&](int t, const uint8_t* st) __attribute__((always_inline)) {
+#pragma unroll
+        for (int s = 0; s < SK; ++s) {
+            // the scale byte of block g; behind a row's last block the codes are 0 and so is this
+            const uint32_t sel = 4 * (SK * t + s) + g < nblk ? 0x0c0c0c00u | g : 0x0c0c0c0cu;
+            u32x4m ca[NT][AF == MX_E4M3 ? 2 : 1];
+            int sa[NT];
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                const int R = G::AR < 16 ? r & (G::AR - 1) : r;  // (the other rows' sums are not used)
+                const uint8_t* const row = st + G::A_OFF + (j * 16 + R) * G::A_ROW;
+                const int x = turn<G::A_ROW>(R);
+                if constexpr (AF == MX_E4M3) {
+                    const int c = 8 * s + (G::EXACT ? 2 * g : g);
+                    ca[j][0] = *reinterpret_cast<const u32x4m*>(row + (c ^ x) * 16);
+                    ca[j][1] = *reinterpret_cast<const u32x4m*>(row + ((c + (G::EXACT ? 1 : 4)) ^ x) * 16);
+                } else {
+                    ca[j][0] = *reinterpret_cast<const u32x4m*>(row + ((4 * s + g) ^ x) * 16);
+                }
+                sa[j] = (int)__builtin_amdgcn_perm(0, *reinterpret_cast<const uint32_t*>(st + G::SA_OFF + ((j * 16 + R) * SK + s) * 4), sel);
+            }
+            bf16x8m oa[NT][4];
+            if constexpr (G::EXACT) {
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    if constexpr (AF == MX_E4M3)
+                        operands8(ca[j], mx_scale(sa[j]), oa[j]);
+                    else
+                        operands4(ca[j][0], mx_scale(sa[j]), oa[j]);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                const u32x4m cw =
+                    *reinterpret_cast<const u32x4m*>(st + (i * 16 + r) * G::W_ROW + ((4 * s + g) ^ turn<G::W_ROW>(r)) * 16);
+                const int sw = (int)__builtin_amdgcn_perm(
+                    0, *reinterpret_cast<const uint32_t*>(st + G::SW_OFF + i / G::FT * G::NSM * 256 + ((i % G::FT * 16 + r) * SK + s) * 4), sel);
+                if constexpr (G::EXACT) {
+                    bf16x8m ow[4];
+                    operands4(cw, mx_scale(sw), ow);
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+#pragma unroll
+                        for (int j = 0; j < NT; ++j)
+                            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ow[q], oa[j][q], acc[i][j], 0, 0, 0);
+                } else {
+                    const i32x8m ow = i32x8m{(int)cw[0], (int)cw[1], (int)cw[2], (int)cw[3], 0, 0, 0, 0};
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) {
+                        const u32x4m &lo = ca[j][0], &hi = ca[j][AF == MX_E4M3 ? 1 : 0];
+                        const i32x8m o = AF == MX_E4M3 ? i32x8m{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]}
+                                                       : i32x8m{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], 0, 0, 0, 0};
+                        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(ow, o, acc[i][j], 4, AF == MX_E4M3 ? 0 : 4, 0, sw, 0, sa[j]);
+                    }
+                }
+            }
+        }
+    };
+
+    // wave w takes steps w, w + WAVES, ...
+#pragma unroll
+    for (int s = 0; s < G::STAGES - 1; ++s) request(wave + s * WAVES, ring + s * G::STAGE);
+    int cur = 0;
+    for (int t = wave; t < steps; t += WAVES) {
+        const int next = cur == 0 ? G::STAGES - 1 : cur - 1;
+        wait_lds();  // the step before this one has been read: its place is free
+        request(t + (G::STAGES - 1) * WAVES, ring + next * G::STAGE);
+        wait_vm<(G::STAGES - 1) * G::NI>();
+        multiply(t, s_mem + (wave * G::STAGES + cur) * G::STAGE);
+        cur = cur == G::STAGES - 1 ? 0 : cur + 1;
+    }
+    wait_vm<0>();
+    barrier_lds();  // no wave reads or fills the rings any more
+
+    // lane (r, g) holds weight rows 4 g .. 4 g + 3 of each tile for activation row r
+    float* const s_sum = reinterpret_cast<float*>(s_mem);
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+            *reinterpret_cast<f32x4m*>(s_sum + ((wave * MT + i) * NT + j) * G::TILE + r * 20 + 4 * g) = acc[i][j];
+    barrier_lds();
+    auto total = [&](int tile, int quad, int t) __attribute__((always_inline)) {
+        f32x4m x = {0, 0, 0, 0};
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w)
+            x = x + *reinterpret_cast<const f32x4m*>(s_sum + ((w * MT + tile) * NT + t / 16) * G::TILE + t % 16 * 20 + 4 * quad);
+        return x;
+    };
+    constexpr int QUADS = G::FT * 4;
+    for (int e = threadIdx.x; e < QUADS * NT * 16; e += 64 * WAVES) {  // (whole waves)
+        const int f = e % QUADS, t = e / QUADS, c0 = col0 + 4 * f, tok = tok0 + t;
+        const f32x4m x = total(f / 4, f % 4, t);
+        const bool in = tok < a.n && c0 < a.rows;
+        if constexpr (!G::GATED) {
+            if (!in) continue;
+            const size_t at = (size_t)tok * a.rows + c0;
+            if (a.vec && (a.rows & 3) == 0) {
+                f32x4m y = x;
+                if (a.bf16) {
+                    if (a.residual) {
+                        const u32x2m v = *reinterpret_cast<const u32x2m*>(static_cast<const uint16_t*>(a.residual) + at);
+                        y = y + f32x4m{mx_f32(v[0] & 0xffff), __uint_as_float(v[0] & 0xffff0000u), mx_f32(v[1] & 0xffff),
+                                       __uint_as_float(v[1] & 0xffff0000u)};
+                    }
+                    *reinterpret_cast<u32x2m*>(static_cast<uint16_t*>(a.out) + at) =
+                        u32x2m{mx_bf16(y[0]) | (uint32_t)mx_bf16(y[1]) << 16, mx_bf16(y[2]) | (uint32_t)mx_bf16(y[3]) << 16};
+                } else {
+                    if (a.residual) y = y + *reinterpret_cast<const f32x4m*>(static_cast<const float*>(a.residual) + at);
+                    *reinterpret_cast<f32x4m*>(static_cast<float*>(a.out) + at) = y;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (c0 + i < a.rows) put_sum(a, at + i, x[i]);
+            }
+        } else {
+            const f32x4m u = total(G::FT + f / 4, f % 4, t);
+            float v[4];
+            uint32_t m = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                v[i] = mx_act(x[i], a.fn) * u[i];
+                m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+            }
+            m = quad_max(m);
+            m = max(m, (uint32_t)__shfl_xor((int)m, 4));  // a block: 8 lanes' 32 columns
+            if (!in) continue;
+            uint8_t* const to = a.hidden.codes + (size_t)tok * mx_row_bytes(a.hidden.format, a.rows);
+            int byte;
+            if (a.hidden.format == MX_E2M1) {
+                byte = mx_scale_byte<MX_E2M1>(m);
+                *reinterpret_cast<uint16_t*>(to + c0 / 2) = (uint16_t)mx_encode4<MX_E2M1>(v, byte);
+            } else {
+                byte = mx_scale_byte<MX_E4M3>(m);
+                *reinterpret_cast<uint32_t*>(to + c0) = mx_encode4<MX_E4M3>(v, byte);
+            }
+            if ((f & 7) == 0) a.hidden.scales[(size_t)tok * mx_pitch(a.rows) + c0 / 32] = (uint8_t)byte;
+        }
+    }
+}
+
+template <class G>
+hipError_t ring(const MxMatArgs& a, hipStream_t st) {
+    const int groups = (a.n + G::NT * 16 - 1) / (G::NT * 16), strips = (a.rows + G::FT * 16 - 1) / (G::FT * 16);
+    const hipError_t e =
+        hipFuncSetAttribute(reinterpret_cast<const void*>(mx_ring_kernel<G>), hipFuncAttributeMaxDynamicSharedMemorySize, G::LDS);
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL((mx_ring_kernel<G>), dim3((unsigned)groups * strips), dim3(64 * G::WAVES), G::LDS, st, a, groups);
+    return hipGetLastError();
+}
+
+//                  AF, gated, exact, MT, NT, AR, SK, STAGES, WAVES
+template <int AF>
+hipError_t few(const MxMatArgs& a, hipStream_t st) {
+    constexpr bool X = AF == MX_E4M3;
+    if (a.gated) {
+        if (a.n <= 4) return ring<RingGeom<AF, true, X, 4, 1, 4, 2, 3, 4>>(a, st);
+        return ring<RingGeom<AF, true, X, 4, 1, 16, 2, 3, 4>>(a, st);
+    }
+    if (a.n <= 4) return ring<RingGeom<AF, false, X, 1, 1, 4, 2, 4, 8>>(a, st);
+    if (a.n <= 16) return ring<RingGeom<AF, false, X, 1, 1, 16, 2, 2, 8>>(a, st);
+    return ring<RingGeom<AF, false, X, 4, 4, 64, 1, 3, 4>>(a, st);
+}
+
+}  // namespace
+
+hipError_t launch_mx_matmul(const MxMatArgs& a, hipStream_t st) {
+    if (a.n <= 0 || a.rows <= 0) return hipSuccess;
+    // f32 sums of 8 bit codes: the bf16 MFMA's
+    if (a.n > 16 && (a.gated || a.bf16 || a.act.format == MX_E2M1)) return launch_mx_tile(a, st);
+    return a.act.format == MX_E2M1 ? few<MX_E2M1>(a, st) : few<MX_E4M3>(a, st);
+}
+
+}  // namespace dr

@@ -18,35 +18,6 @@
 namespace dr {
 namespace {
 
-using i32x8m = int __attribute__((ext_vector_type(8)));
-
-constexpr int OUT_OF_RANGE = 1 << 30;  // past every tile's bytes (256 rows of 2^21 at most)
-
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_rsrc(const void* base, size_t bytes) {
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, (int)bytes, 0x00020000);
-}
-// lane i: 16 (4) bytes at rsrc + voff + soff -> LDS byte address lds + 16 (4) i.  Inline
-// asm without outputs, so that the compiler does not make every LDS read wait for it;
-// the kernel's own waits order them.  (M0 needs a wait state; nothing else here uses it.)
-__device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t r, uint32_t lds, int voff, int soff) {
-#if defined(__HIP_DEVICE_COMPILE__)
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(voff), "s"(r), "s"(soff)
-                 : "memory");
-#endif
-}
-__device__ __forceinline__ void dma4(__amdgpu_buffer_rsrc_t r, uint32_t lds, int voff, int soff) {
-#if defined(__HIP_DEVICE_COMPILE__)
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds" ::"s"(lds), "v"(voff), "s"(r), "s"(soff)
-                 : "memory");
-#endif
-}
-template <int N>
-__device__ __forceinline__ void wait_vm() {
-    static_assert(N >= 0 && N < 64, "vmcnt");
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
-}
-__device__ __forceinline__ void barrier_lds() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
-
 // A workgroup of WM x WN waves, each with Q groups of 64 weight rows by TN tiles
 // of 16 activation rows.  Group q of a wave is rows of `w` (gated: odd groups
 // are rows of `up`, of the same output columns as the group before).  Tile i, row
@@ -79,14 +50,10 @@ __global__ __launch_bounds__(G::THREADS, 512 / G::THREADS * 2) void mx_tile_kern
     constexpr int AF = G::AF, Q = G::Q, TN = G::TN;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, g = lane >> 4;
-    // Workgroups go to the 8 XCDs in turn: each XCD takes a run of tiles, 4 along
-    // the weights by as many as there are along the activations, whose rows its L2
-    // then holds.
+    // an XCD's run of tiles: 4 along the weights by as many as there are along the activations
     int mt, nt;
     {
-        const int total = n_m * n_n, id = blockIdx.x, x = id & 7, per = total >> 3, rest = total & 7;
-        const int lin = x * per + min(x, rest) + (id >> 3);
-        const int band = lin / (4 * n_n), in = lin - band * 4 * n_n, wide = min(4, n_m - 4 * band);
+        const int lin = xcd_order(blockIdx.x, n_m * n_n), band = lin / (4 * n_n), in = lin - band * 4 * n_n, wide = min(4, n_m - 4 * band);
         nt = __builtin_amdgcn_readfirstlane(in / wide);  // (divided on the vector unit)
         mt = __builtin_amdgcn_readfirstlane(4 * band + in - nt * wide);
     }
@@ -97,15 +64,13 @@ __global__ __launch_bounds__(G::THREADS, 512 / G::THREADS * 2) void mx_tile_kern
     const int cols_in = min(G::COLS, a.rows - col0), toks_in = min(G::BN, a.n - tok0);
     // first output column (within the tile) of weight group q
     auto group_col = [](int q) { return G::GATED ? (q >> 1) * 64 : q * 64; };
-    // 16-byte pieces of a step.  64-byte rows: piece c of row R lies at slot c ^ (R / 4 % 4),
-    // 128-byte rows: at c ^ (R / 2 % 8): 16 lanes of a read touch every bank once.
-    // (buffers over the tile's rows; an instruction's is the wave's own choice)
+    // 16-byte pieces of a step (buffers over the tile's rows; an instruction's is the wave's own choice)
     __amdgpu_buffer_rsrc_t rw[G::NI_W], rs[G::NI_S];
     const __amdgpu_buffer_rsrc_t ra = tile_rsrc(a.act.codes + (size_t)tok0 * a_row, (size_t)toks_in * a_row);
     int vw[G::NI_W], bw[G::NI_W], va[G::NI_A], ba[G::NI_A];
 #pragma unroll
     for (int k = 0; k < G::NI_W; ++k) {  // instruction j: tile j % 4 of group j / 4
-        const int j = wave * G::NI_W + k, R = lane >> 2, c = (lane & 3) ^ ((R >> 2) & 3);
+        const int j = wave * G::NI_W + k, R = lane >> 2, c = (lane & 3) ^ turn<64>(R);
         const int row = group_col(j >> 2) + 16 * (R >> 2) + 4 * (j & 3) + (R & 3);
         vw[k] = row * w_row + c * 16;
         bw[k] = c;
@@ -115,11 +80,11 @@ __global__ __launch_bounds__(G::THREADS, 512 / G::THREADS * 2) void mx_tile_kern
     for (int k = 0; k < G::NI_A; ++k) {
         const int j = wave * G::NI_A + k;
         if constexpr (AF == MX_E4M3) {  // 8 rows
-            const int R = j * 8 + (lane >> 3), c = (lane & 7) ^ ((R >> 1) & 7);
+            const int R = j * 8 + (lane >> 3), c = (lane & 7) ^ turn<128>(R);
             va[k] = R * a_row + c * 16;
             ba[k] = c >> 1;
         } else {  // 16 rows
-            const int R = j * 16 + (lane >> 2), c = (lane & 3) ^ ((R >> 2) & 3);
+            const int R = j * 16 + (lane >> 2), c = (lane & 3) ^ turn<64>(R);
             va[k] = R * a_row + c * 16;
             ba[k] = c;
         }
@@ -136,7 +101,7 @@ __global__ __launch_bounds__(G::THREADS, 512 / G::THREADS * 2) void mx_tile_kern
         rs[k] = tile_rsrc(base + (size_t)(j >= G::NSW ? tok0 : col0) * pitch, (size_t)(j >= G::NSW ? toks_in : cols_in) * pitch);
     }
 
-    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)s_mem;
+    const uint32_t lds0 = lds_address(s_mem);
     auto request = [&](int t, uint32_t at) __attribute__((always_inline)) {
         const int left = nblk - 4 * t;  // blocks from here on (none: every lane out of range)
 #pragma unroll
@@ -152,9 +117,9 @@ __global__ __launch_bounds__(G::THREADS, 512 / G::THREADS * 2) void mx_tile_kern
     const int wm = wave % G::WM, wn = wave / G::WM;
     f32x4m acc[Q][4][TN] = {};
     // byte offsets of this wave's operands within a stage
-    const int at_w = wm * Q * 4096 + r * 64 + ((g ^ ((r >> 2) & 3)) * 16);
-    const int at_a = AF == MX_E4M3 ? G::W_BYTES + wn * TN * 2048 + r * 128 + ((g ^ ((r >> 1) & 7)) * 16)
-                                   : G::W_BYTES + wn * TN * 1024 + r * 64 + ((g ^ ((r >> 2) & 3)) * 16);
+    const int at_w = wm * Q * 4096 + r * 64 + ((g ^ turn<64>(r)) * 16);
+    const int at_a = AF == MX_E4M3 ? G::W_BYTES + wn * TN * 2048 + r * 128 + ((g ^ turn<128>(r)) * 16)
+                                   : G::W_BYTES + wn * TN * 1024 + r * 64 + ((g ^ turn<64>(r)) * 16);
     const int at_sw = G::S_OFF + wm * Q * 256 + r * 16;
     const int at_sa = G::S_OFF + G::NSW * 256 + (wn * TN / 4) * 256 + r * 16 + (wn * TN % 4) * 4;
 
