@@ -191,12 +191,16 @@ __device__ __forceinline__ int xcd_order(int id, int total) {
     return x * per + min(x, rest) + (id >> 3);
 }
 
-// 16-byte piece c of row R of a staged tile lies at slot c ^ turn(R): the 16 lanes that
-// read a piece of 16 rows together then touch every bank once.  ROW: bytes of a row,
-// 64, 128 or 256.
-template <int ROW>
+// 16-byte piece c of row R of a staged tile lies at slot c ^ turn(R), so that a read of
+// one piece per lane group of 16 rows, or (PAIRS, 128-byte rows) of one of two that
+// belong together, touches every bank once (SQ_LDS_BANK_CONFLICT is 0; a read serves
+// lanes 0-3, 12-15 and 20-27 at a time, so rows 0-3 and 12-15 of a group meet rows 4-11
+// of the next).  ROW: bytes of a row, 64, 128 or more.
+template <int ROW, bool PAIRS = false>
 __device__ __forceinline__ int turn(int R) {
-    return ROW == 64 ? (R >> 2) & 3 : ROW == 128 ? (R >> 1) & 7 : R & 15;
+    if (ROW == 64) return (R >> 1) & 3;
+    if (ROW == 128 && PAIRS) return (((R >> 2) ^ (R >> 3)) & 1) | (R & 2) | ((R & 8) >> 1);
+    return ROW == 128 ? (R >> 1) & 7 : R & 15;
 }
 
 // One sum of a product, with its residual, at element `at` of out.

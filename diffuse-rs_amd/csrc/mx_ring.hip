@@ -50,6 +50,7 @@ struct RingGeom {
     static constexpr int AF = AF_, MT = MT_, NT = NT_, AR = AR_, SK = SK_, STAGES = STAGES_, WAVES = WAVES_;
     static constexpr bool GATED = GATED_, EXACT = EXACT_;
     static constexpr int FT = GATED ? MT / 2 : MT;  // tiles of output columns
+    static constexpr bool PAIRS = EXACT && AF == MX_E4M3;
     static constexpr int W_ROW = SK * 64, A_ROW = SK * (AF == MX_E4M3 ? 128 : 64);  // bytes of a row and step
     static constexpr int NW = MT * 16 * W_ROW / 1024;                               // DMA instructions of a step
     static constexpr int NA = (AR * A_ROW + 1023) / 1024;
@@ -99,7 +100,7 @@ __global__ __launch_bounds__(64 * G::WAVES) void mx_ring_kernel(const MxMatArgs 
     }
 #pragma unroll
     for (int k = 0; k < G::NA; ++k) {
-        const int R = k * A_ROWS % 16 + lane / A_LANES, c = (lane % A_LANES) ^ turn<G::A_ROW>(R);
+        const int R = k * A_ROWS % 16 + lane / A_LANES, c = (lane % A_LANES) ^ turn<G::A_ROW, G::PAIRS>(R);
         va[k] = R + k * A_ROWS / 16 * 16 < G::AR ? (R + k * A_ROWS / 16 * 16) * a_row + c * 16 : OUT_OF_RANGE;
         ba[k] = AF == MX_E4M3 ? c >> 1 : c;
     }
@@ -143,7 +144,7 @@ __global__ __launch_bounds__(64 * G::WAVES) void mx_ring_kernel(const MxMatArgs 
             for (int j = 0; j < NT; ++j) {
                 const int R = G::AR < 16 ? r & (G::AR - 1) : r;  // (the other rows' sums are not used)
                 const uint8_t* const row = st + G::A_OFF + (j * 16 + R) * G::A_ROW;
-                const int x = turn<G::A_ROW>(R);
+                const int x = turn<G::A_ROW, G::PAIRS>(R);
                 if constexpr (AF == MX_E4M3) {
                     const int c = 8 * s + (G::EXACT ? 2 * g : g);
                     ca[j][0] = *reinterpret_cast<const u32x4m*>(row + (c ^ x) * 16);

@@ -8,11 +8,12 @@
 // the 128); and block g's scale byte.  The weights are the A operand, so a lane's
 // four sums are consecutive output columns of one activation row.
 //
-// A workgroup's tile of BM weight rows by BN activation rows goes over the
-// columns in steps of 128.  Codes and scales of a step come by LDS DMA, 16 bytes
-// (codes) or four scale bytes a lane, STAGES - 1 steps ahead; columns behind a
-// row's end and rows behind the last are out of the buffer's range and read as 0
-// codes.
+// A workgroup's tile goes over the columns in steps of 128.  A step's codes come by LDS
+// DMA, 16 bytes a lane, STAGES - 1 steps ahead; columns behind a row's end and rows
+// behind the last are out of the buffer's range and read as 0 codes.  Scale bytes come
+// for four steps at a time, 16 bytes of a row: four bytes a row and step were half
+// of all requests to L2.  A wave issues its DMA between its products: all of it
+// at the start of a step, the address unit kept the products waiting.
 #include "mx_common.hpp"
 
 namespace dr {
@@ -34,28 +35,78 @@ struct TileGeom {
     static constexpr int ROW_B = AF == MX_E4M3 ? 128 : 64;    // bytes of an activation row and step
     static constexpr int W_BYTES = GROUPS * 64 * 64, A_BYTES = BN * ROW_B;
     static constexpr int NW = W_BYTES / 1024, NA = A_BYTES / 1024;  // DMA instructions of a step
-    static constexpr int NSW = GROUPS, NSA = (BN + 63) / 64;        // of its scales
-    static constexpr int NI_W = NW / WAVES, NI_A = NA / WAVES;
-    static constexpr int NI_S = (NSW + NSA + WAVES - 1) / WAVES, NI = NI_W + NI_A + NI_S;  // of a wave
-    static constexpr int S_OFF = W_BYTES + A_BYTES, STAGE = S_OFF + NI_S * WAVES * 256;
-    static constexpr int LDS = STAGE * STAGES;
+    static constexpr int NSW = GROUPS, NSA = (BN + 63) / 64;        // of four steps' scales
+    static constexpr int NI_W = NW / WAVES, NI_A = NA / WAVES, NI = NI_W + NI_A;  // of a wave and step
+    static constexpr int NI_S = (NSW + NSA + WAVES - 1) / WAVES;
+    static constexpr int STAGE = W_BYTES + A_BYTES, S_OFF = STAGE * STAGES, S_STAGE = NI_S * WAVES * 1024;
+    static constexpr int LDS = S_OFF + 2 * S_STAGE;
+    static constexpr int BAND = AF == MX_E4M3 ? 8 : 4;
+    static constexpr int PER_SIMD = Q * TN >= 8 ? 2 : 4;  // waves that registers leave room for
     static_assert(NW % WAVES == 0 && NA % WAVES == 0, "every wave issues the same number");
     static_assert(!GATED || Q % 2 == 0, "gate and up groups pair up in a wave");
     static_assert(LDS <= 160 * 1024, "LDS");
 };
 
+// A wave's sums, 16-byte pieces (rows a multiple of 8, out and residual aligned): lane's
+// activation rows tok1 + 16 j, columns c1 + 64 q .. + 15.  The residuals of all of them
+// (f32: of half) are asked for before the first is used; lanes behind the last row or
+// column read a valid place instead and write nothing.
+template <bool BF16, int Q, int TN>
+__device__ __forceinline__ void put_tile(const MxMatArgs& a, const f32x4m (&acc)[Q][4][TN], int tok1, int c1) {
+    constexpr int JB = BF16 || TN < 2 ? TN : TN / 2, P = BF16 ? 2 : 4, E = 16 / P;  // pieces of 16 columns, their values
+    constexpr size_t SIZE = BF16 ? 2 : 4;
+    const char* const res = static_cast<const char*>(a.residual);
+    char* const out = static_cast<char*>(a.out);
+#pragma unroll
+    for (int j0 = 0; j0 < TN; j0 += JB) {
+        u32x4m y[JB][Q][P] = {};
+        if (res) {
+#pragma unroll
+            for (int j = 0; j < JB; ++j)
+#pragma unroll
+                for (int q = 0; q < Q; ++q)
+#pragma unroll
+                    for (int h = 0; h < P; ++h)
+                        y[j][q][h] = *reinterpret_cast<const u32x4m*>(
+                            res + ((size_t)min(tok1 + (j0 + j) * 16, a.n - 1) * a.rows + min(c1 + q * 64 + h * E, a.rows - E)) * SIZE);
+        }
+#pragma unroll
+        for (int j = 0; j < JB; ++j) {
+            const int tok = tok1 + (j0 + j) * 16;
+#pragma unroll
+            for (int q = 0; q < Q; ++q)
+#pragma unroll
+                for (int h = 0; h < P; ++h) {
+                    const int c0 = c1 + q * 64 + h * E;
+                    u32x4m v;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const uint32_t b = y[j][q][h][e];
+                        if constexpr (BF16)
+                            v[e] = mx_bf16(acc[q][2 * h + e / 2][j0 + j][e % 2 * 2] + mx_f32(b & 0xffff)) |
+                                   (uint32_t)mx_bf16(acc[q][2 * h + e / 2][j0 + j][e % 2 * 2 + 1] + __uint_as_float(b & 0xffff0000u)) << 16;
+                        else
+                            v[e] = __float_as_uint(acc[q][h][j0 + j][e] + __uint_as_float(b));
+                    }
+                    if (tok < a.n && c0 < a.rows) *reinterpret_cast<u32x4m*>(out + ((size_t)tok * a.rows + c0) * SIZE) = v;
+                }
+        }
+    }
+}
+
 template <class G>
-__global__ __launch_bounds__(G::THREADS, 512 / G::THREADS * 2) void mx_tile_kernel(const MxMatArgs a, int n_m, int n_n) {
+__global__ __launch_bounds__(G::THREADS, G::PER_SIMD) void mx_tile_kernel(const MxMatArgs a, int n_m, int n_n) {
     extern __shared__ __align__(16) uint8_t s_mem[];
     constexpr int AF = G::AF, Q = G::Q, TN = G::TN;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, g = lane >> 4;
-    // an XCD's run of tiles: 4 along the weights by as many as there are along the activations
+    // an XCD's run of tiles: BAND along the weights by as many as there are along the
+    // activations, about as many bytes of one as of the other
     int mt, nt;
     {
-        const int lin = xcd_order(blockIdx.x, n_m * n_n), band = lin / (4 * n_n), in = lin - band * 4 * n_n, wide = min(4, n_m - 4 * band);
+        const int lin = xcd_order(blockIdx.x, n_m * n_n), band = lin / (G::BAND * n_n), in = lin - band * G::BAND * n_n, wide = min(G::BAND, n_m - G::BAND * band);
         nt = __builtin_amdgcn_readfirstlane(in / wide);  // (divided on the vector unit)
-        mt = __builtin_amdgcn_readfirstlane(4 * band + in - nt * wide);
+        mt = __builtin_amdgcn_readfirstlane(G::BAND * band + in - nt * wide);
     }
     const int nblk = a.cols / 32, steps = (nblk + 3) / 4;
     const int pitch = (int)mx_pitch(a.cols), w_row = a.cols / 2, a_row = (int)mx_row_bytes(AF, a.cols);
@@ -89,30 +140,32 @@ __global__ __launch_bounds__(G::THREADS, 512 / G::THREADS * 2) void mx_tile_kern
             ba[k] = c;
         }
     }
-    // scales: instruction j < NSW: group j's, dword r * 4 + i that of tile i, row r; then
-    // 64 activation rows' in the same order
+    // scales: 64 rows an instruction, the weight groups' and then the activations'
     int vs[G::NI_S];
 #pragma unroll
     for (int k = 0; k < G::NI_S; ++k) {
-        const int j = wave * G::NI_S + k, R = lane >> 2, i = lane & 3;
-        vs[k] = j < G::NSW ? (group_col(j) + 16 * (R >> 2) + 4 * i + (R & 3)) * pitch : ((j - G::NSW) * 64 + i * 16 + R) * pitch;
-        if (j >= G::NSW && (j - G::NSW) * 64 + i * 16 + R >= G::BN) vs[k] = OUT_OF_RANGE;  // (every wave issues the same number)
+        const int j = wave * G::NI_S + k, R = lane & 15, i = lane >> 4;
+        vs[k] = j < G::NSW ? (group_col(j) + 16 * (R >> 2) + 4 * i + (R & 3)) * pitch : ((j - G::NSW) * 64 + lane) * pitch;
+        if (j >= G::NSW && (j - G::NSW) * 64 + lane >= G::BN) vs[k] = OUT_OF_RANGE;  // (every wave issues the same number)
         const uint8_t* const base = j >= G::NSW ? a.act.scales : G::GATED && (j & 1) ? a.up.scales : a.w.scales;
         rs[k] = tile_rsrc(base + (size_t)(j >= G::NSW ? tok0 : col0) * pitch, (size_t)(j >= G::NSW ? toks_in : cols_in) * pitch);
     }
 
     const uint32_t lds0 = lds_address(s_mem);
-    auto request = [&](int t, uint32_t at) __attribute__((always_inline)) {
+    // instruction k of this wave's of step t, into the stage at LDS address `at`
+    auto request = [&](int k, int t, uint32_t at) __attribute__((always_inline)) {
         const int left = nblk - 4 * t;  // blocks from here on (none: every lane out of range)
-#pragma unroll
-        for (int k = 0; k < G::NI_W; ++k)
+        if (k < G::NI_W)
             dma16(rw[k], at + (wave * G::NI_W + k) * 1024, bw[k] < left ? vw[k] : OUT_OF_RANGE, t * 64);
+        else
+            dma16(ra, at + G::W_BYTES + (wave * G::NI_A + k - G::NI_W) * 1024, ba[k - G::NI_W] < left ? va[k - G::NI_W] : OUT_OF_RANGE,
+                  t * G::ROW_B);
+    };
+    // the scales of steps 4 c .. 4 c + 3
+    auto request_scales = [&](int c) __attribute__((always_inline)) {
+        const uint32_t at = lds0 + G::S_OFF + (c & 1) * G::S_STAGE + wave * G::NI_S * 1024;
 #pragma unroll
-        for (int k = 0; k < G::NI_A; ++k)
-            dma16(ra, at + G::W_BYTES + (wave * G::NI_A + k) * 1024, ba[k] < left ? va[k] : OUT_OF_RANGE, t * G::ROW_B);
-#pragma unroll
-        for (int k = 0; k < G::NI_S; ++k)
-            dma4(rs[k], at + G::S_OFF + (wave * G::NI_S + k) * 256, left > 0 ? vs[k] : OUT_OF_RANGE, t * 4);
+        for (int k = 0; k < G::NI_S; ++k) dma16(rs[k], at + k * 1024, 16 * c < nblk ? vs[k] : OUT_OF_RANGE, c * 16);
     };
     const int wm = wave % G::WM, wn = wave / G::WM;
     f32x4m acc[Q][4][TN] = {};
@@ -120,97 +173,98 @@ __global__ __launch_bounds__(G::THREADS, 512 / G::THREADS * 2) void mx_tile_kern
     const int at_w = wm * Q * 4096 + r * 64 + ((g ^ turn<64>(r)) * 16);
     const int at_a = AF == MX_E4M3 ? G::W_BYTES + wn * TN * 2048 + r * 128 + ((g ^ turn<128>(r)) * 16)
                                    : G::W_BYTES + wn * TN * 1024 + r * 64 + ((g ^ turn<64>(r)) * 16);
-    const int at_sw = G::S_OFF + wm * Q * 256 + r * 16;
-    const int at_sa = G::S_OFF + G::NSW * 256 + (wn * TN / 4) * 256 + r * 16 + (wn * TN % 4) * 4;
+    const int at_sw = G::S_OFF + wm * Q * 1024 + r * 16, at_sa = G::S_OFF + G::NSW * 1024 + wn * TN * 256 + r * 16;
 
-    auto multiply = [&](int t, const uint8_t* st) __attribute__((always_inline)) {
+    auto weights = [&](const uint8_t* st, int n) __attribute__((always_inline)) {  // tile n % 4 of group n / 4
+        return *reinterpret_cast<const u32x4m*>(st + at_w + n * 1024);
+    };
+    // the products of step t; between them `more` of the DMA of a later one
+    auto multiply = [&](int t, const uint8_t* st, auto&& more) __attribute__((always_inline)) {
         // the scale byte of block g; behind a row's last block the codes are 0 and so is this
         const uint32_t sel = 4 * t + g < nblk ? 0x0c0c0c00u | g : 0x0c0c0c0cu;
+        const uint8_t* const sc = s_mem + ((t >> 2) & 1) * G::S_STAGE + (t & 3) * 4;
+        auto scale = [&](int at) __attribute__((always_inline)) {
+            return (int)__builtin_amdgcn_perm(0, *reinterpret_cast<const uint32_t*>(sc + at), sel);
+        };
         i32x8m oa[TN];
-        uint32_t sa[TN];
-#pragma unroll
-        for (int j = 0; j < TN; ++j) {
+        int sa[TN], sw = scale(at_sw);
+        u32x4m w = weights(st, 0);
+        auto acts = [&](int j) __attribute__((always_inline)) {
             const u32x4m lo = *reinterpret_cast<const u32x4m*>(st + at_a + j * 16 * G::ROW_B);
             oa[j] = i32x8m{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], 0, 0, 0, 0};
             if constexpr (AF == MX_E4M3) {
                 const u32x4m hi = *reinterpret_cast<const u32x4m*>(st + (at_a ^ 64) + j * 16 * G::ROW_B);
                 oa[j][4] = (int)hi[0], oa[j][5] = (int)hi[1], oa[j][6] = (int)hi[2], oa[j][7] = (int)hi[3];
             }
-            sa[j] = __builtin_amdgcn_perm(0, *reinterpret_cast<const uint32_t*>(st + at_sa + j * 4), sel);
-        }
+            sa[j] = scale(at_sa + j * 256);
+        };
 #pragma unroll
-        for (int q = 0; q < Q; ++q) {
-            const u32x4m s4 = *reinterpret_cast<const u32x4m*>(st + at_sw + q * 256);
+        for (int j = 0; j < TN; ++j) acts(j);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const u32x4m w = *reinterpret_cast<const u32x4m*>(st + at_w + q * 4096 + i * 1024);
-                const i32x8m ow = i32x8m{(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
-                const int sw = (int)__builtin_amdgcn_perm(0, s4[i], sel);
+        for (int n = 0; n < 4 * Q; ++n) {
+            u32x4m w_next = w;
+            int s_next = sw;
+            if (n + 1 < 4 * Q) w_next = weights(st, n + 1), s_next = scale(at_sw + (n + 1) * 256);
+            more(n);
+            const i32x8m ow = i32x8m{(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
 #pragma unroll
-                for (int j = 0; j < TN; ++j)
-                    acc[q][i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(ow, oa[j], acc[q][i][j], 4, AF == MX_E4M3 ? 0 : 4,
-                                                                                     0, sw, 0, (int)sa[j]);
-            }
+            for (int j = 0; j < TN; ++j)
+                acc[n / 4][n % 4][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(ow, oa[j], acc[n / 4][n % 4][j], 4,
+                                                                                         AF == MX_E4M3 ? 0 : 4, 0, sw, 0, sa[j]);
+            w = w_next, sw = s_next;
+            __builtin_amdgcn_sched_barrier(0);  // or all the DMA would come before all the products
         }
     };
 
+    request_scales(0);
 #pragma unroll
-    for (int s = 0; s < G::STAGES - 1; ++s) request(s, lds0 + s * G::STAGE);
+    for (int s = 0; s < G::STAGES - 1; ++s)
+#pragma unroll
+        for (int k = 0; k < G::NI; ++k) request(k, s, lds0 + s * G::STAGE);
     int cur = 0;
     for (int t = 0; t < steps; ++t) {
-        // this wave's pieces of step t are there; behind the barrier everybody's, and
-        // everybody has read step t - 1, whose place is free
+        // This wave's pieces of step t are there, and its scales, which were asked for
+        // before them; behind the barrier everybody's, and everybody has read step t - 1,
+        // whose place is free.
         wait_vm<(G::STAGES - 2) * G::NI>();
         barrier_lds();
         const int next = cur == 0 ? G::STAGES - 1 : cur - 1;
-        request(t + G::STAGES - 1, lds0 + next * G::STAGE);
-        multiply(t, s_mem + cur * G::STAGE);
+        if ((t & 3) == 0) request_scales((t >> 2) + 1);
+        constexpr int PER = (G::NI + 4 * Q - 1) / (4 * Q);  // DMA instructions between two rows of products
+        multiply(t, s_mem + cur * G::STAGE, [&](int n) __attribute__((always_inline)) {
+#pragma unroll
+            for (int k = n * PER; k < (n + 1) * PER && k < G::NI; ++k) request(k, t + G::STAGES - 1, lds0 + next * G::STAGE);
+        });
         cur = cur == G::STAGES - 1 ? 0 : cur + 1;
     }
     wait_vm<0>();
 
     // lane (r, g): activation row r of each tile, 16 columns of each group
+    const int tok1 = tok0 + wn * TN * 16 + r;
+    if constexpr (!G::GATED) {
+        const int c1 = col0 + wm * Q * 64 + 16 * g;
+        if ((a.rows & 7) == 0 && a.vec) {
+            if (a.bf16)
+                put_tile<true, Q, TN>(a, acc, tok1, c1);
+            else
+                put_tile<false, Q, TN>(a, acc, tok1, c1);
+            return;
+        }
 #pragma unroll
-    for (int j = 0; j < TN; ++j) {
-        const int tok = tok0 + (wn * TN + j) * 16 + r;
-        if constexpr (!G::GATED) {
+        for (int j = 0; j < TN; ++j)
 #pragma unroll
             for (int q = 0; q < Q; ++q) {
-                const int c0 = col0 + (wm * Q + q) * 64 + 16 * g;
-                if (tok >= a.n || c0 >= a.rows) continue;
-                const size_t at = (size_t)tok * a.rows + c0;
-                const int in = min(16, a.rows - c0);
-                const bool whole = in == 16 && ((a.rows & 7) == 0) && a.vec;
+                const int tok = tok1 + j * 16, c0 = c1 + q * 64;
+                if (tok >= a.n) continue;
 #pragma unroll
-                for (int i = 0; i < 4; i += 2) {
-                    float x[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) x[e] = acc[q][i + e / 4][j][e % 4];
-                    if (whole) {
-                        float y[8];
-                        if (a.bf16) {
-                            if (a.residual) {
-                                load8<true>(a.residual, at + 4 * i, y);
-#pragma unroll
-                                for (int e = 0; e < 8; ++e) x[e] += y[e];
-                            }
-                            store8<true>(a.out, at + 4 * i, x);
-                        } else {
-                            if (a.residual) {
-                                load8<false>(a.residual, at + 4 * i, y);
-#pragma unroll
-                                for (int e = 0; e < 8; ++e) x[e] += y[e];
-                            }
-                            store8<false>(a.out, at + 4 * i, x);
-                        }
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 8; ++e)
-                            if (4 * i + e < in) put_sum(a, at + 4 * i + e, x[e]);
-                    }
-                }
+                for (int e = 0; e < 16; ++e)
+                    if (c0 + e < a.rows) put_sum(a, (size_t)tok * a.rows + c0 + e, acc[q][e / 4][j][e % 4]);
             }
-        } else {
+    } else {
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+            const int tok = tok1 + j * 16;
 #pragma unroll
             for (int q = 0; q < Q; q += 2) {
                 const int c0 = col0 + (wm * Q + q) / 2 * 64 + 16 * g;
