@@ -14,6 +14,8 @@
 //           written.
 #pragma once
 
+#include <type_traits>
+
 #include "dr_internal.hpp"
 
 namespace dr {
@@ -144,6 +146,17 @@ __device__ __forceinline__ void store8(void* base, size_t at, const float (&x)[8
 __device__ __forceinline__ float mx_act(float x, int fn) {
     const float z = fn == MX_SILU ? x : 1.5957691216057308f * (x + 0.044715f * x * x * x);
     return x / (1.0f + expf(-z));
+}
+
+// f(Int<0>{}) .. f(Int<N - 1>{})
+template <int I>
+using Int = std::integral_constant<int, I>;
+template <int N, int I = 0, class F>
+__device__ __forceinline__ void static_for(F&& f) {
+    if constexpr (I < N) {
+        f(Int<I>{});
+        static_for<N, I + 1>(f);
+    }
 }
 
 // ---- staging through LDS (mx_ring.hip, mx_tile.hip)

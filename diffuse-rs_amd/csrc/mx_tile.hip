@@ -8,12 +8,14 @@
 // the 128); and block g's scale byte.  The weights are the A operand, so a lane's
 // four sums are consecutive output columns of one activation row.
 //
-// A workgroup's tile goes over the columns in steps of 128.  A step's codes come by LDS
-// DMA, 16 bytes a lane, STAGES - 1 steps ahead; columns behind a row's end and rows
+// A workgroup's tile goes over the columns in stages of SB * 128.  A stage's codes come by
+// LDS DMA, 16 bytes a lane, STAGES - 1 stages ahead; columns behind a row's end and rows
 // behind the last are out of the buffer's range and read as 0 codes.  Scale bytes come
-// for four steps at a time, 16 bytes of a row: four bytes a row and step were half
-// of all requests to L2.  A wave issues its DMA between its products: all of it
-// at the start of a step, the address unit kept the products waiting.
+// for 512 columns (a chunk) at a time, 16 bytes of a row (four bytes a row and 128
+// columns were half of all requests to L2), and wait in registers, a lane's four bytes
+// of a row in one, from which the MFMA takes the one it is told.  A wave issues its DMA
+// between its products: all of it at the start of a stage, the address unit kept the
+// products waiting.
 #include "mx_common.hpp"
 
 namespace dr {
@@ -24,27 +26,32 @@ namespace {
 // are rows of `up`, of the same output columns as the group before).  Tile i, row
 // 4 g + e of a group is its weight row 16 g + 4 i + e, so that lane group g's sums
 // over the four tiles are 16 consecutive output columns.
-template <int AF_, bool GATED_, int WM_, int Q_, int WN_, int TN_, int STAGES_>
+template <int AF_, bool GATED_, int WM_, int Q_, int WN_, int TN_, int SB_, int STAGES_>
 struct TileGeom {
-    static constexpr int AF = AF_, WM = WM_, Q = Q_, WN = WN_, TN = TN_, STAGES = STAGES_;
+    static constexpr int AF = AF_, WM = WM_, Q = Q_, WN = WN_, TN = TN_, SB = SB_, STAGES = STAGES_;
     static constexpr bool GATED = GATED_;
     static constexpr int WAVES = WM * WN, THREADS = 64 * WAVES;
-    static constexpr int GROUPS = WM * Q;                     // of 64 weight rows
+    static constexpr int GROUPS = WM * Q;                       // of 64 weight rows
     static constexpr int COLS = GROUPS * 64 / (GATED ? 2 : 1);  // output columns
     static constexpr int BN = WN * TN * 16;
-    static constexpr int ROW_B = AF == MX_E4M3 ? 128 : 64;    // bytes of an activation row and step
-    static constexpr int W_BYTES = GROUPS * 64 * 64, A_BYTES = BN * ROW_B;
-    static constexpr int NW = W_BYTES / 1024, NA = A_BYTES / 1024;  // DMA instructions of a step
-    static constexpr int NSW = GROUPS, NSA = (BN + 63) / 64;        // of four steps' scales
-    static constexpr int NI_W = NW / WAVES, NI_A = NA / WAVES, NI = NI_W + NI_A;  // of a wave and step
+    static constexpr int W_ROW = SB * 64, A_ROW = SB * (AF == MX_E4M3 ? 128 : 64);  // bytes of a row and stage
+    static constexpr int W_BYTES = GROUPS * 64 * W_ROW, A_BYTES = BN * A_ROW;
+    static constexpr int NW = W_BYTES / 1024, NA = A_BYTES / 1024;  // DMA instructions of a stage
+    static constexpr int NSW = GROUPS, NSA = (BN + 63) / 64;        // of a chunk's scales
+    static constexpr int NI_W = NW / WAVES, NI_A = NA / WAVES, NI = NI_W + NI_A;  // of a wave
     static constexpr int NI_S = (NSW + NSA + WAVES - 1) / WAVES;
+    static constexpr int PARTS = 4 / SB;                           // stages of a chunk
+    static constexpr int AHEAD = (STAGES - 1 + PARTS - 1) / PARTS;  // chunks that scales are asked for ahead
     static constexpr int STAGE = W_BYTES + A_BYTES, S_OFF = STAGE * STAGES, S_STAGE = NI_S * WAVES * 1024;
-    static constexpr int LDS = S_OFF + 2 * S_STAGE;
+    static constexpr int LDS = S_OFF + (AHEAD + 1) * S_STAGE;
+    static constexpr int FIT = 160 * 1024 / LDS * WAVES / 4;  // waves per SIMD that LDS leaves room for
+    static constexpr int MOST = Q * TN >= 8 ? 2 : 4, PER_SIMD = FIT < 1 ? 1 : FIT < MOST ? FIT : MOST;
+    static constexpr bool WHOLE = Q * 16 + TN * 8 <= 24;  // two steps' operands fit in registers
     static constexpr int BAND = AF == MX_E4M3 ? 8 : 4;
-    static constexpr int PER_SIMD = Q * TN >= 8 ? 2 : 4;  // waves that registers leave room for
     static_assert(NW % WAVES == 0 && NA % WAVES == 0, "every wave issues the same number");
     static_assert(!GATED || Q % 2 == 0, "gate and up groups pair up in a wave");
     static_assert(LDS <= 160 * 1024, "LDS");
+    static_assert((STAGES - 2) * NI < 64, "vmcnt");
 };
 
 // A wave's sums, 16-byte pieces (rows a multiple of 8, out and residual aligned): lane's
@@ -108,37 +115,32 @@ __global__ __launch_bounds__(G::THREADS, G::PER_SIMD) void mx_tile_kernel(const 
         nt = __builtin_amdgcn_readfirstlane(in / wide);  // (divided on the vector unit)
         mt = __builtin_amdgcn_readfirstlane(G::BAND * band + in - nt * wide);
     }
-    const int nblk = a.cols / 32, steps = (nblk + 3) / 4;
+    const int nblk = a.cols / 32, stages = (nblk + 4 * G::SB - 1) / (4 * G::SB), chunks = (nblk + 15) / 16;
     const int pitch = (int)mx_pitch(a.cols), w_row = a.cols / 2, a_row = (int)mx_row_bytes(AF, a.cols);
     const int col0 = mt * G::COLS, tok0 = nt * G::BN;
 
     const int cols_in = min(G::COLS, a.rows - col0), toks_in = min(G::BN, a.n - tok0);
     // first output column (within the tile) of weight group q
     auto group_col = [](int q) { return G::GATED ? (q >> 1) * 64 : q * 64; };
-    // 16-byte pieces of a step (buffers over the tile's rows; an instruction's is the wave's own choice)
+    // 16-byte pieces of a stage (buffers over the tile's rows; an instruction's is the wave's own choice)
     __amdgpu_buffer_rsrc_t rw[G::NI_W], rs[G::NI_S];
     const __amdgpu_buffer_rsrc_t ra = tile_rsrc(a.act.codes + (size_t)tok0 * a_row, (size_t)toks_in * a_row);
+    constexpr int W_LANES = G::W_ROW / 16, A_LANES = G::A_ROW / 16;  // lanes of a row
     int vw[G::NI_W], bw[G::NI_W], va[G::NI_A], ba[G::NI_A];
 #pragma unroll
-    for (int k = 0; k < G::NI_W; ++k) {  // instruction j: tile j % 4 of group j / 4
-        const int j = wave * G::NI_W + k, R = lane >> 2, c = (lane & 3) ^ turn<64>(R);
-        const int row = group_col(j >> 2) + 16 * (R >> 2) + 4 * (j & 3) + (R & 3);
-        vw[k] = row * w_row + c * 16;
+    for (int k = 0; k < G::NI_W; ++k) {  // LDS row L: row L % 16 of tile L / 16 % 4 of group L / 64
+        const int j = wave * G::NI_W + k, L = j * (64 / W_LANES) + lane / W_LANES, R = L & 15;
+        const int c = (lane % W_LANES) ^ turn<G::W_ROW>(R);
+        vw[k] = (group_col(L >> 6) + 16 * (R >> 2) + 4 * (L >> 4 & 3) + (R & 3)) * w_row + c * 16;
         bw[k] = c;
-        rw[k] = tile_rsrc((G::GATED && (j & 4) ? a.up.codes : a.w.codes) + (size_t)col0 * w_row, (size_t)cols_in * w_row);
+        const bool second = G::GATED && (j * (64 / W_LANES) >> 6 & 1);  // (a group is whole instructions)
+        rw[k] = tile_rsrc((second ? a.up.codes : a.w.codes) + (size_t)col0 * w_row, (size_t)cols_in * w_row);
     }
 #pragma unroll
     for (int k = 0; k < G::NI_A; ++k) {
-        const int j = wave * G::NI_A + k;
-        if constexpr (AF == MX_E4M3) {  // 8 rows
-            const int R = j * 8 + (lane >> 3), c = (lane & 7) ^ turn<128>(R);
-            va[k] = R * a_row + c * 16;
-            ba[k] = c >> 1;
-        } else {  // 16 rows
-            const int R = j * 16 + (lane >> 2), c = (lane & 3) ^ turn<64>(R);
-            va[k] = R * a_row + c * 16;
-            ba[k] = c;
-        }
+        const int R = (wave * G::NI_A + k) * (64 / A_LANES) + lane / A_LANES, c = (lane % A_LANES) ^ turn<G::A_ROW>(R);
+        va[k] = R * a_row + c * 16;
+        ba[k] = AF == MX_E4M3 ? c >> 1 : c;
     }
     // scales: 64 rows an instruction, the weight groups' and then the activations'
     int vs[G::NI_S];
@@ -151,92 +153,142 @@ __global__ __launch_bounds__(G::THREADS, G::PER_SIMD) void mx_tile_kernel(const 
         rs[k] = tile_rsrc(base + (size_t)(j >= G::NSW ? tok0 : col0) * pitch, (size_t)(j >= G::NSW ? toks_in : cols_in) * pitch);
     }
 
-    const uint32_t lds0 = lds_address(s_mem);
-    // instruction k of this wave's of step t, into the stage at LDS address `at`
+    // instruction k of this wave's of stage t, to LDS address `at`
     auto request = [&](int k, int t, uint32_t at) __attribute__((always_inline)) {
-        const int left = nblk - 4 * t;  // blocks from here on (none: every lane out of range)
+        const int left = nblk - 4 * G::SB * t;  // blocks from here on (none: every lane out of range)
         if (k < G::NI_W)
-            dma16(rw[k], at + (wave * G::NI_W + k) * 1024, bw[k] < left ? vw[k] : OUT_OF_RANGE, t * 64);
+            dma16(rw[k], at + (wave * G::NI_W + k) * 1024, bw[k] < left ? vw[k] : OUT_OF_RANGE, t * G::W_ROW);
         else
             dma16(ra, at + G::W_BYTES + (wave * G::NI_A + k - G::NI_W) * 1024, ba[k - G::NI_W] < left ? va[k - G::NI_W] : OUT_OF_RANGE,
-                  t * G::ROW_B);
+                  t * G::A_ROW);
     };
-    // the scales of steps 4 c .. 4 c + 3
-    auto request_scales = [&](int c) __attribute__((always_inline)) {
-        const uint32_t at = lds0 + G::S_OFF + (c & 1) * G::S_STAGE + wave * G::NI_S * 1024;
+    auto request_scales = [&](int c, uint32_t at) __attribute__((always_inline)) {  // of chunk c
 #pragma unroll
-        for (int k = 0; k < G::NI_S; ++k) dma16(rs[k], at + k * 1024, 16 * c < nblk ? vs[k] : OUT_OF_RANGE, c * 16);
+        for (int k = 0; k < G::NI_S; ++k)
+            dma16(rs[k], at + (wave * G::NI_S + k) * 1024, 16 * c < nblk ? vs[k] : OUT_OF_RANGE, c * 16);
     };
     const int wm = wave % G::WM, wn = wave / G::WM;
     f32x4m acc[Q][4][TN] = {};
-    // byte offsets of this wave's operands within a stage
-    const int at_w = wm * Q * 4096 + r * 64 + ((g ^ turn<64>(r)) * 16);
-    const int at_a = AF == MX_E4M3 ? G::W_BYTES + wn * TN * 2048 + r * 128 + ((g ^ turn<128>(r)) * 16)
-                                   : G::W_BYTES + wn * TN * 1024 + r * 64 + ((g ^ turn<64>(r)) * 16);
-    const int at_sw = G::S_OFF + wm * Q * 1024 + r * 16, at_sa = G::S_OFF + G::NSW * 1024 + wn * TN * 256 + r * 16;
+    // byte offsets of this wave's operands within a stage, and of its scales within a chunk's
+    const int at_w = (wm * Q * 64 + r) * G::W_ROW, at_a = G::W_BYTES + (wn * TN * 16 + r) * G::A_ROW;
+    const int at_sw = wm * Q * 1024 + r * 16, at_sa = G::NSW * 1024 + wn * TN * 256 + r * 16;
+    const int turn_w = turn<G::W_ROW>(r), turn_a = turn<G::A_ROW>(r);
 
-    auto weights = [&](const uint8_t* st, int n) __attribute__((always_inline)) {  // tile n % 4 of group n / 4
-        return *reinterpret_cast<const u32x4m*>(st + at_w + n * 1024);
+    // operands of the 128 columns s of a stage: tile n % 4 of group n / 4, activation tile j
+    auto weights = [&](const uint8_t* st, int s, int n) __attribute__((always_inline)) {
+        const u32x4m w = *reinterpret_cast<const u32x4m*>(st + at_w + n * 16 * G::W_ROW + ((4 * s + g) ^ turn_w) * 16);
+        return i32x8m{(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
     };
-    // the products of step t; between them `more` of the DMA of a later one
-    auto multiply = [&](int t, const uint8_t* st, auto&& more) __attribute__((always_inline)) {
-        // the scale byte of block g; behind a row's last block the codes are 0 and so is this
-        const uint32_t sel = 4 * t + g < nblk ? 0x0c0c0c00u | g : 0x0c0c0c0cu;
-        const uint8_t* const sc = s_mem + ((t >> 2) & 1) * G::S_STAGE + (t & 3) * 4;
-        auto scale = [&](int at) __attribute__((always_inline)) {
-            return (int)__builtin_amdgcn_perm(0, *reinterpret_cast<const uint32_t*>(sc + at), sel);
+    auto acts = [&](const uint8_t* st, int s, int j) __attribute__((always_inline)) {
+        const uint8_t* const row = st + at_a + j * 16 * G::A_ROW;
+        if constexpr (AF == MX_E4M3) {
+            const u32x4m lo = *reinterpret_cast<const u32x4m*>(row + ((8 * s + g) ^ turn_a) * 16);
+            const u32x4m hi = *reinterpret_cast<const u32x4m*>(row + ((8 * s + 4 + g) ^ turn_a) * 16);
+            return i32x8m{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
+        } else {
+            const u32x4m lo = *reinterpret_cast<const u32x4m*>(row + ((4 * s + g) ^ turn_a) * 16);
+            return i32x8m{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], 0, 0, 0, 0};
+        }
+    };
+    // A row's 16 scale bytes -> block g's of each 128 columns.  Behind a row's last block
+    // the codes are 0 and so is this (the bytes there are no scales).
+    int sw[4 * Q], sa[TN];
+    auto scales = [&](int c, const uint8_t* sc) __attribute__((always_inline)) {
+        const int left = nblk - 16 * c - g;
+        const uint32_t s01 = (left > 0 ? g : 0x0c) | (left > 4 ? 4 + g : 0x0c) << 8 | 0x0c0c0000u;
+        const uint32_t s23 = (left > 8 ? g : 0x0c) << 16 | (left > 12 ? 4 + g : 0x0cu) << 24 | 0x0c0cu;
+        auto four = [&](int at) __attribute__((always_inline)) {
+            const u32x4m d = *reinterpret_cast<const u32x4m*>(sc + at);
+            return (int)(__builtin_amdgcn_perm(d[1], d[0], s01) | __builtin_amdgcn_perm(d[3], d[2], s23));
         };
-        i32x8m oa[TN];
-        int sa[TN], sw = scale(at_sw);
-        u32x4m w = weights(st, 0);
-        auto acts = [&](int j) __attribute__((always_inline)) {
-            const u32x4m lo = *reinterpret_cast<const u32x4m*>(st + at_a + j * 16 * G::ROW_B);
-            oa[j] = i32x8m{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], 0, 0, 0, 0};
-            if constexpr (AF == MX_E4M3) {
-                const u32x4m hi = *reinterpret_cast<const u32x4m*>(st + (at_a ^ 64) + j * 16 * G::ROW_B);
-                oa[j][4] = (int)hi[0], oa[j][5] = (int)hi[1], oa[j][6] = (int)hi[2], oa[j][7] = (int)hi[3];
-            }
-            sa[j] = scale(at_sa + j * 256);
-        };
 #pragma unroll
-        for (int j = 0; j < TN; ++j) acts(j);
-        __builtin_amdgcn_sched_barrier(0);
+        for (int n = 0; n < 4 * Q; ++n) sw[n] = four(at_sw + n * 256);
 #pragma unroll
-        for (int n = 0; n < 4 * Q; ++n) {
-            u32x4m w_next = w;
-            int s_next = sw;
-            if (n + 1 < 4 * Q) w_next = weights(st, n + 1), s_next = scale(at_sw + (n + 1) * 256);
-            more(n);
-            const i32x8m ow = i32x8m{(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
+        for (int j = 0; j < TN; ++j) sa[j] = four(at_sa + j * 256);
+    };
+    auto mfma = [&](auto byte, const i32x8m& w, const i32x8m& o, int n, int j) __attribute__((always_inline)) {
+        constexpr int BYTE = decltype(byte)::value;
+        f32x4m& d = acc[n / 4][n % 4][j];
+        d = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, o, d, 4, AF == MX_E4M3 ? 0 : 4, BYTE, sw[n], BYTE, sa[j]);
+    };
+    // The products of a stage, the first of whose 128 columns are number PART of the
+    // chunk's; between them `more` (of 4 Q a step) of the DMA of a later one.
+    auto multiply = [&](auto part, const uint8_t* st, auto&& more) __attribute__((always_inline)) {
+        constexpr int PART = decltype(part)::value;
+        if constexpr (G::WHOLE) {
+            // few products a step: the next step's operands are on their way before this one's
+            i32x8m w[2][4 * Q], o[2][TN];
+            auto load = [&](int s) __attribute__((always_inline)) {
 #pragma unroll
-            for (int j = 0; j < TN; ++j)
-                acc[n / 4][n % 4][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(ow, oa[j], acc[n / 4][n % 4][j], 4,
-                                                                                         AF == MX_E4M3 ? 0 : 4, 0, sw, 0, sa[j]);
-            w = w_next, sw = s_next;
-            __builtin_amdgcn_sched_barrier(0);  // or all the DMA would come before all the products
+                for (int j = 0; j < TN; ++j) o[s & 1][j] = acts(st, s, j);
+#pragma unroll
+                for (int n = 0; n < 4 * Q; ++n) w[s & 1][n] = weights(st, s, n);
+            };
+            load(0);
+            static_for<G::SB>([&](auto step) __attribute__((always_inline)) {
+                constexpr int S = decltype(step)::value;
+                if constexpr (S + 1 < G::SB) load(S + 1);
+#pragma unroll
+                for (int n = 0; n < 4 * Q; ++n) more(S * 4 * Q + n);
+#pragma unroll
+                for (int n = 0; n < 4 * Q; ++n)
+#pragma unroll
+                    for (int j = 0; j < TN; ++j) mfma(Int<PART + S>{}, w[S & 1][n], o[S & 1][j], n, j);
+                __builtin_amdgcn_sched_barrier(0);
+            });
+        } else {
+            static_for<G::SB>([&](auto step) __attribute__((always_inline)) {
+                constexpr int S = decltype(step)::value;
+                i32x8m o[TN], w = weights(st, S, 0);
+#pragma unroll
+                for (int j = 0; j < TN; ++j) o[j] = acts(st, S, j);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int n = 0; n < 4 * Q; ++n) {
+                    i32x8m next = w;
+                    if (n + 1 < 4 * Q) next = weights(st, S, n + 1);
+                    more(S * 4 * Q + n);
+#pragma unroll
+                    for (int j = 0; j < TN; ++j) mfma(Int<PART + S>{}, w, o[j], n, j);
+                    w = next;
+                    __builtin_amdgcn_sched_barrier(0);  // or all the DMA would come before all the products
+                }
+            });
         }
     };
 
-    request_scales(0);
+    const uint32_t lds0 = lds_address(s_mem);
+#pragma unroll
+    for (int c = 0; c < G::AHEAD; ++c) request_scales(c, lds0 + G::S_OFF + c * G::S_STAGE);
 #pragma unroll
     for (int s = 0; s < G::STAGES - 1; ++s)
 #pragma unroll
         for (int k = 0; k < G::NI; ++k) request(k, s, lds0 + s * G::STAGE);
-    int cur = 0;
-    for (int t = 0; t < steps; ++t) {
-        // This wave's pieces of step t are there, and its scales, which were asked for
-        // before them; behind the barrier everybody's, and everybody has read step t - 1,
-        // whose place is free.
-        wait_vm<(G::STAGES - 2) * G::NI>();
-        barrier_lds();
-        const int next = cur == 0 ? G::STAGES - 1 : cur - 1;
-        if ((t & 3) == 0) request_scales((t >> 2) + 1);
-        constexpr int PER = (G::NI + 4 * Q - 1) / (4 * Q);  // DMA instructions between two rows of products
-        multiply(t, s_mem + cur * G::STAGE, [&](int n) __attribute__((always_inline)) {
+    int cur = 0, slot = 0, t = 0;
+    for (int c = 0; c < chunks; ++c) {
+        static_for<G::PARTS>([&](auto of_chunk) __attribute__((always_inline)) {
+            constexpr int U = decltype(of_chunk)::value;
+            if (U > 0 && t >= stages) return;
+            // This wave's pieces of stage t are there, and the chunk's scales, which were asked
+            // for before them; behind the barrier everybody's, and everybody has read stage
+            // t - 1 and the last chunk's scales, whose places are free.
+            wait_vm<(G::STAGES - 2) * G::NI>();
+            barrier_lds();
+            if constexpr (U == 0) {
+                const int behind = slot == 0 ? G::AHEAD : slot - 1;
+                scales(c, s_mem + G::S_OFF + slot * G::S_STAGE);
+                request_scales(c + G::AHEAD, lds0 + G::S_OFF + behind * G::S_STAGE);
+                slot = slot == G::AHEAD ? 0 : slot + 1;
+            }
+            const int next = cur == 0 ? G::STAGES - 1 : cur - 1;
+            constexpr int GAPS = G::SB * 4 * Q, PER = (G::NI + GAPS - 1) / GAPS;  // DMA instructions between two rows of products
+            multiply(Int<U * G::SB>{}, s_mem + cur * G::STAGE, [&](int n) __attribute__((always_inline)) {
 #pragma unroll
-            for (int k = n * PER; k < (n + 1) * PER && k < G::NI; ++k) request(k, t + G::STAGES - 1, lds0 + next * G::STAGE);
+                for (int k = n * PER; k < (n + 1) * PER && k < G::NI; ++k) request(k, t + G::STAGES - 1, lds0 + next * G::STAGE);
+            });
+            cur = cur == G::STAGES - 1 ? 0 : cur + 1;
+            ++t;
         });
-        cur = cur == G::STAGES - 1 ? 0 : cur + 1;
     }
     wait_vm<0>();
 
@@ -309,11 +361,11 @@ hipError_t tiles(const MxMatArgs& a, hipStream_t st) {
     constexpr int BIG = AF == MX_E4M3 ? 3 : 4;
     const long cols = GATED ? 2l * a.rows : a.rows;
     const long big = (cols + 255) / 256 * ((a.n + 255) / 256);
-    if (big >= a.n_cu / 2) return tile<TileGeom<AF, GATED, 2, 2, 4, 4, BIG>>(a, st);
+    if (big >= a.n_cu / 2) return tile<TileGeom<AF, GATED, 2, 2, 4, 4, 1, BIG>>(a, st);
     if constexpr (GATED)
-        return tile<TileGeom<AF, GATED, 1, 2, 4, 2, 3>>(a, st);
+        return tile<TileGeom<AF, GATED, 1, 2, 4, 2, 1, 3>>(a, st);
     else
-        return tile<TileGeom<AF, GATED, 1, 1, 4, 1, 4>>(a, st);
+        return tile<TileGeom<AF, GATED, 1, 1, 4, 1, 2, 3>>(a, st);
 }
 
 }  // namespace
