@@ -1375,6 +1375,16 @@ int dr_mx_gated(dr_ctx* ctx, const dr_mx_rows* gate, const dr_mx_rows* up, size_
     return DR_OK;
 }
 
+int dr_debug_mx_plan(int gated, int act_format, int dtype, size_t rows, size_t cols, size_t n, int n_cu, int* kernel) {
+    const char* who = "dr_debug_mx_plan";
+    DR_CHECK(mx_dtype(who, dtype));
+    DR_CHECK(mx_cols(who, "cols", cols));
+    if (!kernel || n_cu <= 0 || rows == 0 || n == 0 || rows > (size_t)INT32_MAX / 256 || n > (size_t)INT32_MAX / 256)
+        return fail(DR_ERR_INVALID, "%s: bad sizes, compute units or NULL kernel", who);
+    *kernel = dr::mx_plan(gated != 0, act_format == DR_MX_E4M3 && !gated && dtype == DR_DTYPE_F32, (int)rows, (int)cols, (int)n, n_cu);
+    return DR_OK;
+}
+
 int dr_cache_update_seq(dr_step_cache* cache, size_t batch, const int32_t* seq, size_t n) {
     if (!cache) return fail(DR_ERR_INVALID, "dr_cache_update_seq: cache is NULL");
     if (batch >= cache->n_batch) return fail(DR_ERR_INVALID, "dr_cache_update_seq: batch %zu >= %zu", batch, cache->n_batch);

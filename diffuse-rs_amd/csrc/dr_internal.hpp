@@ -476,6 +476,20 @@ struct MxMatArgs {
     int n_cu;
 };
 hipError_t launch_mx_matmul(const MxMatArgs& a, hipStream_t st);
-hipError_t launch_mx_tile(const MxMatArgs& a, hipStream_t st);
+// Its kernels: mx_ring_kernel with up to 4 or 16 activation rows or tiles of 16 x 32 to 64 x
+// 64 (weight by activation rows; gated: twice the output columns), mx_tile_kernel above that.
+enum MxKernel : int {
+    MX_KERNEL_4 = 0,
+    MX_KERNEL_16 = 1,
+    MX_KERNEL_16x32 = 2,
+    MX_KERNEL_32x32 = 3,
+    MX_KERNEL_64x64_EXACT = 4,
+    MX_KERNEL_64x64 = 5,
+    MX_KERNEL_64x128 = 6,
+    MX_KERNEL_256x128 = 7,
+    MX_KERNEL_256x256 = 8,
+};
+int mx_plan(bool gated, bool exact, int rows, int cols, int n, int n_cu);
+hipError_t launch_mx_tile(int kernel, const MxMatArgs& a, hipStream_t st);
 
 }  // namespace dr

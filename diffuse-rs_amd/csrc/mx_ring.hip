@@ -18,6 +18,8 @@
 // behind the loads.  A product does not depend on the order of the columns, so
 // the MFMA's k index is whatever both operands agree on: lane group g takes block g
 // of a step's four, and instruction j multiplies the blocks' values 8 j .. 8 j + 7.
+#include <climits>
+
 #include "mx_common.hpp"
 
 namespace dr {
@@ -285,26 +287,87 @@ hipError_t ring(const MxMatArgs& a, hipStream_t st) {
     return hipGetLastError();
 }
 
-//                  AF, gated, exact, MT, NT, AR, SK, STAGES, WAVES
-template <int AF>
-hipError_t few(const MxMatArgs& a, hipStream_t st) {
-    constexpr bool X = AF == MX_E4M3;
-    if (a.gated) {
-        if (a.n <= 4) return ring<RingGeom<AF, true, X, 4, 1, 4, 2, 3, 4>>(a, st);
-        return ring<RingGeom<AF, true, X, 4, 1, 16, 2, 3, 4>>(a, st);
+//                              AF, gated, exact, MT, NT, AR, SK, STAGES, WAVES
+template <int AF, bool X>
+hipError_t launch(int kernel, const MxMatArgs& a, hipStream_t st) {
+    // One row through 2 x 12288 x 4096: 12.3 us (4.3 TB/s of weights), 4096 x 12288: 7.1 us;
+    // a third stage 15.2 and 7.6: fewer workgroups fit on a CU.
+    if constexpr (X || AF == MX_E2M1) {
+        if (kernel == MX_KERNEL_4)
+            return a.gated ? ring<RingGeom<AF, true, X, 4, 1, 4, 2, 2, 4>>(a, st) : ring<RingGeom<AF, false, X, 1, 1, 4, 2, 2, 8>>(a, st);
+        if (kernel == MX_KERNEL_16)
+            return a.gated ? ring<RingGeom<AF, true, X, 4, 1, 16, 2, 2, 4>>(a, st) : ring<RingGeom<AF, false, X, 1, 1, 16, 2, 2, 8>>(a, st);
     }
-    if (a.n <= 4) return ring<RingGeom<AF, false, X, 1, 1, 4, 2, 4, 8>>(a, st);
-    if (a.n <= 16) return ring<RingGeom<AF, false, X, 1, 1, 16, 2, 2, 8>>(a, st);
-    return ring<RingGeom<AF, false, X, 4, 4, 64, 1, 3, 4>>(a, st);
+    if constexpr (X) {
+        if (kernel == MX_KERNEL_64x64_EXACT) return ring<RingGeom<AF, false, X, 4, 4, 64, 1, 1, 8>>(a, st);
+    } else {
+        if (a.gated && kernel == MX_KERNEL_32x32) return ring<RingGeom<AF, true, X, 4, 2, 32, 1, 2, 4>>(a, st);
+    }
+    if (kernel == MX_KERNEL_16x32) return ring<RingGeom<AF, false, X, 1, 2, 32, 2, 1, 8>>(a, st);
+    if (kernel == MX_KERNEL_32x32) return ring<RingGeom<AF, false, X, 2, 2, 32, 1, 2, 8>>(a, st);
+    return hipErrorInvalidValue;
 }
 
 }  // namespace
 
+// The kernel for a product.  Up to 16 rows: strips of 16 weight rows (gated: 32 of
+// either projection), with 4 or 16 activation rows staged.  More: the kernel whose
+// estimate is least.  An estimate is a start and, for each round of workgroups that
+// the device holds at once, a time per 128 columns; nanoseconds fitted to 17 to 2048
+// rows through 1024 x 2048 to 18944 x 3584, which they meet to about 20 %:
+//                         start  per round and 128 columns
+//   16 x 32                2500    90   4096 x 4096, 32 rows 5.5 us, 4096 x 12288 10.7
+//   32 x 32                2500   110   (gated 160) 64 rows 6.1 and 13.2; 12288 x 4096 gated, 64 rows 18.1
+//   64 x 64, bf16 MFMA     2500   340   f32 sums of 8 bit codes; 256 rows 13.5 and 30
+//   64 x 64                2500   220   256 rows 9.7 and 21.9
+//   64 x 64 gated, 2 a CU  2500   500   12288 x 4096, 128 rows 18.9 us
+//   64 x 128 gated, 2 a CU 2500   880   (540 where one is enough) 512 rows 49, 256 rows 30
+//   256 x 128              4000   880   (gated: 128 output columns; 700 where at most 3/4 of the CUs have
+//                                       one) 2048 rows 33 and 81, 1024 rows 26 and 65; gated 256 rows 27
+//   256 x 256              8000  1350   4096 x 12288, 4096 rows 155
+// Both sides of a step: 12288 x 4096 gated, 256 rows: 256 x 128 27 us, 256 x 256 44,
+// 64 x 128 30, 64 x 64 34; 2048 rows: 173, 156, 184, 222.
+int mx_plan(bool gated, bool exact, int rows, int cols, int n, int n_cu) {
+    if (n <= 16) return n <= 4 ? MX_KERNEL_4 : MX_KERNEL_16;
+    const long steps = (cols + 127) / 128;
+    int best = 0;
+    long least = LONG_MAX;
+    auto tiles = [&](int columns, int acts) { return (long)((rows + columns - 1) / columns) * ((n + acts - 1) / acts); };
+    auto offer = [&](int kernel, int columns, int acts, int per_cu, long start, long step) {
+        const long t = start + (tiles(columns, acts) + (long)per_cu * n_cu - 1) / ((long)per_cu * n_cu) * steps * step;
+        if (t < least) least = t, best = kernel;
+    };
+    if (gated) {
+        offer(MX_KERNEL_32x32, 32, 32, 1, 2500, 160);
+        offer(MX_KERNEL_64x64, 64, 64, 2, 2500, 500);
+        offer(MX_KERNEL_64x128, 64, 128, 2, 2500, tiles(64, 128) <= n_cu ? 540 : 880);
+        offer(MX_KERNEL_256x128, 128, 128, 1, 4000, 4 * tiles(128, 128) <= 3 * n_cu ? 700 : 880);
+        offer(MX_KERNEL_256x256, 128, 256, 1, 8000, 1350);
+    } else {
+        offer(MX_KERNEL_16x32, 16, 32, 1, 2500, 90);
+        offer(MX_KERNEL_32x32, 32, 32, 1, 2500, 110);
+        if (exact) {
+            offer(MX_KERNEL_64x64_EXACT, 64, 64, 1, 2500, 340);
+        } else {
+            offer(MX_KERNEL_64x64, 64, 64, 1, 2500, 220);
+            offer(MX_KERNEL_256x128, 256, 128, 1, 4000, 4 * tiles(256, 128) <= 3 * n_cu ? 700 : 880);
+            offer(MX_KERNEL_256x256, 256, 256, 1, 8000, 1350);
+        }
+    }
+    return best;
+}
+
 hipError_t launch_mx_matmul(const MxMatArgs& a, hipStream_t st) {
     if (a.n <= 0 || a.rows <= 0) return hipSuccess;
-    // f32 sums of 8 bit codes: the bf16 MFMA's
-    if (a.n > 16 && (a.gated || a.bf16 || a.act.format == MX_E2M1)) return launch_mx_tile(a, st);
-    return a.act.format == MX_E2M1 ? few<MX_E2M1>(a, st) : few<MX_E4M3>(a, st);
+    const bool eight = a.act.format == MX_E4M3;
+    // f32 sums of 8 bit codes stay on the bf16 MFMA; so do bf16 sums and the gated block up
+    // to 16 rows, where the conversions hide behind the weights.
+    const bool exact = eight && !a.gated && !a.bf16;
+    const int kernel = mx_plan(a.gated, exact, a.rows, a.cols, a.n, a.n_cu);
+    if (kernel > MX_KERNEL_64x64_EXACT) return launch_mx_tile(kernel, a, st);
+    if (!eight) return launch<MX_E2M1, false>(kernel, a, st);
+    if (exact || kernel <= MX_KERNEL_16) return launch<MX_E4M3, true>(kernel, a, st);
+    return launch<MX_E4M3, false>(kernel, a, st);
 }
 
 }  // namespace dr

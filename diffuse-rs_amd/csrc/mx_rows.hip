@@ -82,16 +82,15 @@ __global__ __launch_bounds__(256) void mx_norm_kernel(const MxNormArgs a) {
     __shared__ double s_part[4];
     const size_t row = blockIdx.x;
     const size_t xo = row * a.x_stride, ro = row * (size_t)a.cols;
-    float h[NV][8];
+    float h[NV][8], w[NV][8];
     double ss = 0.0;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
         const int at = (v * 256 + (int)threadIdx.x) * 8;
-        if (at >= a.cols) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) h[v][i] = 0.0f;
-            continue;
-        }
+        for (int i = 0; i < 8; ++i) h[v][i] = 0.0f, w[v][i] = 1.0f;
+        if (at >= a.cols) continue;
+        if (a.w) load8<false>(a.w, at, w[v]);  // (on its way while the squares are summed)
         load8<BF16>(a.x, xo + at, h[v]);
         if (a.residual) {
             float r[8];
@@ -112,11 +111,9 @@ __global__ __launch_bounds__(256) void mx_norm_kernel(const MxNormArgs a) {
         const int at = (v * 256 + (int)threadIdx.x) * 8;
         float y[8];
         uint32_t m = 0;
-        float w[8] = {1, 1, 1, 1, 1, 1, 1, 1};
-        if (a.w && at < a.cols) load8<false>(a.w, at, w);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            y[i] = h[v][i] * scale * w[i];
+            y[i] = h[v][i] * scale * w[v][i];
             m = max(m, __float_as_uint(y[i]) & 0x7fffffffu);
         }
         const int byte = mx_scale_byte<FMT>(quad_max(m));

@@ -324,7 +324,7 @@ __global__ __launch_bounds__(G::THREADS, G::PER_SIMD) void mx_tile_kernel(const 
                 uint32_t m = 0;
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                    const float v = mx_act(acc[q][e / 4][j][e % 4], a.fn) * acc[q + 1][e / 4][j][e % 4];
+                    const float v = mx_act_fast(acc[q][e / 4][j][e % 4], a.fn) * acc[q + 1][e / 4][j][e % 4];
                     x[e / 8][e % 8] = v;
                     m = max(m, __float_as_uint(v) & 0x7fffffffu);
                 }
@@ -356,23 +356,32 @@ hipError_t tile(const MxMatArgs& a, hipStream_t st) {
     return hipGetLastError();
 }
 
+//                              AF, gated, WM, Q, WN, TN, SB, STAGES
 template <int AF, bool GATED>
-hipError_t tiles(const MxMatArgs& a, hipStream_t st) {
-    constexpr int BIG = AF == MX_E4M3 ? 3 : 4;
-    const long cols = GATED ? 2l * a.rows : a.rows;
-    const long big = (cols + 255) / 256 * ((a.n + 255) / 256);
-    if (big >= a.n_cu / 2) return tile<TileGeom<AF, GATED, 2, 2, 4, 4, 1, BIG>>(a, st);
-    if constexpr (GATED)
-        return tile<TileGeom<AF, GATED, 1, 2, 4, 2, 1, 3>>(a, st);
-    else
-        return tile<TileGeom<AF, GATED, 1, 1, 4, 1, 2, 3>>(a, st);
+hipError_t tiles(int kernel, const MxMatArgs& a, hipStream_t st) {
+    constexpr bool EIGHT = AF == MX_E4M3;
+    switch (kernel) {
+        case MX_KERNEL_64x64:
+            if constexpr (GATED)
+                return tile<TileGeom<AF, true, 1, 2, 4, 1, 2, 2>>(a, st);
+            else
+                return tile<TileGeom<AF, false, 1, 1, 4, 1, 2, 4>>(a, st);
+        case MX_KERNEL_64x128:
+            if constexpr (GATED) return tile<TileGeom<AF, true, 1, 2, 4, 2, 1, 3>>(a, st);
+            return hipErrorInvalidValue;
+        case MX_KERNEL_256x128: return tile<TileGeom<AF, GATED, 2, 2, 4, 2, 2, 2>>(a, st);
+        // 8 bit codes: three stages of 128 columns fill LDS.  4 bit: two of 256 (2553 rows
+        // through 18944 x 3584 124 us, three of 128 130 us).
+        case MX_KERNEL_256x256: return tile<TileGeom<AF, GATED, 2, 2, 4, 4, EIGHT ? 1 : 2, EIGHT ? 3 : 2>>(a, st);
+        default: return hipErrorInvalidValue;
+    }
 }
 
 }  // namespace
 
-hipError_t launch_mx_tile(const MxMatArgs& a, hipStream_t st) {
-    if (a.act.format == MX_E4M3) return a.gated ? tiles<MX_E4M3, true>(a, st) : tiles<MX_E4M3, false>(a, st);
-    return a.gated ? tiles<MX_E2M1, true>(a, st) : tiles<MX_E2M1, false>(a, st);
+hipError_t launch_mx_tile(int kernel, const MxMatArgs& a, hipStream_t st) {
+    if (a.act.format == MX_E4M3) return a.gated ? tiles<MX_E4M3, true>(kernel, a, st) : tiles<MX_E4M3, false>(kernel, a, st);
+    return a.gated ? tiles<MX_E2M1, true>(kernel, a, st) : tiles<MX_E2M1, false>(kernel, a, st);
 }
 
 }  // namespace dr

@@ -189,6 +189,7 @@ _SIGS = {
     "dr_debug_alloc_count": (ctypes.c_long, []),
     "dr_debug_ring_tiles": (_I, [_SZ, _SZ, _SZ, ctypes.c_longlong, ctypes.c_longlong, ctypes.c_longlong, _SZ,
                                  ctypes.POINTER(_I), ctypes.POINTER(_I), ctypes.POINTER(_I)]),
+    "dr_debug_mx_plan": (_I, [_I, _I, _I, _SZ, _SZ, _SZ, _I, ctypes.POINTER(_I)]),
     "dr_debug_qmm_plan": (_I, [_I, _SZ, _SZ, _SZ, _I, ctypes.POINTER(_I), c_size_p, c_size_p]),
 }
 
@@ -746,3 +747,11 @@ def mx_gated(ctx: Context, gate: MxRows, up: MxRows, rows: int, cols: int, act: 
              activation: int = ACT_SILU) -> None:
     """The gated projections: f(act gate^T) * (act up^T), quantised (dr_mx_gated)."""
     _check(ctx.lib.dr_mx_gated(ctx.h, gate.c, up.c, rows, cols, act.c, n, activation, out.c))
+
+
+def mx_plan(rows: int, cols: int, n: int, gated: bool = False, act_format: int = MX_E4M3, dtype: int = DTYPE_F32,
+            n_cu: int = 256) -> int:
+    """The kernel of mx_matmul or mx_gated for these sizes (dr_debug_mx_plan); host-only."""
+    k = ctypes.c_int()
+    _check(load().dr_debug_mx_plan(1 if gated else 0, act_format, dtype, rows, cols, n, n_cu, ctypes.byref(k)))
+    return k.value

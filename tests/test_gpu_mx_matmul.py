@@ -32,18 +32,26 @@ def acts(rng, n, cols, fmt):
     return mx.quantise((rng.standard_normal((n, cols)) * np.exp(0.8 * rng.standard_normal(cols))).astype(np.float32), fmt)
 
 
-def product(w, a, fmt, cols, exact_sums):
-    """(sums, what each may be off by), f64."""
+def product(w, a, fmt, cols, exact_sums, dev=None):
+    """(sums, sums of magnitudes, what each sum may be off by), f64 (large ones on the device)."""
     wv, av = mx.values(*w, dr.MX_E2M1, cols), mx.values(*a, fmt, cols)
-    s, p = av @ wv.T, np.abs(av) @ np.abs(wv).T
+    if dev is not None and wv.size * av.shape[0] > 1 << 28:
+        t = dev.t
+        x, y = t.from_numpy(av).cuda(), t.from_numpy(np.ascontiguousarray(wv.T)).cuda()
+        s, p = (x @ y).cpu().numpy(), (x.abs() @ y.abs()).cpu().numpy()
+    else:
+        s, p = av @ wv.T, np.abs(av) @ np.abs(wv).T
     tol = 4 * np.sqrt(cols) * 2.0**-23 * p
     if not exact_sums:
         tol = tol + cols * 2.0**-18 * np.abs(av).max(-1)[:, None] * np.abs(wv).max(-1)[None]
     return s, p, tol
 
 
-SIZES = [(1, 1, 32), (1, 16, 512), (1, 257, 544), (3, 100, 1056), (16, 64, 2048), (17, 33, 96), (40, 130, 4096), (70, 48, 1120),
-         (129, 300, 640), (260, 520, 416), (513, 272, 1152)]
+# Up to 4 and 16 rows, and tiles of 16 x 32, 32 x 32, 64 x 64, 256 x 128 and 256 x 256
+# (tests/test_mx_refusals.py checks that no kernel is left out).
+SIZES = [(1, 1, 32), (1, 16, 512), (1, 257, 544), (3, 100, 1056), (4, 33, 1024), (5, 48, 96), (16, 64, 2048), (17, 33, 96),
+         (40, 130, 4096), (70, 48, 1120), (129, 300, 640), (129, 1028, 544), (260, 520, 416), (513, 272, 1152), (513, 1028, 544),
+         (777, 1028, 32), (513, 8200, 544), (2060, 4100, 1184)]
 
 
 @pytest.mark.parametrize("fmt", list(FMTS))
@@ -57,7 +65,7 @@ def test_matmul(dev, fmt, bf16, n, rows, cols):
     w[1][:, cols // 32:] = 255  # bytes between scale rows are no scales
     a[1][:, cols // 32:] = 255
     dtype = dr.DTYPE_BF16 if bf16 else dr.DTYPE_F32
-    s, p, tol = product(w, a, fmt, cols, exact_sums=not bf16)
+    s, p, tol = product(w, a, fmt, cols, not bf16, dev)
     half = 2.0**-8 if bf16 else 2.0**-24
     res = rng.standard_normal((n, rows)).astype(np.float32)
     res = mx.bf16(res) if bf16 else res
@@ -81,7 +89,7 @@ def test_matmul(dev, fmt, bf16, n, rows, cols):
     # the bound sees one block of 32 columns missing
     cut = (a[0].copy(), a[1].copy())
     cut[0][:, -(16 if fmt == dr.MX_E2M1 else 32):] = 0
-    assert (np.abs(product(w, cut, fmt, cols, True)[0] - s) > tol).any()
+    assert (np.abs(product(w, cut, fmt, cols, True, dev)[0] - s) > tol).any()
 
 
 @pytest.mark.parametrize("fmt", list(FMTS))
@@ -101,9 +109,27 @@ def test_gated(dev, fmt, to, fn, n, rows, cols):
     check_gated(gate, up, a, fmt, cols, fn, codes, scales, to)
 
 
-def check_gated(gate, up, a, fmt, cols, fn, codes, scales, to):
-    g, _, dg = product(gate, a, fmt, cols, False)
-    u, _, du = product(up, a, fmt, cols, False)
+# tiles of 64 x 64, 64 x 128, 256 x 128 and 256 x 256
+LARGE_GATED = [(129, 6176, 544), (129, 12320, 544), (513, 4128, 1056), (1030, 6176, 2080)]
+
+
+@pytest.mark.parametrize("fmt,to,fn", [("e4m3", "e4m3", dr.ACT_SILU), ("e2m1", "e2m1", dr.ACT_GELU)], ids=["8bit", "4bit"])
+@pytest.mark.parametrize("n,rows,cols", LARGE_GATED)
+def test_gated_large(dev, fmt, to, fn, n, rows, cols):
+    fmt, to = FMTS[fmt], FMTS[to]
+    say(f"gated fmt {fmt} to {to} fn {fn} n {n} rows {rows} cols {cols}")
+    rng = np.random.default_rng(n + rows + cols)
+    gate, up, a = weights(rng, rows, cols), weights(rng, rows, cols), acts(rng, n, cols, fmt)
+    out = empty_rows(dev, n, rows, to)
+    dr.mx_gated(dev.ctx, put_rows(dev, *gate, dr.MX_E2M1), put_rows(dev, *up, dr.MX_E2M1), rows, cols, put_rows(dev, *a, fmt), n,
+                out, activation=fn)
+    codes, scales = get_rows(dev, out, n, rows)
+    check_gated(gate, up, a, fmt, cols, fn, codes, scales, to, dev)
+
+
+def check_gated(gate, up, a, fmt, cols, fn, codes, scales, to, dev=None):
+    g, _, dg = product(gate, a, fmt, cols, False, dev)
+    u, _, du = product(up, a, fmt, cols, False, dev)
     f = mx.act(g, fn)
     # |f'| <= 1.13 for both; f itself: e^z of |z| <= 100 or so to (|z| + 4) 2^-24, four more roundings; the product one
     df = 1.13 * dg + np.abs(f) * (np.abs(2 * g) + 2 * np.abs(g) ** 3 * 0.08 + 10) * 2.0**-24
