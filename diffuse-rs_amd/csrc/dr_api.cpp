@@ -1204,6 +1204,9 @@ int dr_quantize_q8k(dr_ctx* ctx, const float* act, size_t n, size_t cols, void* 
 
 // Largest row of microscaled values (32-bit offsets within a tile of 256 rows).
 static constexpr size_t MX_COLS = (size_t)1 << 22;
+// Most blocks of a quantisation (four lanes each, fewer than 2^32 in a grid), rows of a
+// product's operands, and outputs of a product (its workgroups' lanes fewer than 2^32).
+static constexpr size_t MX_BLOCKS = ((size_t)1 << 30) - 64, MX_ROWS = (size_t)INT32_MAX / 256, MX_OUTPUTS = (size_t)1 << 34;
 
 static int mx_cols(const char* who, const char* what, size_t cols) {
     if (cols == 0 || cols % 32 != 0 || cols > MX_COLS)
@@ -1248,7 +1251,7 @@ int dr_mx_quantize(dr_ctx* ctx, const void* x, int dtype, size_t n, size_t cols,
     DR_CHECK(mx_rows(who, "out", out, a.rows));
     if (!x) return fail(DR_ERR_INVALID, "%s: x is NULL", who);
     DR_CHECK(mx_stride(who, x, dtype, cols, x_stride));
-    if (n > ((size_t)1 << 30) / (cols / 32) || x_stride > SIZE_MAX / 4 / n)
+    if (n > MX_BLOCKS / (cols / 32) || x_stride > SIZE_MAX / 4 / n)
         return fail(DR_ERR_INVALID, "%s: %zu x %zu too large", who, n, cols);
     DR_CHECK(use_device(ctx));
     a.x = x;
@@ -1270,7 +1273,7 @@ int dr_mx_dequantize(dr_ctx* ctx, const dr_mx_rows* rows, size_t n, size_t cols,
     dr::MxConvertArgs a{};
     DR_CHECK(mx_rows(who, "rows", rows, a.rows));
     if (!out || ((uintptr_t)out & 15)) return fail(DR_ERR_INVALID, "%s: out is NULL or not 16-byte aligned", who);
-    if (n > ((size_t)1 << 30) / (cols / 32)) return fail(DR_ERR_INVALID, "%s: %zu x %zu too large", who, n, cols);
+    if (n > MX_BLOCKS / (cols / 32)) return fail(DR_ERR_INVALID, "%s: %zu x %zu too large", who, n, cols);
     DR_CHECK(use_device(ctx));
     a.out = out;
     a.n = (uint32_t)n;
@@ -1296,7 +1299,7 @@ int dr_rms_norm_mx(dr_ctx* ctx, const void* x, const void* residual, void* sum, 
         return fail(DR_ERR_INVALID, "%s: residual, sum and w must be 16-byte aligned", who);
     if (sum == x && x_stride != cols)
         return fail(DR_ERR_INVALID, "%s: sum is x, whose rows are %zu apart and not %zu", who, x_stride, cols);
-    if (n > (size_t)INT32_MAX / 256 || x_stride > SIZE_MAX / 4 / n)
+    if (n > UINT32_MAX / (cols <= 16384 ? 256 : 1024) || x_stride > SIZE_MAX / 4 / n)
         return fail(DR_ERR_INVALID, "%s: %zu x %zu too large", who, n, cols);
     DR_CHECK(use_device(ctx));
     a.x = x;
@@ -1320,7 +1323,7 @@ static int mx_operands(const char* who, const dr_mx_rows* w, size_t rows, size_t
     DR_CHECK(mx_rows(who, "act", act, a.act));
     if (a.w.format != DR_MX_E2M1)
         return fail(DR_ERR_UNSUPPORTED, "%s: weights of format %d not built (DR_MX_E2M1 = 0)", who, a.w.format);
-    if (rows > (size_t)INT32_MAX / 256 || n > (size_t)INT32_MAX / 256 || (rows + 15) / 16 * ((n + 15) / 16) > (size_t)INT32_MAX)
+    if (rows > MX_ROWS || n > MX_ROWS || rows > MX_OUTPUTS / n)
         return fail(DR_ERR_INVALID, "%s: %zu x %zu x %zu too large", who, n, rows, cols);
     a.rows = (int)rows;
     a.cols = (int)cols;
@@ -1379,7 +1382,7 @@ int dr_debug_mx_plan(int gated, int act_format, int dtype, size_t rows, size_t c
     const char* who = "dr_debug_mx_plan";
     DR_CHECK(mx_dtype(who, dtype));
     DR_CHECK(mx_cols(who, "cols", cols));
-    if (!kernel || n_cu <= 0 || rows == 0 || n == 0 || rows > (size_t)INT32_MAX / 256 || n > (size_t)INT32_MAX / 256)
+    if (!kernel || n_cu <= 0 || rows == 0 || n == 0 || rows > MX_ROWS || n > MX_ROWS)
         return fail(DR_ERR_INVALID, "%s: bad sizes, compute units or NULL kernel", who);
     *kernel = dr::mx_plan(gated != 0, act_format == DR_MX_E4M3 && !gated && dtype == DR_DTYPE_F32, (int)rows, (int)cols, (int)n, n_cu);
     return DR_OK;

@@ -438,7 +438,7 @@ struct MxConvertArgs {
     void* out;      // dequantise: contiguous rows
     MxRows rows;
     size_t x_stride;
-    uint32_t n, blocks;  // rows, blocks of a row; n * blocks < 2^30
+    uint32_t n, blocks;  // rows, blocks of a row; n * blocks * 4 lanes < 2^32
     int bf16;            // x, out: bf16 rather than f32
 };
 hipError_t launch_mx_quantize(const MxConvertArgs& a, hipStream_t st);

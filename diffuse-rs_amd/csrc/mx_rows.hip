@@ -6,6 +6,7 @@ namespace dr {
 namespace {
 
 // n / d for n < 2^31 (d == 1: m unused): m = ceil(2^(31 + s) / d), s = ceil(log2 d).
+// (m d is less than 2^s over 2^(31 + s), and n times that less than 2^(31 + s): the quotient is exact.)
 struct Div31 {
     uint32_t d, m, s;
     explicit Div31(uint32_t d_) : d(d_), m(0), s(0) {
