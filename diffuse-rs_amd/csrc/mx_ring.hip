@@ -6,9 +6,9 @@
 // With few rows the weights' bytes bound the product, or the latency of the few
 // steps a workgroup takes: what counts is how many bytes are under way, in as many
 // workgroups as a CU holds (direct loads into registers, with half as many waves: 21.5
-// us for one row through 2 x 12288 x 4096 against 12.3, 79 us for 256 rows through 4096 x
+// us for one row through 2 x 12288 x 4096 against 12.1, 79 us for 256 rows through 4096 x
 // 4096 against 13.3; the large copy's rate allows 11.2 and 3.9).  Each wave
-// keeps STAGES - 1 steps of weights, activations and scales in flight by LDS DMA
+// keeps STAGES steps of weights, activations and scales in flight by LDS DMA
 // (whole rows of 64 or 128 bytes, consecutive lanes on consecutive bytes), waits for
 // nobody but its own loads and meets the others once, at the end.
 //
@@ -137,14 +137,15 @@ __global__ __launch_bounds__(64 * G::WAVES) void mx_ring_kernel(const MxMatArgs 
             dma4(ras, at + G::SA_OFF + k * 256, 4 * ss < left ? vsa[k] : OUT_OF_RANGE, t * SK * 4);
     };
 
-    f32x4m acc[MT][NT] = {};
-    auto multiply = [&](int t, const uint8_t* st) __attribute__((always_inline)) {
+    // A step's operands, from LDS: weight tile i (block g of each 128 columns s), activation
+    // tile j, and the scale bytes of block g.
+    u32x4m cw[SK][MT], ca[SK][NT][AF == MX_E4M3 ? 2 : 1];
+    int sw[SK][MT], sa[SK][NT];
+    auto load = [&](int t, const uint8_t* st) __attribute__((always_inline)) {
 #pragma unroll
         for (int s = 0; s < SK; ++s) {
-            // the scale byte of block g; behind a row's last block the codes are 0 and so is this
+            // behind a row's last block the codes are 0 and so is its byte (the bytes there are no scales)
             const uint32_t sel = 4 * (SK * t + s) + g < nblk ? 0x0c0c0c00u | g : 0x0c0c0c0cu;
-            u32x4m ca[NT][AF == MX_E4M3 ? 2 : 1];
-            int sa[NT];
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
                 const int R = G::AR < 16 ? r & (G::AR - 1) : r;  // (the other rows' sums are not used)
@@ -152,61 +153,71 @@ __global__ __launch_bounds__(64 * G::WAVES) void mx_ring_kernel(const MxMatArgs 
                 const int x = turn<G::A_ROW, G::PAIRS>(R);
                 if constexpr (AF == MX_E4M3) {
                     const int c = 8 * s + (G::EXACT ? 2 * g : g);
-                    ca[j][0] = *reinterpret_cast<const u32x4m*>(row + (c ^ x) * 16);
-                    ca[j][1] = *reinterpret_cast<const u32x4m*>(row + ((c + (G::EXACT ? 1 : 4)) ^ x) * 16);
+                    ca[s][j][0] = *reinterpret_cast<const u32x4m*>(row + (c ^ x) * 16);
+                    ca[s][j][1] = *reinterpret_cast<const u32x4m*>(row + ((c + (G::EXACT ? 1 : 4)) ^ x) * 16);
                 } else {
-                    ca[j][0] = *reinterpret_cast<const u32x4m*>(row + ((4 * s + g) ^ x) * 16);
+                    ca[s][j][0] = *reinterpret_cast<const u32x4m*>(row + ((4 * s + g) ^ x) * 16);
                 }
-                sa[j] = (int)__builtin_amdgcn_perm(0, *reinterpret_cast<const uint32_t*>(st + G::SA_OFF + ((j * 16 + R) * SK + s) * 4), sel);
+                sa[s][j] = (int)__builtin_amdgcn_perm(0, *reinterpret_cast<const uint32_t*>(st + G::SA_OFF + ((j * 16 + R) * SK + s) * 4), sel);
             }
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                cw[s][i] = *reinterpret_cast<const u32x4m*>(st + (i * 16 + r) * G::W_ROW + ((4 * s + g) ^ turn<G::W_ROW>(r)) * 16);
+                sw[s][i] = (int)__builtin_amdgcn_perm(
+                    0, *reinterpret_cast<const uint32_t*>(st + G::SW_OFF + i / G::FT * G::NSM * 256 + ((i % G::FT * 16 + r) * SK + s) * 4), sel);
+            }
+        }
+    };
+    f32x4m acc[MT][NT] = {};
+    auto multiply = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int s = 0; s < SK; ++s) {
             bf16x8m oa[NT][4];
             if constexpr (G::EXACT) {
 #pragma unroll
                 for (int j = 0; j < NT; ++j) {
                     if constexpr (AF == MX_E4M3)
-                        operands8(ca[j], mx_scale(sa[j]), oa[j]);
+                        operands8(ca[s][j], mx_scale(sa[s][j]), oa[j]);
                     else
-                        operands4(ca[j][0], mx_scale(sa[j]), oa[j]);
+                        operands4(ca[s][j][0], mx_scale(sa[s][j]), oa[j]);
                 }
             }
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
-                const u32x4m cw =
-                    *reinterpret_cast<const u32x4m*>(st + (i * 16 + r) * G::W_ROW + ((4 * s + g) ^ turn<G::W_ROW>(r)) * 16);
-                const int sw = (int)__builtin_amdgcn_perm(
-                    0, *reinterpret_cast<const uint32_t*>(st + G::SW_OFF + i / G::FT * G::NSM * 256 + ((i % G::FT * 16 + r) * SK + s) * 4), sel);
+                const u32x4m& w = cw[s][i];
                 if constexpr (G::EXACT) {
                     bf16x8m ow[4];
-                    operands4(cw, mx_scale(sw), ow);
+                    operands4(w, mx_scale(sw[s][i]), ow);
 #pragma unroll
                     for (int q = 0; q < 4; ++q)
 #pragma unroll
                         for (int j = 0; j < NT; ++j)
                             acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ow[q], oa[j][q], acc[i][j], 0, 0, 0);
                 } else {
-                    const i32x8m ow = i32x8m{(int)cw[0], (int)cw[1], (int)cw[2], (int)cw[3], 0, 0, 0, 0};
+                    const i32x8m ow = i32x8m{(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
 #pragma unroll
                     for (int j = 0; j < NT; ++j) {
-                        const u32x4m &lo = ca[j][0], &hi = ca[j][AF == MX_E4M3 ? 1 : 0];
+                        const u32x4m &lo = ca[s][j][0], &hi = ca[s][j][AF == MX_E4M3 ? 1 : 0];
                         const i32x8m o = AF == MX_E4M3 ? i32x8m{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]}
                                                        : i32x8m{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], 0, 0, 0, 0};
-                        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(ow, o, acc[i][j], 4, AF == MX_E4M3 ? 0 : 4, 0, sw, 0, sa[j]);
+                        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(ow, o, acc[i][j], 4, AF == MX_E4M3 ? 0 : 4, 0, sw[s][i], 0, sa[s][j]);
                     }
                 }
             }
         }
     };
 
-    // wave w takes steps w, w + WAVES, ...
+    // Wave w takes steps w, w + WAVES, ...  A step's operands wait in registers while it is
+    // multiplied, so that its place in the ring is on its way again meanwhile.
 #pragma unroll
-    for (int s = 0; s < G::STAGES - 1; ++s) request(wave + s * WAVES, ring + s * G::STAGE);
+    for (int s = 0; s < G::STAGES; ++s) request(wave + s * WAVES, ring + s * G::STAGE);
     int cur = 0;
     for (int t = wave; t < steps; t += WAVES) {
-        const int next = cur == 0 ? G::STAGES - 1 : cur - 1;
-        wait_lds();  // the step before this one has been read: its place is free
-        request(t + (G::STAGES - 1) * WAVES, ring + next * G::STAGE);
         wait_vm<(G::STAGES - 1) * G::NI>();
-        multiply(t, s_mem + (wave * G::STAGES + cur) * G::STAGE);
+        load(t, s_mem + (wave * G::STAGES + cur) * G::STAGE);
+        wait_lds();
+        request(t + G::STAGES * WAVES, ring + cur * G::STAGE);
+        multiply();
         cur = cur == G::STAGES - 1 ? 0 : cur + 1;
     }
     wait_vm<0>();
@@ -293,13 +304,31 @@ hipError_t ring(const MxMatArgs& a, hipStream_t st) {
 //                              AF, gated, exact, MT, NT, AR, SK, STAGES, WAVES
 template <int AF, bool X>
 hipError_t launch(int kernel, const MxMatArgs& a, hipStream_t st) {
-    // One row through 2 x 12288 x 4096: 12.3 us (4.3 TB/s of weights), 4096 x 12288: 7.1 us;
-    // a third stage 15.2 and 7.6: fewer workgroups fit on a CU.
+    // One place in the ring (and a step in registers): one row through 2 x 12288 x 4096 12.1 us
+    // (4.4 TB/s of weights), 4096 x 12288 7.2, 16 rows 12.7 and 8.2; two places 13.2, 7.3,
+    // 15.9 and 8.7: fewer workgroups fit on a CU.  Where no CU gets a second workgroup and there
+    // are steps for all, twice the waves keep as many bytes under way as two would.  With weights
+    // that no cache holds: one row through 3584 x 18944 9.2 us (8 waves 12.0), 2048 x 8192 5.5
+    // (6.3), 2 x 4096 x 4096 7.8 (4 waves 9.4), 2 x 8192 x 4096 9.6 (11.6); with more columns
+    // they take away workgroups instead, 2 x 9216 x 4096 16 rows 17.3 (15.7), one row 5120 x 8192
+    // 9.1 (8.3), and with fewer steps they have none, 2 x 1024 x 1024 4.2 (4.0).
     if constexpr (X || AF == MX_E2M1) {
-        if (kernel == MX_KERNEL_4)
-            return a.gated ? ring<RingGeom<AF, true, X, 4, 1, 4, 2, 2, 4>>(a, st) : ring<RingGeom<AF, false, X, 1, 1, 4, 2, 2, 8>>(a, st);
-        if (kernel == MX_KERNEL_16)
-            return a.gated ? ring<RingGeom<AF, true, X, 4, 1, 16, 2, 2, 4>>(a, st) : ring<RingGeom<AF, false, X, 1, 1, 16, 2, 2, 8>>(a, st);
+        const int steps = (a.cols + 255) / 256;
+        const bool one = (a.rows + (a.gated ? 31 : 15)) / (a.gated ? 32 : 16) <= a.n_cu;
+        if (kernel == MX_KERNEL_4) {
+            if (a.gated && one && steps >= 8) return ring<RingGeom<AF, true, X, 4, 1, 4, 2, 1, 8>>(a, st);
+            if (a.gated) return ring<RingGeom<AF, true, X, 4, 1, 4, 2, 1, 4>>(a, st);
+            if (one && steps >= 32) return ring<RingGeom<AF, false, X, 1, 1, 4, 2, 1, 16>>(a, st);
+            return ring<RingGeom<AF, false, X, 1, 1, 4, 2, 1, 8>>(a, st);
+        }
+        if (kernel == MX_KERNEL_16) {
+            if (a.gated && one && steps >= 8) return ring<RingGeom<AF, true, X, 4, 1, 16, 2, 1, 8>>(a, st);
+            if (a.gated) return ring<RingGeom<AF, true, X, 4, 1, 16, 2, 1, 4>>(a, st);
+            // 16 rows' bytes and conversions are as much as 32 weight rows': where a CU gets more than
+            // 16 columns, it reads them once for 32 (8192 x 8192 11.1 us, 16 a time 13.5; 65536 x 4096
+            // 37.9 and 46.4; 4096 x 12288 13.4 and 10.7, half the CUs have none).
+            return one ? ring<RingGeom<AF, false, X, 1, 1, 16, 2, 1, 8>>(a, st) : ring<RingGeom<AF, false, X, 2, 1, 16, 2, 1, 8>>(a, st);
+        }
     }
     if constexpr (X) {
         if (kernel == MX_KERNEL_64x64_EXACT) return ring<RingGeom<AF, false, X, 4, 4, 64, 1, 1, 8>>(a, st);
@@ -307,7 +336,7 @@ hipError_t launch(int kernel, const MxMatArgs& a, hipStream_t st) {
         if (a.gated && kernel == MX_KERNEL_32x32) return ring<RingGeom<AF, true, X, 4, 2, 32, 1, 2, 4>>(a, st);
     }
     if (kernel == MX_KERNEL_16x32) return ring<RingGeom<AF, false, X, 1, 2, 32, 2, 1, 8>>(a, st);
-    if (kernel == MX_KERNEL_32x32) return ring<RingGeom<AF, false, X, 2, 2, 32, 1, 2, 8>>(a, st);
+    if (kernel == MX_KERNEL_32x32) return ring<RingGeom<AF, false, X, 2, 2, 32, 1, 1, 8>>(a, st);
     return hipErrorInvalidValue;
 }
 
@@ -320,9 +349,10 @@ hipError_t launch(int kernel, const MxMatArgs& a, hipStream_t st) {
 // rows through 1024 x 2048 to 18944 x 3584, which they meet to about 20 %:
 //                         start  per round and 128 columns
 //   16 x 32                2500    90   4096 x 4096, 32 rows 5.5 us, 4096 x 12288 10.7
-//   32 x 32                2500   110   (gated 160) 64 rows 6.1 and 13.2; 12288 x 4096 gated, 64 rows 18.1
+//   32 x 32                2500   110   (gated 160) 64 rows 6.3 and 13.1; 12288 x 4096 gated, 64 rows 18.8
 //   64 x 64, bf16 MFMA     2500   340   f32 sums of 8 bit codes; 256 rows 13.5 and 30
-//   64 x 64                2500   220   256 rows 9.7 and 21.9
+//   64 x 64                2500   220   256 rows 9.5 and 21.2
+//   64 x 128               4500   285   512 rows 13.3 and 31.4 (64 x 64: 17.6 and 40.6)
 //   64 x 64 gated, 2 a CU  2500   500   12288 x 4096, 128 rows 18.9 us
 //   64 x 128 gated, 2 a CU 2500   880   (540 where one is enough) 512 rows 49, 256 rows 30
 //   256 x 128              4000   880   (gated: 128 output columns; 700 where at most 3/4 of the CUs have
@@ -353,6 +383,7 @@ int mx_plan(bool gated, bool exact, int rows, int cols, int n, int n_cu) {
             offer(MX_KERNEL_64x64_EXACT, 64, 64, 1, 2500, 340);
         } else {
             offer(MX_KERNEL_64x64, 64, 64, 1, 2500, 220);
+            offer(MX_KERNEL_64x128, 64, 128, 1, 4500, 285);
             offer(MX_KERNEL_256x128, 256, 128, 1, 4000, 4 * tiles(256, 128) <= 3 * n_cu ? 700 : 880);
             offer(MX_KERNEL_256x256, 256, 256, 1, 8000, 1350);
         }

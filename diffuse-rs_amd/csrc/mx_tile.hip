@@ -376,8 +376,10 @@ hipError_t tiles(int kernel, const MxMatArgs& a, hipStream_t st) {
             else
                 return tile<TileGeom<AF, false, 1, 1, 4, 1, 2, 4>>(a, st);
         case MX_KERNEL_64x128:
-            if constexpr (GATED) return tile<TileGeom<AF, true, 1, 2, 4, 2, 1, 3>>(a, st);
-            return hipErrorInvalidValue;
+            if constexpr (GATED)
+                return tile<TileGeom<AF, true, 1, 2, 4, 2, 1, 3>>(a, st);
+            else
+                return tile<TileGeom<AF, false, 1, 1, 4, 2, 2, 3>>(a, st);
         case MX_KERNEL_256x128: return tile<TileGeom<AF, GATED, 2, 2, 4, 2, 2, 2>>(a, st);
         // 8 bit codes: three stages of 128 columns fill LDS.  4 bit: two of 256 (2553 rows
         // through 18944 x 3584 124 us, three of 128 130 us).

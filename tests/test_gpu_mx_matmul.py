@@ -47,11 +47,11 @@ def product(w, a, fmt, cols, exact_sums, dev=None):
     return s, p, tol
 
 
-# Up to 4 and 16 rows, and tiles of 16 x 32, 32 x 32, 64 x 64, 256 x 128 and 256 x 256
+# Up to 4 and 16 rows (many columns; more rows of weights than 16 a CU), and tiles of 16 x 32, 32 x 32, 64 x 64, 64 x 128, 256 x 128 and 256 x 256
 # (tests/test_mx_refusals.py checks that no kernel is left out).
-SIZES = [(1, 1, 32), (1, 16, 512), (1, 257, 544), (3, 100, 1056), (4, 33, 1024), (5, 48, 96), (16, 64, 2048), (17, 33, 96),
+SIZES = [(1, 1, 32), (1, 16, 512), (1, 257, 544), (3, 100, 1056), (2, 130, 8224), (4, 33, 1024), (5, 48, 96), (16, 64, 2048), (13, 4200, 320), (17, 33, 96),
          (40, 130, 4096), (70, 48, 1120), (129, 300, 640), (129, 1028, 544), (260, 520, 416), (513, 272, 1152), (513, 1028, 544),
-         (777, 1028, 32), (513, 8200, 544), (2060, 4100, 1184)]
+         (777, 1028, 32), (513, 8200, 544), (2060, 4100, 1184), (1030, 12290, 1216)]
 
 
 @pytest.mark.parametrize("fmt", list(FMTS))
@@ -95,7 +95,7 @@ def test_matmul(dev, fmt, bf16, n, rows, cols):
 @pytest.mark.parametrize("fmt", list(FMTS))
 @pytest.mark.parametrize("to", list(FMTS))
 @pytest.mark.parametrize("fn", [dr.ACT_SILU, dr.ACT_GELU], ids=["silu", "gelu"])
-@pytest.mark.parametrize("n,rows,cols", [(1, 32, 32), (1, 160, 4096), (5, 96, 544), (16, 64, 96), (33, 288, 1056), (150, 352, 640),
+@pytest.mark.parametrize("n,rows,cols", [(1, 32, 32), (1, 160, 4096), (2, 288, 2080), (5, 96, 544), (12, 288, 2080), (16, 64, 96), (33, 288, 1056), (150, 352, 640),
                                          (300, 96, 2048), (520, 544, 160)])
 def test_gated(dev, fmt, to, fn, n, rows, cols):
     fmt, to = FMTS[fmt], FMTS[to]
