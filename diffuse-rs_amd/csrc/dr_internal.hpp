@@ -483,11 +483,12 @@ enum MxKernel : int {
     MX_KERNEL_16 = 1,
     MX_KERNEL_16x32 = 2,
     MX_KERNEL_32x32 = 3,
-    MX_KERNEL_64x64_EXACT = 4,
-    MX_KERNEL_64x64 = 5,
-    MX_KERNEL_64x128 = 6,
-    MX_KERNEL_256x128 = 7,
-    MX_KERNEL_256x256 = 8,
+    MX_KERNEL_64x32 = 4,
+    MX_KERNEL_64x64_EXACT = 5,
+    MX_KERNEL_64x64 = 6,
+    MX_KERNEL_64x128 = 7,
+    MX_KERNEL_256x128 = 8,
+    MX_KERNEL_256x256 = 9,
 };
 int mx_plan(bool gated, bool exact, int rows, int cols, int n, int n_cu);
 hipError_t launch_mx_tile(int kernel, const MxMatArgs& a, hipStream_t st);

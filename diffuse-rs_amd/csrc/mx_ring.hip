@@ -337,6 +337,7 @@ hipError_t launch(int kernel, const MxMatArgs& a, hipStream_t st) {
     }
     if (kernel == MX_KERNEL_16x32) return ring<RingGeom<AF, false, X, 1, 2, 32, 2, 1, 8>>(a, st);
     if (kernel == MX_KERNEL_32x32) return ring<RingGeom<AF, false, X, 2, 2, 32, 1, 1, 8>>(a, st);
+    if (kernel == MX_KERNEL_64x32) return ring<RingGeom<AF, false, X, 4, 2, 32, 1, 1, 8>>(a, st);
     return hipErrorInvalidValue;
 }
 
@@ -349,17 +350,18 @@ hipError_t launch(int kernel, const MxMatArgs& a, hipStream_t st) {
 // rows through 1024 x 2048 to 18944 x 3584, which they meet to about 20 %:
 //                         start  per round and 128 columns
 //   16 x 32                2500    90   4096 x 4096, 32 rows 5.5 us, 4096 x 12288 10.7
-//   32 x 32                2500   110   (gated 160) 64 rows 6.3 and 13.1; 12288 x 4096 gated, 64 rows 18.8
+//   32 x 32                2500   110   (gated 200) 64 rows 6.3 and 13.1; 12288 x 4096 gated, 32 rows 15.3
+//   64 x 32                2500   170   (bf16 MFMA 185) 128 rows 8.1 and 18.3 (32 x 32: 9.4 and 22.4; 64 x 64: 9.5 and 21)
 //   64 x 64, bf16 MFMA     2500   340   f32 sums of 8 bit codes; 256 rows 13.5 and 30
-//   64 x 64                2500   220   256 rows 9.5 and 21.2
+//   64 x 64                2500   220   256 rows 9.7 and 21.2
 //   64 x 128               4500   285   512 rows 13.3 and 31.4 (64 x 64: 17.6 and 40.6)
-//   64 x 64 gated, 2 a CU  2500   500   12288 x 4096, 128 rows 18.9 us
-//   64 x 128 gated, 2 a CU 2500   880   (540 where one is enough) 512 rows 49, 256 rows 30
+//   64 x 64 gated, 2 a CU  2500   500   (385 where one is enough) 12288 x 4096, 128 rows 19.1 us, 64 rows 14.9
+//   64 x 128 gated, 2 a CU 2500   880   (490 where one is enough) 512 rows 49, 256 rows 29, 128 rows 17.8
 //   256 x 128              4000   880   (gated: 128 output columns; 700 where at most 3/4 of the CUs have
 //                                       one) 2048 rows 33 and 81, 1024 rows 26 and 65; gated 256 rows 27
 //   256 x 256              8000  1350   4096 x 12288, 4096 rows 155
 // Both sides of a step: 12288 x 4096 gated, 256 rows: 256 x 128 27 us, 256 x 256 44,
-// 64 x 128 30, 64 x 64 34; 2048 rows: 173, 156, 184, 222.
+// 64 x 128 29, 64 x 64 34; 2048 rows: 173, 156, 184, 222.
 int mx_plan(bool gated, bool exact, int rows, int cols, int n, int n_cu) {
     if (n <= 16) return n <= 4 ? MX_KERNEL_4 : MX_KERNEL_16;
     const long steps = (cols + 127) / 128;
@@ -371,14 +373,15 @@ int mx_plan(bool gated, bool exact, int rows, int cols, int n, int n_cu) {
         if (t < least) least = t, best = kernel;
     };
     if (gated) {
-        offer(MX_KERNEL_32x32, 32, 32, 1, 2500, 160);
-        offer(MX_KERNEL_64x64, 64, 64, 2, 2500, 500);
-        offer(MX_KERNEL_64x128, 64, 128, 2, 2500, tiles(64, 128) <= n_cu ? 540 : 880);
+        offer(MX_KERNEL_32x32, 32, 32, 1, 2500, 200);
+        offer(MX_KERNEL_64x64, 64, 64, 2, 2500, tiles(64, 64) <= n_cu ? 385 : 500);
+        offer(MX_KERNEL_64x128, 64, 128, 2, 2500, tiles(64, 128) <= n_cu ? 490 : 880);
         offer(MX_KERNEL_256x128, 128, 128, 1, 4000, 4 * tiles(128, 128) <= 3 * n_cu ? 700 : 880);
         offer(MX_KERNEL_256x256, 128, 256, 1, 8000, 1350);
     } else {
         offer(MX_KERNEL_16x32, 16, 32, 1, 2500, 90);
         offer(MX_KERNEL_32x32, 32, 32, 1, 2500, 110);
+        offer(MX_KERNEL_64x32, 64, 32, 1, 2500, exact ? 185 : 170);
         if (exact) {
             offer(MX_KERNEL_64x64_EXACT, 64, 64, 1, 2500, 340);
         } else {

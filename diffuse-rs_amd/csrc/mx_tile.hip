@@ -369,18 +369,24 @@ hipError_t tile(const MxMatArgs& a, hipStream_t st) {
 template <int AF, bool GATED>
 hipError_t tiles(int kernel, const MxMatArgs& a, hipStream_t st) {
     constexpr bool EIGHT = AF == MX_E4M3;
+    // Where no CU gets a second tile, a tile takes the LDS of two.  Weights that no cache holds,
+    // gated, 64 x 64 tiles: 64 rows through 12288 x 4096 17.4 us (two stages 23.3; 128 rows, two
+    // tiles a CU, 29.4 and 26.2), 64 x 128: 128 rows 22.6 (26.4; 512 rows 58 and 54).  Products, 64
+    // x 64: 256 rows through 4096 x 12288 27.0 (four stages of half as many columns 29.5).
+    auto one = [&](int columns, int acts) { return ((a.rows + columns - 1) / columns) * (long)((a.n + acts - 1) / acts) <= a.n_cu; };
     switch (kernel) {
         case MX_KERNEL_64x64:
             if constexpr (GATED)
-                return tile<TileGeom<AF, true, 1, 2, 4, 1, 2, 2>>(a, st);
+                return one(64, 64) ? tile<TileGeom<AF, true, 1, 2, 4, 1, 2, 3>>(a, st) : tile<TileGeom<AF, true, 1, 2, 4, 1, 2, 2>>(a, st);
             else
-                return tile<TileGeom<AF, false, 1, 1, 4, 1, 2, 4>>(a, st);
+                return tile<TileGeom<AF, false, 1, 1, 4, 1, 4, 3>>(a, st);
         case MX_KERNEL_64x128:
             if constexpr (GATED)
-                return tile<TileGeom<AF, true, 1, 2, 4, 2, 1, 3>>(a, st);
+                return one(64, 128) ? tile<TileGeom<AF, true, 1, 2, 4, 2, 2, 3>>(a, st) : tile<TileGeom<AF, true, 1, 2, 4, 2, 1, 3>>(a, st);
             else
                 return tile<TileGeom<AF, false, 1, 1, 4, 2, 2, 3>>(a, st);
-        case MX_KERNEL_256x128: return tile<TileGeom<AF, GATED, 2, 2, 4, 2, 2, 2>>(a, st);
+        // Stages that fill LDS: 4 bit codes, gated, 1024 rows through 12288 x 4096 72 us (two stages 79).
+        case MX_KERNEL_256x128: return tile<TileGeom<AF, GATED, 2, 2, 4, 2, 2, EIGHT ? 2 : 3>>(a, st);
         // 8 bit codes: three stages of 128 columns fill LDS.  4 bit: two of 256 (2553 rows
         // through 18944 x 3584 124 us, three of 128 130 us).
         case MX_KERNEL_256x256: return tile<TileGeom<AF, GATED, 2, 2, 4, 4, EIGHT ? 1 : 2, EIGHT ? 3 : 2>>(a, st);

@@ -682,8 +682,8 @@ int dr_debug_qmm_plan(int wtype, size_t rows, size_t cols, size_t n, int n_cu, i
 
 /* The kernel that dr_mx_matmul (gated == 0; dtype of out) or dr_mx_gated runs for these sizes
  * on a device of n_cu compute units: 0 and 1, strips for up to 4 and 16 activation rows; 2
- * to 8, tiles of 16 x 32, 32 x 32, 64 x 64 (bf16 MFMA), 64 x 64, 64 x 128, 256 x 128 and 256 x
- * 256 weight by activation rows.  Host-only. */
+ * to 9, tiles of 16 x 32, 32 x 32, 64 x 32, 64 x 64 (bf16 MFMA), 64 x 64, 64 x 128, 256 x 128
+ * and 256 x 256 weight by activation rows.  Host-only. */
 int dr_debug_mx_plan(int gated, int act_format, int dtype, size_t rows, size_t cols, size_t n, int n_cu, int* kernel);
 
 #ifdef __cplusplus

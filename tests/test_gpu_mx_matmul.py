@@ -47,11 +47,12 @@ def product(w, a, fmt, cols, exact_sums, dev=None):
     return s, p, tol
 
 
-# Up to 4 and 16 rows (many columns; more rows of weights than 16 a CU), and tiles of 16 x 32, 32 x 32, 64 x 64, 64 x 128, 256 x 128 and 256 x 256
-# (tests/test_mx_refusals.py checks that no kernel is left out).
-SIZES = [(1, 1, 32), (1, 16, 512), (1, 257, 544), (3, 100, 1056), (2, 130, 8224), (4, 33, 1024), (5, 48, 96), (16, 64, 2048), (13, 4200, 320), (17, 33, 96),
-         (40, 130, 4096), (70, 48, 1120), (129, 300, 640), (129, 1028, 544), (260, 520, 416), (513, 272, 1152), (513, 1028, 544),
-         (777, 1028, 32), (513, 8200, 544), (2060, 4100, 1184), (1030, 12290, 1216)]
+# Up to 4 and 16 rows (many columns; more rows of weights than 16 a CU), and tiles of 16 x 32, 32 x 32, 64 x 32, 64 x 64,
+# 64 x 128, 256 x 128 and 256 x 256 (tests/test_mx_refusals.py checks that no kernel is left out).
+SIZES = [(1, 1, 32), (1, 16, 512), (1, 257, 544), (3, 100, 1056), (2, 130, 8224), (4, 33, 1024), (5, 48, 96), (16, 64, 2048),
+         (13, 4200, 320), (17, 33, 96), (40, 130, 4096), (70, 48, 1120), (129, 300, 640), (129, 1028, 544), (260, 520, 416),
+         (120, 4028, 1120), (513, 272, 1152), (513, 1028, 544), (250, 4028, 2336), (777, 1028, 32), (513, 8200, 544), (513, 8200, 1312),
+         (2060, 4100, 1184), (1030, 12290, 1216)]
 
 
 @pytest.mark.parametrize("fmt", list(FMTS))
@@ -95,8 +96,8 @@ def test_matmul(dev, fmt, bf16, n, rows, cols):
 @pytest.mark.parametrize("fmt", list(FMTS))
 @pytest.mark.parametrize("to", list(FMTS))
 @pytest.mark.parametrize("fn", [dr.ACT_SILU, dr.ACT_GELU], ids=["silu", "gelu"])
-@pytest.mark.parametrize("n,rows,cols", [(1, 32, 32), (1, 160, 4096), (2, 288, 2080), (5, 96, 544), (12, 288, 2080), (16, 64, 96), (33, 288, 1056), (150, 352, 640),
-                                         (300, 96, 2048), (520, 544, 160)])
+@pytest.mark.parametrize("n,rows,cols", [(1, 32, 32), (1, 160, 4096), (2, 288, 2080), (5, 96, 544), (12, 288, 2080), (16, 64, 96),
+                                         (33, 288, 1056), (150, 352, 640), (300, 96, 2048), (520, 544, 160)])
 def test_gated(dev, fmt, to, fn, n, rows, cols):
     fmt, to = FMTS[fmt], FMTS[to]
     say(f"gated fmt {fmt} to {to} fn {fn} n {n} rows {rows} cols {cols}")
@@ -109,8 +110,8 @@ def test_gated(dev, fmt, to, fn, n, rows, cols):
     check_gated(gate, up, a, fmt, cols, fn, codes, scales, to)
 
 
-# tiles of 64 x 64, 64 x 128, 256 x 128 and 256 x 256
-LARGE_GATED = [(129, 6176, 544), (129, 12320, 544), (513, 4128, 1056), (1030, 6176, 2080)]
+# tiles of 64 x 64 and 64 x 128, one and two a CU, 256 x 128 and 256 x 256
+LARGE_GATED = [(100, 6176, 1184), (50, 18976, 544), (129, 6176, 1184), (129, 12320, 544), (513, 4128, 1056), (1030, 6176, 2080)]
 
 
 @pytest.mark.parametrize("fmt,to,fn", [("e4m3", "e4m3", dr.ACT_SILU), ("e2m1", "e2m1", dr.ACT_GELU)], ids=["8bit", "4bit"])

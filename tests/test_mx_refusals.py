@@ -159,13 +159,13 @@ def test_plan():
     from test_gpu_mx_matmul import LARGE_GATED, SIZES
 
     met = {dr.mx_plan(rows, cols, n, act_format=f, dtype=d) for n, rows, cols in SIZES for f in (0, 1) for d in (0, 1)}
-    assert met == set(range(9))
-    assert [dr.mx_plan(rows, cols, n, gated=True) for n, rows, cols in LARGE_GATED] == [5, 6, 7, 8]
+    assert met == set(range(10))
+    assert [dr.mx_plan(rows, cols, n, gated=True) for n, rows, cols in LARGE_GATED] == [6, 6, 7, 7, 8, 9]
     assert {dr.mx_plan(64, 512, n, gated=True) for n in (1, 4, 5, 16, 17, 100)} == {0, 1, 3}
     # f32 sums of 8 bit codes never take the block-scaled MFMA's kernels, others never the bf16 MFMA's tile
     for n in (1, 16, 17, 100, 1000, 10000):
-        assert dr.mx_plan(4096, 4096, n) <= 4
-        assert 4 not in (dr.mx_plan(4096, 4096, n, act_format=dr.MX_E2M1), dr.mx_plan(4096, 4096, n, dtype=dr.DTYPE_BF16))
+        assert dr.mx_plan(4096, 4096, n) <= 5
+        assert 5 not in (dr.mx_plan(4096, 4096, n, act_format=dr.MX_E2M1), dr.mx_plan(4096, 4096, n, dtype=dr.DTYPE_BF16))
     for bad in (dict(rows=0, cols=32, n=1), dict(rows=1, cols=31, n=1), dict(rows=1, cols=32, n=0), dict(rows=1, cols=32, n=1, n_cu=0),
                 dict(rows=1, cols=32, n=1, dtype=3), dict(rows=1 << 40, cols=32, n=1)):
         with pytest.raises(dr.DrError):
