@@ -305,8 +305,9 @@ hipError_t ring(const MxMatArgs& a, hipStream_t st) {
 template <int AF, bool X>
 hipError_t launch(int kernel, const MxMatArgs& a, hipStream_t st) {
     // One place in the ring (and a step in registers): one row through 2 x 12288 x 4096 12.1 us
-    // (4.4 TB/s of weights), 4096 x 12288 7.2, 16 rows 12.7 and 8.2; two places 13.2, 7.3,
-    // 15.9 and 8.7: fewer workgroups fit on a CU.  Where no CU gets a second workgroup and there
+    // (4.4 TB/s of weights, which the memory-side cache holds; 14.6 from memory), 4096 x 12288
+    // 7.2, 16 rows 12.7 and 8.2; two places 13.2, 7.3, 15.9 and 8.7: fewer workgroups fit on a
+    // CU.  Where no CU gets a second workgroup and there
     // are steps for all, twice the waves keep as many bytes under way as two would.  With weights
     // that no cache holds: one row through 3584 x 18944 9.2 us (8 waves 12.0), 2048 x 8192 5.5
     // (6.3), 2 x 4096 x 4096 7.8 (4 waves 9.4), 2 x 8192 x 4096 9.6 (11.6); with more columns
@@ -343,7 +344,7 @@ hipError_t launch(int kernel, const MxMatArgs& a, hipStream_t st) {
 
 }  // namespace
 
-// The kernel for a product.  Up to 16 rows: strips of 16 weight rows (gated: 32 of
+// The kernel for a product.  Up to 16 rows: strips of 16 or 32 weight rows (gated: 32 of
 // either projection), with 4 or 16 activation rows staged.  More: the kernel whose
 // estimate is least.  An estimate is a start and, for each round of workgroups that
 // the device holds at once, a time per 128 columns; nanoseconds fitted to 17 to 2048

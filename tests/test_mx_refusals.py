@@ -170,3 +170,20 @@ def test_plan():
                 dict(rows=1, cols=32, n=1, dtype=3), dict(rows=1 << 40, cols=32, n=1)):
         with pytest.raises(dr.DrError):
             dr.mx_plan(**bad)
+
+
+@pytest.mark.parametrize("gated", [False, True], ids=["product", "gated"])
+@pytest.mark.parametrize("dtype", [dr.DTYPE_F32, dr.DTYPE_BF16], ids=["f32", "bf16"])
+def test_grids(gated, dtype):
+    """The largest sizes that are taken launch fewer than 2^32 lanes."""
+    tile = {2: (16, 32), 3: (32, 32), 4: (64, 32), 5: (64, 64), 6: (64, 64), 7: (64, 128), 8: (128 if gated else 256, 128),
+            9: (128 if gated else 256, 256)}
+    most = (2**31 - 1) // 256
+    for n in [1, 4, 5, 16, 17, 31, 32, 33, 64, 65, 127, 129, 1000, 2047, 2048, 2049, 2080, 2081, 4000, 2**16, 2**20 + 1, most]:
+        rows = min(most, 2**34 // n)
+        for rows in {rows, rows - 31, rows // 2 + 1}:
+            rows = rows // 32 * 32 if gated else rows
+            kernel = dr.mx_plan(rows, 4096, n, gated=gated, dtype=dtype)
+            columns, acts = tile.get(kernel, (32 if gated else 16, n))
+            lanes = -(-rows // columns) * -(-n // acts) * (512 if kernel != 0 or not gated else 256)  # (or fewer)
+            assert lanes < 2**32, (n, rows, kernel)
