@@ -709,19 +709,48 @@ def mx_pitch(cols: int) -> int:
     return (cols // 32 + 3) // 4 * 4
 
 
+def _byte_plane(what: str, t):
+    """(t, False) where t is a device address or a contiguous tensor of one-byte
+    values; (a copy of its values in contiguous bytes, True) for strided ones and
+    for whole numbers of a wider type, as torch's arithmetic on codes leaves them."""
+    if t is None or isinstance(t, int):
+        return t, False
+    if t.element_size() == 1:
+        return (t, False) if t.is_contiguous() else (t.contiguous(), True)
+    if t.is_floating_point() or t.is_complex():
+        raise TypeError(f"{what}: {t.dtype} values are not bytes")
+    if bool(((t < 0) | (t > 255)).any()):
+        raise ValueError(f"{what}: {t.dtype} values that are no bytes (0 to 255)")
+    return t.byte().contiguous(), True
+
+
 class MxRows:
     """dr_mx_rows: device tensors (or addresses) of microscaled rows' codes
     ([n][cols / 2] bytes for MX_E2M1, [n][cols] for MX_E4M3) and scale bytes
-    ([n][mx_pitch(cols)])."""
+    ([n][mx_pitch(cols)]).  Contiguous tensors of a one-byte type are used in place.
+    Strided ones and whole numbers of a wider type (0 to 255) are copied into bytes
+    here, on torch's current stream, and such rows can be read but not written.
+    Other tensors, and tensors that are not on a GPU, are refused."""
 
     def __init__(self, codes, scales, format: int):
-        self.codes, self.scales, self.format = codes, scales, format  # (held: the struct has their addresses)
-        self.c = CMxRows(_ptr(codes), _ptr(scales), format)
+        for what, t in (("codes", codes), ("scales", scales)):
+            if t is not None and not isinstance(t, int) and not t.is_cuda:
+                raise TypeError(f"{what}: a tensor on {t.device}, not on a GPU")
+        (self.codes, a), (self.scales, b) = _byte_plane("codes", codes), _byte_plane("scales", scales)  # (held: the struct has their addresses)
+        self.format, self.copied = format, a or b
+        self.c = CMxRows(_ptr(self.codes), _ptr(self.scales), format)
+
+    def written(self) -> CMxRows:
+        """The struct, for a call that writes the rows."""
+        if self.copied:
+            raise TypeError("rows whose codes or scales are a copy of the given tensor cannot be written: "
+                            "give contiguous tensors of bytes")
+        return self.c
 
 
 def mx_quantize(ctx: Context, x, n: int, cols: int, out: MxRows, dtype: int = DTYPE_F32, stride: int = 0) -> None:
     """f32 or bf16 rows, ``stride`` elements apart (0: cols), into microscaled rows (dr_mx_quantize)."""
-    _check(ctx.lib.dr_mx_quantize(ctx.h, _ptr(x), dtype, n, cols, stride, out.c))
+    _check(ctx.lib.dr_mx_quantize(ctx.h, _ptr(x), dtype, n, cols, stride, out.written()))
 
 
 def mx_dequantize(ctx: Context, rows: MxRows, n: int, cols: int, out, dtype: int = DTYPE_F32) -> None:
@@ -734,7 +763,7 @@ def rms_norm_mx(ctx: Context, x, n: int, cols: int, out: MxRows, w=None, eps: fl
     """x + residual (into ``total`` where given), its RMSNorm with the gain w,
     quantised into ``out`` (dr_rms_norm_mx)."""
     _check(ctx.lib.dr_rms_norm_mx(ctx.h, _ptr(x), _ptr(residual) or None, _ptr(total) or None, dtype, n, cols, stride,
-                                  _ptr(w) or None, eps, out.c))
+                                  _ptr(w) or None, eps, out.written()))
 
 
 def mx_matmul(ctx: Context, w: MxRows, rows: int, cols: int, act: MxRows, n: int, out, residual=None,
@@ -746,7 +775,7 @@ def mx_matmul(ctx: Context, w: MxRows, rows: int, cols: int, act: MxRows, n: int
 def mx_gated(ctx: Context, gate: MxRows, up: MxRows, rows: int, cols: int, act: MxRows, n: int, out: MxRows,
              activation: int = ACT_SILU) -> None:
     """The gated projections: f(act gate^T) * (act up^T), quantised (dr_mx_gated)."""
-    _check(ctx.lib.dr_mx_gated(ctx.h, gate.c, up.c, rows, cols, act.c, n, activation, out.c))
+    _check(ctx.lib.dr_mx_gated(ctx.h, gate.c, up.c, rows, cols, act.c, n, activation, out.written()))
 
 
 def mx_plan(rows: int, cols: int, n: int, gated: bool = False, act_format: int = MX_E4M3, dtype: int = DTYPE_F32,
