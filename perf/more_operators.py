@@ -268,7 +268,7 @@ def _quantise(x, fmt):
         return y.to(torch.float8_e4m3fn).view(torch.uint8).reshape(n, cols), scales
     a = y.abs()
     code = ((a > 0.25).to(torch.uint8) + (a >= 0.75) + (a > 1.25) + (a >= 1.75) + (a > 2.5) + (a >= 3.5) + (a > 5)
-            + 8 * torch.signbit(y).to(torch.uint8)).reshape(n, cols // 2, 2)
+            + 8 * torch.signbit(y)).reshape(n, cols // 2, 2)
     return code[..., 0] + 16 * code[..., 1], scales
 
 
