@@ -1388,6 +1388,23 @@ int dr_debug_mx_plan(int gated, int act_format, int dtype, size_t rows, size_t c
     return DR_OK;
 }
 
+int dr_debug_mx_scale_end(size_t rows, size_t cols, size_t* end) {
+    const char* who = "dr_debug_mx_scale_end";
+    DR_CHECK(mx_cols(who, "cols", cols));
+    if (!end || rows == 0 || rows > MX_ROWS) return fail(DR_ERR_INVALID, "%s: bad sizes or NULL end", who);
+    // the last tile's rows (256 at most) end the plane
+    const size_t pitch = dr::mx_pitch(cols), first = rows > 256 ? rows - 256 : 0, bytes = (rows - first) * pitch;
+    size_t most = 0;
+    for (size_t r = 0; r < rows - first; ++r)
+        for (size_t c = 0; c * 512 < cols; ++c) {
+            const dr::MxScalePiece p = dr::mx_scale_piece((int)r, (int)pitch, (int)c);
+            for (size_t dword = p.lane; dword < (size_t)p.lane + 16 && dword < bytes; dword += 4)
+                most = std::max(most, dword + p.scalar + 4);
+        }
+    *end = first * pitch + most;
+    return DR_OK;
+}
+
 int dr_cache_update_seq(dr_step_cache* cache, size_t batch, const int32_t* seq, size_t n) {
     if (!cache) return fail(DR_ERR_INVALID, "dr_cache_update_seq: cache is NULL");
     if (batch >= cache->n_batch) return fail(DR_ERR_INVALID, "dr_cache_update_seq: batch %zu >= %zu", batch, cache->n_batch);

@@ -432,6 +432,15 @@ struct MxRows {
 constexpr size_t mx_pitch(size_t cols) { return (cols / 32 + 3) / 4 * 4; }
 constexpr size_t mx_row_bytes(int format, size_t cols) { return format == MX_E2M1 ? cols / 2 : cols; }
 
+// The offsets at which mx_tile_kernel asks for the 16 scale bytes of chunk c (512 columns) of
+// row `row` of a buffer of scale rows: per lane, which the buffer's range check covers dword by
+// dword, and scalar, which it does not.  A chunk may reach past its row, so the scalar offset has
+// to be 0: behind the last row lies memory that is not the caller's.
+struct MxScalePiece {
+    int lane, scalar;
+};
+__host__ __device__ constexpr MxScalePiece mx_scale_piece(int row, int pitch, int c) { return {row * pitch + c * 16, 0}; }
+
 // dr_mx_quantize, dr_mx_dequantize
 struct MxConvertArgs {
     const void* x;  // quantise: the rows, x_stride elements apart

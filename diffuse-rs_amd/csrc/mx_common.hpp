@@ -176,7 +176,8 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_rsrc(const void* base, si
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, (int)bytes, 0x00020000);
 }
 // lane i: 16 (4) bytes at rsrc + voff + soff -> LDS byte address lds + 16 (4) i; 0 where voff
-// lies past the buffer's end.  Inline asm without outputs, so that the compiler does not
+// lies past the buffer's end (dword by dword; the range check leaves soff out, so a lane whose
+// own bytes may end before voff + soff + 16 must not ask).  Inline asm without outputs, so that the compiler does not
 // make every LDS read wait for it; the kernels' own waits order them.  (M0 needs a wait
 // state; nothing else here uses it.)
 __device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t r, uint32_t lds, int voff, int soff) {

@@ -152,12 +152,12 @@ __global__ __launch_bounds__(G::THREADS, G::PER_SIMD) void mx_tile_kernel(const 
         ba[k] = AF == MX_E4M3 ? c >> 1 : c;
     }
     // scales: 64 rows an instruction, the weight groups' and then the activations'
-    int vs[G::NI_S];
+    int row_s[G::NI_S];
 #pragma unroll
     for (int k = 0; k < G::NI_S; ++k) {
         const int j = wave * G::NI_S + k, R = lane & 15, i = lane >> 4;
-        vs[k] = j < G::NSW ? (group_col(j) + 16 * (R >> 2) + 4 * i + (R & 3)) * pitch : ((j - G::NSW) * 64 + lane) * pitch;
-        if (j >= G::NSW && (j - G::NSW) * 64 + lane >= G::BN) vs[k] = OUT_OF_RANGE;  // (every wave issues the same number)
+        row_s[k] = j < G::NSW ? group_col(j) + 16 * (R >> 2) + 4 * i + (R & 3) : (j - G::NSW) * 64 + lane;
+        if (j >= G::NSW && row_s[k] >= G::BN) row_s[k] = -1;  // (every wave issues the same number)
         const uint8_t* const base = j >= G::NSW ? a.act.scales : G::GATED && (j & 1) ? a.up.scales : a.w.scales;
         rs[k] = tile_rsrc(base + (size_t)(j >= G::NSW ? tok0 : col0) * pitch, (size_t)(j >= G::NSW ? toks_in : cols_in) * pitch);
     }
@@ -173,8 +173,10 @@ __global__ __launch_bounds__(G::THREADS, G::PER_SIMD) void mx_tile_kernel(const 
     };
     auto request_scales = [&](int c, uint32_t at) __attribute__((always_inline)) {  // of chunk c
 #pragma unroll
-        for (int k = 0; k < G::NI_S; ++k)
-            dma16(rs[k], at + (wave * G::NI_S + k) * 1024, 16 * c < nblk ? vs[k] : OUT_OF_RANGE, c * 16);
+        for (int k = 0; k < G::NI_S; ++k) {
+            const MxScalePiece p = mx_scale_piece(row_s[k], pitch, c);
+            dma16(rs[k], at + (wave * G::NI_S + k) * 1024, row_s[k] >= 0 && 16 * c < nblk ? p.lane : OUT_OF_RANGE, p.scalar);
+        }
     };
     const int wm = wave % G::WM, wn = wave / G::WM;
     f32x4m acc[Q][4][TN] = {};

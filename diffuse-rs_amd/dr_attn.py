@@ -190,6 +190,7 @@ _SIGS = {
     "dr_debug_ring_tiles": (_I, [_SZ, _SZ, _SZ, ctypes.c_longlong, ctypes.c_longlong, ctypes.c_longlong, _SZ,
                                  ctypes.POINTER(_I), ctypes.POINTER(_I), ctypes.POINTER(_I)]),
     "dr_debug_mx_plan": (_I, [_I, _I, _I, _SZ, _SZ, _SZ, _I, ctypes.POINTER(_I)]),
+    "dr_debug_mx_scale_end": (_I, [_SZ, _SZ, c_size_p]),
     "dr_debug_qmm_plan": (_I, [_I, _SZ, _SZ, _SZ, _I, ctypes.POINTER(_I), c_size_p, c_size_p]),
 }
 
@@ -784,3 +785,11 @@ def mx_plan(rows: int, cols: int, n: int, gated: bool = False, act_format: int =
     k = ctypes.c_int()
     _check(load().dr_debug_mx_plan(1 if gated else 0, act_format, dtype, rows, cols, n, n_cu, ctypes.byref(k)))
     return k.value
+
+
+def mx_scale_end(rows: int, cols: int) -> int:
+    """Where the last byte ends that the products' tiles ask for in a plane of scale rows
+    (dr_debug_mx_scale_end); host-only."""
+    end = ctypes.c_size_t()
+    _check(load().dr_debug_mx_scale_end(rows, cols, ctypes.byref(end)))
+    return end.value
