@@ -1384,7 +1384,7 @@ int dr_debug_mx_plan(int gated, int act_format, int dtype, size_t rows, size_t c
     DR_CHECK(mx_cols(who, "cols", cols));
     if (!kernel || n_cu <= 0 || rows == 0 || n == 0 || rows > MX_ROWS || n > MX_ROWS)
         return fail(DR_ERR_INVALID, "%s: bad sizes, compute units or NULL kernel", who);
-    *kernel = dr::mx_plan(gated != 0, act_format == DR_MX_E4M3 && !gated && dtype == DR_DTYPE_F32, (int)rows, (int)cols, (int)n, n_cu);
+    *kernel = dr::mx_plan(gated != 0, act_format == DR_MX_E4M3 && (gated || dtype == DR_DTYPE_F32), (int)rows, (int)cols, (int)n, n_cu);
     return DR_OK;
 }
 

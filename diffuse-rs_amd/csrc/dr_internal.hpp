@@ -499,6 +499,7 @@ enum MxKernel : int {
     MX_KERNEL_256x128 = 8,
     MX_KERNEL_256x256 = 9,
 };
+// exact: 8 bit activations whose sums keep f32's bits (f32 outputs, gated)
 int mx_plan(bool gated, bool exact, int rows, int cols, int n, int n_cu);
 hipError_t launch_mx_tile(int kernel, const MxMatArgs& a, hipStream_t st);
 

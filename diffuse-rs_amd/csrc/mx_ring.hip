@@ -14,11 +14,9 @@
 //
 // EXACT: both operands are turned into bf16, which holds every code times its
 // power of two exactly, and multiplied by the bf16 MFMA, whose sums keep f32's
-// bits: the block-scaled MFMA lines the products of a step up with the largest and
-// drops what lies about 2^19 below it (with 8 bit codes: relative errors of 4e-6 to
-// 5e-5 against 1e-7, measured over 4096 columns; none with 4 bit codes, whose
-// products span less).  Taken for f32 outputs, and wherever the conversions hide
-// behind the loads.  A product does not depend on the order of the columns, so
+// bits, where the block-scaled MFMA drops some of 8 bit codes' (mx_split: over 4096 columns
+// relative errors of 4e-6 to 5e-5 against 1e-7).  Taken for f32 outputs of 8 bit codes, and wherever
+// the conversions hide behind the loads.  A product does not depend on the order of the columns, so
 // the MFMA's k index is whatever both operands agree on: lane group g takes block g
 // of a step's four, and instruction j multiplies the blocks' values 8 j .. 8 j + 7.
 #include <climits>
@@ -200,7 +198,17 @@ __global__ __launch_bounds__(64 * G::WAVES) void mx_ring_kernel(const MxMatArgs 
                         const u32x4m &lo = ca[s][j][0], &hi = ca[s][j][AF == MX_E4M3 ? 1 : 0];
                         const i32x8m o = AF == MX_E4M3 ? i32x8m{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]}
                                                        : i32x8m{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], 0, 0, 0, 0};
-                        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(ow, o, acc[i][j], 4, AF == MX_E4M3 ? 0 : 4, 0, sw[s][i], 0, sa[s][j]);
+                        auto add = [&](const i32x8m& x) __attribute__((always_inline)) {
+                            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(ow, x, acc[i][j], 4, AF == MX_E4M3 ? 0 : 4, 0, sw[s][i], 0, sa[s][j]);
+                        };
+                        if constexpr (G::GATED && AF == MX_E4M3) {
+                            i32x8m large, small;
+                            mx_split(o, large, small);  // (once for all weight tiles)
+                            add(large);
+                            add(small);
+                        } else {
+                            add(o);
+                        }
                     }
                 }
             }
@@ -353,16 +361,19 @@ hipError_t launch(int kernel, const MxMatArgs& a, hipStream_t st) {
 //   16 x 32                2500    90   4096 x 4096, 32 rows 5.5 us, 4096 x 12288 10.7
 //   32 x 32                2500   110   (gated 200) 64 rows 6.3 and 13.1; 12288 x 4096 gated, 32 rows 15.3
 //   64 x 32                2500   170   (bf16 MFMA 185) 128 rows 8.1 and 18.3 (32 x 32: 9.4 and 22.4; 64 x 64: 9.5 and 21)
-//   64 x 64, bf16 MFMA     2500   340   f32 sums of 8 bit codes; 256 rows 13.5 and 30
+//   64 x 64, bf16 MFMA     2500   340   f32 outputs of 8 bit codes; 256 rows 13.5 and 30
 //   64 x 64                2500   220   256 rows 9.7 and 21.2
 //   64 x 128               4500   285   512 rows 13.3 and 31.4 (64 x 64: 17.6 and 40.6)
-//   64 x 64 gated, 2 a CU  2500   500   (385 where one is enough) 12288 x 4096, 128 rows 19.1 us, 64 rows 14.9
-//   64 x 128 gated, 2 a CU 2500   880   (490 where one is enough) 512 rows 49, 256 rows 29, 128 rows 17.8
-//   256 x 128              4000   880   (gated: 128 output columns; 700 where at most 3/4 of the CUs have
-//                                       one) 2048 rows 33 and 81, 1024 rows 26 and 65; gated 256 rows 27
+//   256 x 128              4000   880   (700 where at most 3/4 of the CUs have one) 2048 rows 33 and 81, 1024 rows 26 and 65
 //   256 x 256              8000  1350   4096 x 12288, 4096 rows 155
-// Both sides of a step: 12288 x 4096 gated, 256 rows: 256 x 128 27 us, 256 x 256 44,
-// 64 x 128 29, 64 x 64 34; 2048 rows: 173, 156, 184, 222.
+// gated, 4 bit codes (fitted to 8 bit ones in one part), and 8 bit codes, whose products are
+// two MFMAs; 12288 x 4096, 8 bit:
+//   64 x 64, 2 a CU        2500   500   760 (385, 550 where one is enough) 128 rows 26.8 us, 64 rows 20.1
+//   64 x 128, 2 a CU       2500   880  1420 (490, 900 + 910 where one is enough) 512 rows 78, 256 rows 47, 128 rows 31.6
+//   256 x 128              4000   880  1400 (128 output columns; 700, 1210 where at most 3/4 of the CUs have one) 256 rows 47
+//   256 x 256              8000  1350  2400
+// Both sides of a step: 256 rows: 256 x 128 46.7 us, 256 x 256 85, 64 x 128 46.7, 64 x 64 43.5; 1024 rows:
+// 256 x 128 149, 256 x 256 171; 2048 rows: 295, 272; 4096 x 2048, 128 rows: 32 x 32 8.4, 64 x 64 11.0.
 int mx_plan(bool gated, bool exact, int rows, int cols, int n, int n_cu) {
     if (n <= 16) return n <= 4 ? MX_KERNEL_4 : MX_KERNEL_16;
     const long steps = (cols + 127) / 128;
@@ -373,7 +384,14 @@ int mx_plan(bool gated, bool exact, int rows, int cols, int n, int n_cu) {
         const long t = start + (tiles(columns, acts) + (long)per_cu * n_cu - 1) / ((long)per_cu * n_cu) * steps * step;
         if (t < least) least = t, best = kernel;
     };
-    if (gated) {
+    if (gated && exact) {
+        const bool one = tiles(64, 128) <= n_cu;
+        offer(MX_KERNEL_32x32, 32, 32, 1, 2500, 200);
+        offer(MX_KERNEL_64x64, 64, 64, 2, 2500, tiles(64, 64) <= n_cu ? 550 : 760);
+        offer(MX_KERNEL_64x128, 64, 128, 2, one ? 900 : 2500, one ? 910 : 1420);
+        offer(MX_KERNEL_256x128, 128, 128, 1, 4000, 4 * tiles(128, 128) <= 3 * n_cu ? 1210 : 1400);
+        offer(MX_KERNEL_256x256, 128, 256, 1, 8000, 2400);
+    } else if (gated) {
         offer(MX_KERNEL_32x32, 32, 32, 1, 2500, 200);
         offer(MX_KERNEL_64x64, 64, 64, 2, 2500, tiles(64, 64) <= n_cu ? 385 : 500);
         offer(MX_KERNEL_64x128, 64, 128, 2, 2500, tiles(64, 128) <= n_cu ? 490 : 880);
@@ -398,10 +416,11 @@ int mx_plan(bool gated, bool exact, int rows, int cols, int n, int n_cu) {
 hipError_t launch_mx_matmul(const MxMatArgs& a, hipStream_t st) {
     if (a.n <= 0 || a.rows <= 0) return hipSuccess;
     const bool eight = a.act.format == MX_E4M3;
-    // f32 sums of 8 bit codes stay on the bf16 MFMA; so do bf16 sums and the gated block up
-    // to 16 rows, where the conversions hide behind the weights.
+    // f32 outputs of 8 bit codes stay on the bf16 MFMA; so do bf16 outputs and the gated block up
+    // to 16 rows, where the conversions hide behind the weights.  The gated block of more rows
+    // multiplies 8 bit codes in two parts (mx_split).
     const bool exact = eight && !a.gated && !a.bf16;
-    const int kernel = mx_plan(a.gated, exact, a.rows, a.cols, a.n, a.n_cu);
+    const int kernel = mx_plan(a.gated, eight && (a.gated || !a.bf16), a.rows, a.cols, a.n, a.n_cu);
     if (kernel > MX_KERNEL_64x64_EXACT) return launch_mx_tile(kernel, a, st);
     if (!eight) return launch<MX_E2M1, false>(kernel, a, st);
     if (exact || kernel <= MX_KERNEL_16) return launch<MX_E4M3, true>(kernel, a, st);

@@ -17,7 +17,10 @@
 // between its products: all of it at the start of a stage, the address unit kept the
 // products waiting.
 //
-// 4096 rows through 4096 x 12288, bf16: 150-157 us (2.7 PFLOP/s); 2 x 12288 x 4096 gated 300-310;
+// Gated, 8 bit activations: in two parts (mx_split), whose MFMAs bound it.
+//
+// 4096 rows through 4096 x 12288, bf16: 147-155 us (2.7 PFLOP/s); 2 x 12288 x 4096 gated 525-545 (twice
+// 1.5 PFLOP/s; in one part 300, with 1 of 1000 codes on the other side of a border);
 // 4 bit activations, 2553 rows through 18944 x 3584, 120-124.  The matrix instruction alone
 // reaches 4.2 PFLOP/s on such codes (7.1 with 4 bit ones), at 2.0 GHz, which is what power
 // leaves; a large library product of 8 bit numbers 2.9.  The matrix cores are busy 70 % of
@@ -38,7 +41,7 @@ namespace {
 template <int AF_, bool GATED_, int WM_, int Q_, int WN_, int TN_, int SB_, int STAGES_>
 struct TileGeom {
     static constexpr int AF = AF_, WM = WM_, Q = Q_, WN = WN_, TN = TN_, SB = SB_, STAGES = STAGES_;
-    static constexpr bool GATED = GATED_;
+    static constexpr bool GATED = GATED_, SPLIT = GATED && AF == MX_E4M3;  // (mx_split)
     static constexpr int WAVES = WM * WN, THREADS = 64 * WAVES;
     static constexpr int GROUPS = WM * Q;                       // of 64 weight rows
     static constexpr int COLS = GROUPS * 64 / (GATED ? 2 : 1);  // output columns
@@ -222,6 +225,14 @@ __global__ __launch_bounds__(G::THREADS, G::PER_SIMD) void mx_tile_kernel(const 
         f32x4m& d = acc[n / 4][n % 4][j];
         d = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, o, d, 4, AF == MX_E4M3 ? 0 : 4, BYTE, sw[n], BYTE, sa[j]);
     };
+    // an activation operand as the MFMA takes it
+    constexpr int P = G::SPLIT ? 2 : 1;
+    auto parts = [&](const i32x8m& c, i32x8m (&o)[P]) __attribute__((always_inline)) {
+        if constexpr (G::SPLIT)
+            mx_split(c, o[0], o[1]);
+        else
+            o[0] = c;
+    };
     // The products of a stage, the first of whose 128 columns are number PART of the
     // chunk's; between them `more` (of 4 Q a step) of the DMA of a later one.
     auto multiply = [&](auto part, const uint8_t* st, auto&& more) __attribute__((always_inline)) {
@@ -241,18 +252,23 @@ __global__ __launch_bounds__(G::THREADS, G::PER_SIMD) void mx_tile_kernel(const 
                 if constexpr (S + 1 < G::SB) load(S + 1);
 #pragma unroll
                 for (int n = 0; n < 4 * Q; ++n) more(S * 4 * Q + n);
+                i32x8m op[TN][P];
+#pragma unroll
+                for (int j = 0; j < TN; ++j) parts(o[S & 1][j], op[j]);
 #pragma unroll
                 for (int n = 0; n < 4 * Q; ++n)
 #pragma unroll
-                    for (int j = 0; j < TN; ++j) mfma(Int<PART + S>{}, w[S & 1][n], o[S & 1][j], n, j);
+                    for (int p = 0; p < P; ++p)
+#pragma unroll
+                        for (int j = 0; j < TN; ++j) mfma(Int<PART + S>{}, w[S & 1][n], op[j][p], n, j);
                 __builtin_amdgcn_sched_barrier(0);
             });
         } else {
             static_for<G::SB>([&](auto step) __attribute__((always_inline)) {
                 constexpr int S = decltype(step)::value;
-                i32x8m o[TN], w = weights(st, S, 0);
+                i32x8m o[TN][P], w = weights(st, S, 0);
 #pragma unroll
-                for (int j = 0; j < TN; ++j) o[j] = acts(st, S, j);
+                for (int j = 0; j < TN; ++j) parts(acts(st, S, j), o[j]);
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int n = 0; n < 4 * Q; ++n) {
@@ -260,7 +276,9 @@ __global__ __launch_bounds__(G::THREADS, G::PER_SIMD) void mx_tile_kernel(const 
                     if (n + 1 < 4 * Q) next = weights(st, S, n + 1);
                     more(S * 4 * Q + n);
 #pragma unroll
-                    for (int j = 0; j < TN; ++j) mfma(Int<PART + S>{}, w, o[j], n, j);
+                    for (int p = 0; p < P; ++p)
+#pragma unroll
+                        for (int j = 0; j < TN; ++j) mfma(Int<PART + S>{}, w, o[j][p], n, j);
                     w = next;
                     __builtin_amdgcn_sched_barrier(0);  // or all the DMA would come before all the products
                 }
@@ -335,7 +353,7 @@ __global__ __launch_bounds__(G::THREADS, G::PER_SIMD) void mx_tile_kernel(const 
                 uint32_t m = 0;
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                    const float v = mx_act_fast(acc[q][e / 4][j][e % 4], a.fn) * acc[q + 1][e / 4][j][e % 4];
+                    const float v = mx_act(acc[q][e / 4][j][e % 4], a.fn) * acc[q + 1][e / 4][j][e % 4];
                     x[e / 8][e % 8] = v;
                     m = max(m, __float_as_uint(v) & 0x7fffffffu);
                 }
@@ -372,9 +390,9 @@ template <int AF, bool GATED>
 hipError_t tiles(int kernel, const MxMatArgs& a, hipStream_t st) {
     constexpr bool EIGHT = AF == MX_E4M3;
     // Where no CU gets a second tile, a tile takes the LDS of two.  Weights that no cache holds,
-    // gated, 64 x 64 tiles: 64 rows through 12288 x 4096 17.4 us (two stages 23.3; 128 rows, two
-    // tiles a CU, 29.4 and 26.2), 64 x 128: 128 rows 22.6 (26.4; 512 rows 58 and 54).  Products, 64
-    // x 64: 256 rows through 4096 x 12288 27.0 (four stages of half as many columns 29.5).
+    // gated, 8 bit codes, 64 x 64 tiles: 64 rows through 12288 x 4096 20.6 us (two stages 25.7; 128 rows,
+    // two tiles a CU, 36.9 and 30.3), 64 x 128: 128 rows 32.9 (32.4; 512 rows 94 and 80; in one part, as 4
+    // bit codes, 22.6 and 26.4, 58 and 54).  Products, 64 x 64: 256 rows through 4096 x 12288 27.0 (four stages of half as many columns 29.5).
     auto one = [&](int columns, int acts) { return ((a.rows + columns - 1) / columns) * (long)((a.n + acts - 1) / acts) <= a.n_cu; };
     switch (kernel) {
         case MX_KERNEL_64x64:
