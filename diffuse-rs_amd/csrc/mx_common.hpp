@@ -169,7 +169,7 @@ using i32x8m = int __attribute__((ext_vector_type(8)));
 // 2^-2, so nothing is dropped.  E4M3 codes go through in two parts that keep theirs too: those
 // of 2 and more (bit 6; products of 2^10 to a multiple of 2^-3) and those below
 // (of 2^2 to a multiple of 2^-10), with 0 in the others' places.  Random codes and blocks: each part's
-// sums equal the exact ones; in one part they are off by up to 8e-5 of the sum of magnitudes.
+// sums equal the exact ones; in one part they are off by up to 1e-4 of the sum of magnitudes.
 __device__ __forceinline__ void mx_split(const i32x8m& c, i32x8m& large, i32x8m& small) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
