@@ -59,7 +59,7 @@ __global__ __launch_bounds__(256) void mx_dequantize_kernel(const MxConvertArgs 
 }
 
 // The root of a row's mean square: sums of eight f32 squares are added in 64 bits
-// (as the reference sums them), so that the factor is off by its own rounding alone:
+// (the reference adds f32 squares in 64 bits one by one), so that the factor is off by its own rounding alone:
 // an f32 sum's few 2^-24 move ten times as many values past a border between codes.
 template <int WAVES>
 __device__ __forceinline__ float row_factor(double ss, double (&part)[WAVES], const MxNormArgs& a) {

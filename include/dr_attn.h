@@ -542,7 +542,9 @@ int dr_mx_dequantize(dr_ctx* ctx, const dr_mx_rows* rows, size_t n, size_t cols,
  * makes before each block's projections.  x, residual and sum are dtype
  * (DR_DTYPE_F32 or _BF16); x has rows x_stride elements apart (0: cols), residual
  * and sum are [n][cols]; sum may be x (then x_stride is cols) or residual.  The
- * squares of the held h are summed in 64 bits by eights. */
+ * squares of the held h are f32, as the reference's, and summed in 64 bits by eights:
+ * a row whose eight squares pass f32's largest (values of 6e18 to 1.8e19 and more) comes out as
+ * zeros, and with eps 0 rows of values below 1e-16 or so lose digits of their factor. */
 int dr_rms_norm_mx(dr_ctx* ctx, const void* x, const void* residual, void* sum, int dtype, size_t n, size_t cols,
                    size_t x_stride, const float* w, float eps, const dr_mx_rows* out);
 
