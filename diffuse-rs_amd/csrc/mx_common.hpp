@@ -223,9 +223,11 @@ __device__ __forceinline__ int xcd_order(int id, int total) {
 
 // 16-byte piece c of row R of a staged tile lies at slot c ^ turn(R), so that a read of
 // one piece per lane group of 16 rows, or (PAIRS, 128-byte rows) of one of two that
-// belong together, touches every bank once (SQ_LDS_BANK_CONFLICT is 0; a read serves
-// lanes 0-3, 12-15 and 20-27 at a time, so rows 0-3 and 12-15 of a group meet rows 4-11
-// of the next).  ROW: bytes of a row, 64, 128 or more.
+// belong together, touches every bank once (a read serves lanes 0-3, 12-15 and 20-27 at a
+// time, so rows 0-3 and 12-15 of a group meet rows 4-11 of the next): SQ_LDS_BANK_CONFLICT is 0
+// in the tiles' kernels.  The ring kernels have some: where 4 activation rows are staged, two of
+// them meet in a bank (16 cycles of a step's 48 of LDS; loads bound it), and the sums are
+// written over rows of 20 floats.  ROW: bytes of a row, 64, 128 or more.
 template <int ROW, bool PAIRS = false>
 __device__ __forceinline__ int turn(int R) {
     if (ROW == 64) return (R >> 1) & 3;

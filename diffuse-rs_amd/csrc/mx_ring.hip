@@ -13,7 +13,8 @@
 // nobody but its own loads and meets the others once, at the end.
 //
 // EXACT: both operands are turned into bf16, which holds every code times its
-// power of two exactly, and multiplied by the bf16 MFMA, whose sums keep f32's
+// power of two exactly (blocks of scale bytes 3 to 246; below, 8 bit codes' values can lie
+// under its smallest number, and above, the largest codes become infinite), and multiplied by the bf16 MFMA, whose sums keep f32's
 // bits, where the block-scaled MFMA drops some of 8 bit codes' (mx_split: over 4096 columns
 // relative errors of 4e-6 to 5e-5 against 1e-7).  Taken for f32 outputs of 8 bit codes, and wherever
 // the conversions hide behind the loads.  A product does not depend on the order of the columns, so
@@ -317,8 +318,10 @@ hipError_t launch(int kernel, const MxMatArgs& a, hipStream_t st) {
     // 7.2, 16 rows 12.7 and 8.2; two places 13.2, 7.3, 15.9 and 8.7: fewer workgroups fit on a
     // CU.  Where no CU gets a second workgroup and there
     // are steps for all, twice the waves keep as many bytes under way as two would.  With weights
-    // that no cache holds: one row through 3584 x 18944 9.2 us (8 waves 12.0), 2048 x 8192 5.5
-    // (6.3), 2 x 4096 x 4096 7.8 (4 waves 9.4), 2 x 8192 x 4096 9.6 (11.6); with more columns
+    // that no cache holds: one row through 3584 x 18944 9.5 us (8 waves 11.9; 10.3 and 11.0 on another
+    // day), 4096 x 12288 7.8 (8.7), 2048 x 8192 5.5 (6.3); held by the memory-side cache 8.7 (9.0; 8.5 and 8.2),
+    // 7.2 (7.1) and 5.0 (4.8): a layer's weights come from memory.  2 x 4096 x 4096, from
+    // memory, 7.8 (4 waves 9.4), 2 x 8192 x 4096 9.6 (11.6); with more columns
     // they take away workgroups instead, 2 x 9216 x 4096 16 rows 17.3 (15.7), one row 5120 x 8192
     // 9.1 (8.3), and with fewer steps they have none, 2 x 1024 x 1024 4.2 (4.0).
     if constexpr (X || AF == MX_E2M1) {

@@ -557,7 +557,8 @@ int dr_rms_norm_mx(dr_ctx* ctx, const void* x, const void* residual, void* sum, 
  * is 2^-13 of the power of two of the largest; what the others have below it is dropped.  Such a
  * sum is off by at most 2^-10 of its products' sum of magnitudes, a quarter of what bf16 rounds a number by;
  * measured on random codes up to 1e-4, and against the sums themselves 4e-6 to 5e-5.  Values
- * below 2^-126 may count as 0. */
+ * below 2^-126 may count as 0, values past f32's largest (8 bit blocks of scale byte 247 and more,
+ * 4 bit ones of 253) as infinities. */
 int dr_mx_matmul(dr_ctx* ctx, const dr_mx_rows* w, size_t rows, size_t cols, const dr_mx_rows* act, size_t n,
                  void* out, const void* residual, int dtype);
 

@@ -82,3 +82,29 @@ def test_what_bf16_outputs_lose(dev, n, rows, cols):
     beyond = np.maximum(err - 2.0**-8 * (np.abs(s) + tol), 0)
     say(f"  largest error beside the rounding {float((beyond / p).max()):.3g} of the sum of magnitudes")
     assert (beyond <= tol).all()
+
+
+@pytest.mark.parametrize("fmt", list(FMTS))
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+@pytest.mark.parametrize("n", [1, 16, 20, 300])
+def test_ends_of_the_scales(dev, fmt, bf16, n):
+    """Largest codes at the largest scale whose values are f32 numbers, and values down to 2^-126, times weights of the other end."""
+    fmt = FMTS[fmt]
+    rng = np.random.default_rng(n)
+    rows, cols = 48, 160
+    top, most, low = (246, 448.0, 10) if fmt == dr.MX_E4M3 else (252, 6.0, 2)  # (smallest codes 2^-9 and 2^-1)
+    for byte, weight_byte in ((top, 20), (low, 220)):
+        av = np.where(rng.random((n, cols)) < 0.5, most, 1.0) * rng.choice([1, -1], (n, cols))
+        if byte == low:
+            av[:, ::7] = 2.0**-9 if fmt == dr.MX_E4M3 else 0.5
+        wv = rng.choice([0.5, 1, -1.5, 2, -3, 6, 0], (rows, cols))
+        a, w = rows_of(av, fmt, byte), rows_of(wv, dr.MX_E2M1, weight_byte)
+        x, y = mx.values(*a, fmt, cols), mx.values(*w, dr.MX_E2M1, cols)
+        s, p = x @ y.T, np.abs(x) @ np.abs(y).T
+        out = put(dev, np.zeros(n * rows, np.float32), bf16)
+        dr.mx_matmul(dev.ctx, put_rows(dev, *w, dr.MX_E2M1), rows, cols, put_rows(dev, *a, fmt), n, out,
+                     dtype=dr.DTYPE_BF16 if bf16 else dr.DTYPE_F32)
+        lossy = bf16 and fmt == dr.MX_E4M3 and n > 16
+        tol = (4 * np.sqrt(cols) * 2.0**-23 + (2.0**-10 if lossy else 0)) * p
+        err = np.abs(get(dev, out, bf16).reshape(n, rows) - s)
+        assert (err <= tol + (2.0**-8 if bf16 else 2.0**-24) * (np.abs(s) + tol)).all(), byte
