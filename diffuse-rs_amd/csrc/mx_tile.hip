@@ -19,7 +19,7 @@
 //
 // Gated, 8 bit activations: in two parts (mx_split), whose MFMAs bound it.
 //
-// 4096 rows through 4096 x 12288, bf16: 147-155 us (2.7 PFLOP/s); 2 x 12288 x 4096 gated 525-545 (twice
+// 4096 rows through 4096 x 12288, bf16: 147-155 us (2.7 PFLOP/s); 2 x 12288 x 4096 gated 525-560 (twice
 // 1.5 PFLOP/s; in one part 300, with 1 of 1000 codes on the other side of a border);
 // 4 bit activations, 2553 rows through 18944 x 3584, 120-124.  The matrix instruction alone
 // reaches 4.2 PFLOP/s on such codes (7.1 with 4 bit ones), at 2.0 GHz, which is what power
