@@ -690,7 +690,7 @@ int dr_debug_qmm_plan(int wtype, size_t rows, size_t cols, size_t n, int n_cu, i
  * and 256 x 256 weight by activation rows.  Host-only. */
 int dr_debug_mx_plan(int gated, int act_format, int dtype, size_t rows, size_t cols, size_t n, int n_cu, int* kernel);
 
-/* Where the last byte ends that the tiles' kernel (2 to 9 above that are no strips) asks for in a
+/* Where the last byte ends that the kernels of the largest tiles (6 to 9 above) ask for in a
  * plane of scale rows, from the kernel's own offsets: rows * ceil(cols / 32 / 4) * 4 at most.
  * Host-only. */
 int dr_debug_mx_scale_end(size_t rows, size_t cols, size_t* end);
